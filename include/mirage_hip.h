@@ -193,6 +193,70 @@ typedef struct mrg_rowfuse_desc {
 int mrg_rowfuse_fwd(const mrg_rowfuse_desc* d, hipStream_t stream);
 
 /* ---------------------------------------------------------------------------------------------------
+ * Rotary positions with several axes, csrc/rotary.hip (next to the fixed sin-cos tables of mirage/utils.py:24-41): q [B, N, Hq, hd] and
+ * k [B, N, Hk, hd] turned pair by pair by pos[b, n, axis(p)] * freqs[p]; batch / row / head strides in elements, the head itself contiguous.
+ * sections[a] = pairs of axis a (their sum P <= hd / 2); pairing: HALF (p, p + P), INTERLEAVED (2p, 2p + 1), AXIAL (half inside the axis' own
+ * 2 sections[a] elements).  Elements behind the 2 P turned ones are copied.  inverse: by -theta (the gradient).  Outputs may be the inputs
+ * (same pointer and strides); any other overlap is not allowed.  Hk = 0 or Hq = 0: that side is absent. */
+#define MRG_MAX_AXES 3
+enum { MRG_POS_I32 = 0, MRG_POS_F32 = 1 };
+enum { MRG_PAIR_HALF = 0, MRG_PAIR_INTERLEAVED = 1, MRG_PAIR_AXIAL = 2 };
+typedef struct mrg_rotary_desc {
+    const void* q; const void* k; void* q_out; void* k_out;
+    long q_bs, q_rs, q_hs, k_bs, k_rs, k_hs, qo_bs, qo_rs, qo_hs, ko_bs, ko_rs, ko_hs;
+    int dtype, B, N, Hq, Hk, head_dim;
+    int pos_dtype; const void* pos; long pos_bs, pos_rs;   /* positions [B, N, axes], the axes contiguous (pos_bs = 0: shared by the batch) */
+    const double* freqs;                                   /* [P] radians per position unit */
+    int axes, sections[MRG_MAX_AXES], pairing, inverse;
+} mrg_rotary_desc;
+int mrg_rotary_axes(const mrg_rotary_desc* d, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------------------------------
+ * Norm behind a branch, gate, scaled residual and norm in front of the next branch in one pass, csrc/resid_norm.hip (next to mrg_ln_fwd / bwd):
+ *   n = Norm_post(branch);  x_new = alpha x + gate n;  y = Norm_pre(x_new).   Rows contiguous, 16-byte aligned, D % 4 == 0, D <= 4096.
+ * gate fp32 [gate_rows, D]: 0 rows = none, 1 = one for all, `samples` = one per sample of rows_per_sample rows.  A norm is absent when its
+ * weight is NULL (pre_w NULL: no y); its bias is optional.  stats fp32 [4][samples * rows_per_sample], kept for the backward pass.
+ *   bwd: dx_new fp32, dy (y_dtype) -> dx fp32, dbranch (branch_dtype), and the fp32 gradients of every vector that is given; ws: workspace of
+ *   mrg_resid_norm_ws_floats(d) floats. */
+enum { MRG_NORM_LAYER = 0, MRG_NORM_RMS = 1 };
+typedef struct mrg_resid_norm_desc {
+    int samples, rows_per_sample, D, norm, branch_dtype, y_dtype, gate_rows; float alpha, eps;
+    const float* x; const void* branch; const float* gate;
+    const float* post_w; const float* post_b; const float* pre_w; const float* pre_b;
+    float* x_new; void* y; float* stats;
+    const float* dx_new; const void* dy; float* dx; void* dbranch;
+    float* d_gate; float* d_post_w; float* d_post_b; float* d_pre_w; float* d_pre_b; float* ws;
+} mrg_resid_norm_desc;
+int mrg_resid_norm_fwd(const mrg_resid_norm_desc* d, hipStream_t stream);
+long mrg_resid_norm_ws_floats(const mrg_resid_norm_desc* d);
+int mrg_resid_norm_bwd(const mrg_resid_norm_desc* d, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------------------------------
+ * Softmax attention whose scores are modified, csrc/attention_mod.hip (next to mrg_attn_fwd / bwd, which keep the unmodified short rows):
+ *   s = scale q.k;  cap > 0: s = cap tanh(s / cap);  slopes: s -= slopes[h] sum_a |pos_q[b, i, a] - pos_k[b, j, a]|
+ *   visible (i, j):  doc_q[b, i] == doc_k[b, j] >= 0 (documents given)  and  j < max(prefix[b], i + Nk - Nq + 1) (causal)
+ * A row that sees nothing gives o = 0, lse = -inf and no gradient.  bf16, head_dim 32 or 64; H query heads share Hk key / value heads (H a
+ * multiple of Hk: head h reads h / (H / Hk)).  *_bs / *_rs / *_hs: batch, row and head strides in elements.  Rows whose document is negative
+ * are never read as keys; values behind a mask do not reach the result even when they are not finite.
+ *   fwd: o, lse fp32 [B, H, Nq] (may be NULL);  ws: mrg_attn_mod_ws_bytes(d, 0) bytes.
+ *   bwd: reads o, lse, d_o;  writes dq, dk, dv;  ws: mrg_attn_mod_ws_bytes(d, 1) bytes. */
+typedef struct mrg_attn_mod_desc {
+    const void* q; const void* k; const void* v; void* o; float* lse;
+    long q_bs, q_rs, q_hs, k_bs, k_rs, k_hs, v_bs, v_rs, v_hs, o_bs, o_rs, o_hs;
+    int B, H, Hk, Nq, Nk, head_dim; float scale, cap;
+    const float* slopes; const float* pos_q; const float* pos_k; int axes;   /* pos [B, N, axes] contiguous, one batch row after the other */
+    const int* doc_q; const int* doc_k;                                      /* [B, Nq], [B, Nk] */
+    int causal; const int* prefix;                                           /* prefix [B] or NULL (0) */
+    const void* d_o; long do_bs, do_rs, do_hs;
+    void* dq; void* dk; void* dv;
+    long dq_bs, dq_rs, dq_hs, dk_bs, dk_rs, dk_hs, dv_bs, dv_rs, dv_hs;
+    void* ws;
+} mrg_attn_mod_desc;
+long mrg_attn_mod_ws_bytes(const mrg_attn_mod_desc* d, int backward);
+int mrg_attn_mod_fwd(const mrg_attn_mod_desc* d, hipStream_t stream);
+int mrg_attn_mod_bwd(const mrg_attn_mod_desc* d, hipStream_t stream);
+
+/* ---------------------------------------------------------------------------------------------------
  * Fused softmax attention.  Replaces F.scaled_dot_product_attention (mirage/utils.py:181 self, :216 cross;
  * scale = head_dim^-0.5, no mask, dropout 0) and its backward.  All tensors bf16; *_bs / *_rs are batch / row
  * strides in elements, the head stride is head_dim (heads are adjacent inside a row), so q/k/v may point into the

@@ -83,6 +83,39 @@ class RowFuseDesc(C.Structure):
                 ("w1", vp), ("b1", vp), ("h_out", vp), ("hgrad_out", vp), ("w2", vp), ("b2", vp), ("y32", vp), ("y16", vp)]
 
 
+MRG_MAX_AXES = 3
+MRG_POS_I32, MRG_POS_F32 = 0, 1
+MRG_PAIR_HALF, MRG_PAIR_INTERLEAVED, MRG_PAIR_AXIAL = 0, 1, 2
+MRG_NORM_LAYER, MRG_NORM_RMS = 0, 1
+
+
+class RotaryDesc(C.Structure):
+    _fields_ = [("q", vp), ("k", vp), ("q_out", vp), ("k_out", vp),
+                ("q_bs", cl), ("q_rs", cl), ("q_hs", cl), ("k_bs", cl), ("k_rs", cl), ("k_hs", cl),
+                ("qo_bs", cl), ("qo_rs", cl), ("qo_hs", cl), ("ko_bs", cl), ("ko_rs", cl), ("ko_hs", cl),
+                ("dtype", ci), ("B", ci), ("N", ci), ("Hq", ci), ("Hk", ci), ("head_dim", ci),
+                ("pos_dtype", ci), ("pos", vp), ("pos_bs", cl), ("pos_rs", cl), ("freqs", vp),
+                ("axes", ci), ("sections", ci * MRG_MAX_AXES), ("pairing", ci), ("inverse", ci)]
+
+
+class ResidNormDesc(C.Structure):
+    _fields_ = [("samples", ci), ("rows_per_sample", ci), ("D", ci), ("norm", ci), ("branch_dtype", ci), ("y_dtype", ci), ("gate_rows", ci),
+                ("alpha", cf), ("eps", cf), ("x", vp), ("branch", vp), ("gate", vp), ("post_w", vp), ("post_b", vp), ("pre_w", vp), ("pre_b", vp),
+                ("x_new", vp), ("y", vp), ("stats", vp), ("dx_new", vp), ("dy", vp), ("dx", vp), ("dbranch", vp),
+                ("d_gate", vp), ("d_post_w", vp), ("d_post_b", vp), ("d_pre_w", vp), ("d_pre_b", vp), ("ws", vp)]
+
+
+class AttnModDesc(C.Structure):
+    _fields_ = [("q", vp), ("k", vp), ("v", vp), ("o", vp), ("lse", vp),
+                ("q_bs", cl), ("q_rs", cl), ("q_hs", cl), ("k_bs", cl), ("k_rs", cl), ("k_hs", cl), ("v_bs", cl), ("v_rs", cl), ("v_hs", cl),
+                ("o_bs", cl), ("o_rs", cl), ("o_hs", cl),
+                ("B", ci), ("H", ci), ("Hk", ci), ("Nq", ci), ("Nk", ci), ("head_dim", ci), ("scale", cf), ("cap", cf),
+                ("slopes", vp), ("pos_q", vp), ("pos_k", vp), ("axes", ci), ("doc_q", vp), ("doc_k", vp), ("causal", ci), ("prefix", vp),
+                ("d_o", vp), ("do_bs", cl), ("do_rs", cl), ("do_hs", cl), ("dq", vp), ("dk", vp), ("dv", vp),
+                ("dq_bs", cl), ("dq_rs", cl), ("dq_hs", cl), ("dk_bs", cl), ("dk_rs", cl), ("dk_hs", cl), ("dv_bs", cl), ("dv_rs", cl), ("dv_hs", cl),
+                ("ws", vp)]
+
+
 class AdamWDesc(C.Structure):
     _fields_ = [("p", vp), ("g", vp), ("m", vp), ("v", vp), ("shadow_bf16", vp), ("n", cl), ("n_decay", cl),
                 ("lr_table", vp), ("wd_table", vp), ("step", vp), ("table_len", ci),
@@ -140,6 +173,13 @@ SIGNATURES = {
     "mrg_ln_bwd_partial_rows": (ci, [ci, ci]),
     "mrg_reduce_batch": (ci, [vp, ci, vp]),
     "mrg_rowfuse_fwd": (ci, [C.POINTER(RowFuseDesc), vp]),
+    "mrg_rotary_axes": (ci, [C.POINTER(RotaryDesc), vp]),
+    "mrg_resid_norm_fwd": (ci, [C.POINTER(ResidNormDesc), vp]),
+    "mrg_resid_norm_ws_floats": (cl, [C.POINTER(ResidNormDesc)]),
+    "mrg_resid_norm_bwd": (ci, [C.POINTER(ResidNormDesc), vp]),
+    "mrg_attn_mod_ws_bytes": (cl, [C.POINTER(AttnModDesc), ci]),
+    "mrg_attn_mod_fwd": (ci, [C.POINTER(AttnModDesc), vp]),
+    "mrg_attn_mod_bwd": (ci, [C.POINTER(AttnModDesc), vp]),
     "mrg_augment_image": (ci, [vp, vp, vp, ci, ci, ci, ci, vp]),
     "mrg_augment_label": (ci, [vp, vp, vp, ci, ci, ci, ci, vp]),
     "mrg_resize_image": (ci, [vp, vp, ci, ci, ci, ci, ci, vp]),

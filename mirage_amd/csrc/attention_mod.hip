@@ -1,0 +1,865 @@
+// Softmax attention over long rows with modified scores, forward and backward (bf16, head_dim 32 / 64, shared key heads):
+//     s = scale q.k     cap: s = cap tanh(s / cap)     bias: s -= slope_h sum_a |pos_q[i, a] - pos_k[j, a]|
+//     visible (i, j):  doc_q[i] == doc_k[j] >= 0   and   j < max(prefix, i + Nk - Nq + 1)  when causal
+//     p = softmax over the visible j      o = p v      (a row that sees nothing: o = 0, lse = -inf)
+//     dv = p^T do    dp = do v^T    ds = p (dp - sum(do o)) (1 - tanh^2)    dq = scale ds k    dk = scale ds^T q
+//
+// Layout.  A wave owns 32 rows (queries, or keys in the dk / dv kernel) and multiplies with v_mfma_f32_32x32x16_bf16 so that every LANE owns one
+// of them: S^T = K Q^T leaves lane = query and registers = keys, so row maximum, sum and rescale are lane-local (one exchange between the
+// wave's halves), and the same registers, packed to bf16, are the right operand of the next product (O^T = V^T P^T): its contraction index
+// may come in any order as long as both operands agree, and V^T fragments read from LDS with ds_read_b64_tr_b16 take the accumulator's
+// order.  Scores never leave the registers.  Tiles of 64 keys go global -> registers -> LDS one tile ahead of the products, double-buffered,
+// one barrier per tile.
+//
+// Masks by tiles.  A first small launch leaves the smallest and largest document and the count of valid tokens of every 64-token tile; a
+// workgroup tests 64 tiles at a time (one per lane, one ballot) and walks only tiles that some row of it may see.  Per wave a tile is skipped,
+// whole (no test per score) or partial.  Sums, maxima, lse and all products accumulate in fp32; p and ds are rounded to bf16 as operands of
+// the second products (relative 2^-9 each, averaging over the row), the sum of p is taken before the rounding.
+//
+// Values that are not finite behind a mask: 0 * inf would reach the products, so in partial tiles the rows of the second product's left
+// operand that hold such values are replaced by zeros in LDS and noted; a row that SEES one of them is NaN in full.
+//
+// No atomics on results: dq is owned by queries, dk / dv by keys (the scores are computed twice), split rows are joined in a fixed order.
+#include "common.h"
+#include "mirage_hip.h"
+
+namespace {
+
+constexpr float LOG2E_F = 1.4426950408889634f, LN2_F = 0.6931471805599453f;
+constexpr int TT = 64;                        // tokens of a staged tile
+constexpr int MAX_SPLITS = 64;
+
+struct ModArgs {
+    const bf16_t* q; const bf16_t* k; const bf16_t* v; bf16_t* o; float* lse;
+    long q_bs, q_rs, q_hs, k_bs, k_rs, k_hs, v_bs, v_rs, v_hs, o_bs, o_rs, o_hs;
+    int B, H, Hk, G, Nq, Nk;                  // G = H / Hk
+    float scale, cap;
+    const float* slopes; const float* pos_q; const float* pos_k; int axes;
+    const int* doc_q; const int* doc_k;
+    const int4* tab_q; const int4* tab_k; int ntq, ntk;     // per tile {lowest, highest document, valid tokens}
+    int causal; const int* prefix;
+    const bf16_t* d_o; long do_bs, do_rs, do_hs;
+    bf16_t* dq; bf16_t* dk; bf16_t* dv;
+    long dq_bs, dq_rs, dq_hs, dk_bs, dk_rs, dk_hs, dv_bs, dv_rs, dv_hs;
+    float* dsum;                              // [B, H, Nq] sum(do o)
+    float* part; float* part_ml; int splits;  // split rows: [split][rows][HD] unnormalised, [split][rows][2] {max, sum}
+    int nblk;                                 // row blocks of the owner
+};
+
+// byte offset of 16-byte chunk c of row r in a [TT][HD] bf16 tile; the XOR spreads the rows that one instruction reads over the banks
+template <int HD> __device__ __forceinline__ int toff(int r, int c) {
+    if (HD == 64) return r * 128 + ((c ^ ((r >> 1) & 7)) << 4);
+    return r * 64 + ((c ^ ((r >> 2) & 3)) << 4);
+}
+// operand with the contraction along hd: lane -> row row0 + (lane & 31), chunk 2 kk + (lane >> 5)
+template <int HD> __device__ __forceinline__ bf16x8 frag_row(const char* t, int row0, int kk, int lane) {
+    return *reinterpret_cast<const bf16x8*>(t + toff<HD>(row0 + (lane & 31), 2 * kk + (lane >> 5)));
+}
+// operand with the contraction along the tile's rows in accumulator order (rows base + 0..3, base + 8..11, base = row0 + 16 m + 4 (lane >> 5)),
+// lane -> hd element 32 dj + (lane & 31)
+template <int HD> __device__ __forceinline__ bf16x8 frag_col(uint32_t t, int row0, int m, int dj, int lane) {
+    const int i = lane & 15, d = dj * 32 + (lane & 16) + ((i & 3) << 2);
+    const int r = row0 + 16 * m + 4 * (lane >> 5) + (i >> 2);
+    const s16x4 a = lds_read_tr16(t + toff<HD>(r, d >> 3) + ((d & 4) << 1));
+    const s16x4 b = lds_read_tr16(t + toff<HD>(r + 8, d >> 3) + ((d & 4) << 1));
+    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+}
+__device__ __forceinline__ bf16x8 pack_half(const f32x16& s, int m) {
+    const uint4 w = make_uint4(pack_bf2(s[8 * m], s[8 * m + 1]), pack_bf2(s[8 * m + 2], s[8 * m + 3]), pack_bf2(s[8 * m + 4], s[8 * m + 5]), pack_bf2(s[8 * m + 6], s[8 * m + 7]));
+    return __builtin_bit_cast(bf16x8, w);
+}
+__device__ __forceinline__ f32x16 zero16() { f32x16 z; for (int i = 0; i < 16; ++i) z[i] = 0.f; return z; }
+__device__ __forceinline__ int reg_row(int r, int lane) { return (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5); }
+__device__ __forceinline__ int wave_min_i(int v) { for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64)); return v; }
+__device__ __forceinline__ int wave_max_i(int v) { for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64)); return v; }
+
+// does any of the 8 bf16 values have an all-ones exponent
+__device__ __forceinline__ bool not_finite(const uint4 w) {
+    typedef unsigned short u16x2 __attribute__((ext_vector_type(2)));
+    const u16x2 a = __builtin_bit_cast(u16x2, w.x & 0x7fff7fffu), b = __builtin_bit_cast(u16x2, w.y & 0x7fff7fffu);
+    const u16x2 c = __builtin_bit_cast(u16x2, w.z & 0x7fff7fffu), d = __builtin_bit_cast(u16x2, w.w & 0x7fff7fffu);
+    const u16x2 m = __builtin_elementwise_max(__builtin_elementwise_max(a, b), __builtin_elementwise_max(c, d));
+    return m[0] >= 0x7f80 || m[1] >= 0x7f80;
+}
+
+// ---- staging: a tile of two matrices (X, Y) and of the per-token vectors, global -> registers -> LDS
+template <int HD, int NT>                      // NT threads
+struct Stage {
+    static constexpr int CPR = HD / 8, CH = TT * CPR / NT;      // chunks per row, chunks per thread and matrix
+    uint4 x[CH], y[CH];
+    unsigned bad;                              // bit i / 16 + i: chunk i of x / y lies in a row that does not take part
+    // doc: of the tile's tokens, or null where all of them take part
+    __device__ __forceinline__ void load(const bf16_t* X, long xrs, const bf16_t* Y, long yrs, const int* doc, int row0, int n, int tid) {
+        bad = 0;
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int c = tid + NT * i, r = row0 + c / CPR, e = (c % CPR) * 8;
+            const int rc = min(r, n - 1);
+            x[i] = *reinterpret_cast<const uint4*>(X + (long)rc * xrs + e);
+            y[i] = *reinterpret_cast<const uint4*>(Y + (long)rc * yrs + e);
+            if (r >= n || (doc && doc[rc] < 0)) bad |= 1u << i;
+        }
+    }
+    // CX / CY: replace rows that are not finite by zeros and note them (partial tiles only)
+    template <bool CX, bool CY>
+    __device__ __forceinline__ void store(char* lx, char* ly, unsigned long long* noted, bool partial, int tid) {
+        const uint4 z = make_uint4(0, 0, 0, 0);
+#pragma unroll
+        for (int i = 0; i < CH; ++i) {
+            const int c = tid + NT * i, r = c / CPR;
+            uint4 a = x[i], b = y[i];
+            if (partial) {
+                if ((bad >> i) & 1) a = b = z;
+                const bool na = CX && not_finite(a), nb = CY && not_finite(b);
+                if (na) a = z;
+                if (nb) b = z;
+                if (na || nb) atomicOr(noted, 1ull << r);
+            }
+            *reinterpret_cast<uint4*>(lx + toff<HD>(r, c % CPR)) = a;
+            *reinterpret_cast<uint4*>(ly + toff<HD>(r, c % CPR)) = b;
+        }
+    }
+};
+
+// smallest / largest document and number of valid tokens of every 64-token tile of a batch row
+__global__ __launch_bounds__(256) void doc_tiles_kernel(const int* __restrict__ doc, int4* __restrict__ tab, int B, int N, int nt) {
+    const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+    if (t >= B * nt) return;
+    const int b = t / nt, j = (t - b * nt) * TT + lane;
+    const int d = j < N ? doc[(long)b * N + j] : -1;
+    const int lo = wave_min_i(d < 0 ? 0x7fffffff : d), hi = wave_max_i(d);
+    const int n = __popcll(__builtin_amdgcn_ballot_w64(d >= 0));
+    if (lane == 0) tab[t] = make_int4(lo, hi, n, 0);
+}
+
+// blocks are dispatched round-robin over the 8 dies: give each die one contiguous range of work, so that the row blocks of one head find its
+// keys in their own L2
+__device__ __forceinline__ int die_range(int blk, int n) {
+    const int q = n >> 3, r = n & 7, die = blk & 7, idx = blk >> 3;
+    return (die < r ? die * (q + 1) : r * (q + 1) + (die - r) * q) + idx;
+}
+
+// ---- the tiles an owner block walks: 64 at a time, one per lane
+struct Walk {
+    unsigned long long see, part;              // of the current group of 64 tiles: seen by some row; seen, but not whole
+    int base;                                  // first tile of the group
+};
+
+// scores in registers -> log2 units (CAP, BIAS) or left raw; steep: 1 - tanh^2
+template <bool CAP, bool BIAS, bool STEEP>
+__device__ __forceinline__ void modify(f32x16& s, f32x16& steep, const ModArgs& a, const float (&mine)[3], const float* pos, int row0, float slope2, int lane) {
+    const float c1 = a.scale * LOG2E_F;
+    if (CAP) {
+        const float up = 2.f * c1 / a.cap, capl = a.cap * LOG2E_F;
+#pragma unroll
+        for (int r = 0; r < 16; ++r) {
+            const float th = fmaf(-2.f, __builtin_amdgcn_rcpf(fast_exp2(s[r] * up) + 1.f), 1.f);       // tanh(x) = 1 - 2 / (e^2x + 1)
+            s[r] = capl * th;
+            if (STEEP) steep[r] = fmaf(-th, th, 1.f);
+        }
+    }
+    if (BIAS) {
+        f32x16 far = zero16();
+#pragma unroll
+        for (int ax = 0; ax < 3; ++ax) if (ax < a.axes) {
+#pragma unroll
+            for (int g = 0; g < 4; ++g) {
+                const float4 p = *reinterpret_cast<const float4*>(pos + ax * TT + row0 + 8 * g + 4 * (lane >> 5));
+                far[4 * g] += fabsf(p.x - mine[ax]); far[4 * g + 1] += fabsf(p.y - mine[ax]);
+                far[4 * g + 2] += fabsf(p.z - mine[ax]); far[4 * g + 3] += fabsf(p.w - mine[ax]);
+            }
+        }
+#pragma unroll
+        for (int r = 0; r < 16; ++r) s[r] = CAP ? fmaf(far[r], -slope2, s[r]) : fmaf(far[r], -slope2, s[r] * c1);
+    }
+}
+
+// ================================================ forward ===============================================
+// NW waves of 32 queries.  NW = 1 serves up to 32 queries (a pooled or a single new token): every workgroup is one wave, and the keys are
+// split over many of them.
+template <int HD, int NW, bool CAP, bool BIAS>
+__global__ __launch_bounds__(64 * NW, 2) void attn_mod_fwd_kernel(const ModArgs a) {
+    constexpr int KS = HD / 16, DJ = HD / 32, NT = 64 * NW, TB = TT * HD * 2;
+    __shared__ __attribute__((aligned(16))) char ldsK[2][TB];
+    __shared__ __attribute__((aligned(16))) char ldsV[2][TB];
+    __shared__ __attribute__((aligned(16))) float ldsP[2][BIAS ? 3 * TT : 4];
+    __shared__ __attribute__((aligned(16))) int ldsD[2][TT];
+    __shared__ unsigned long long noted[3];                      // of tile n: slot n % 3
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int w = die_range(blockIdx.x, gridDim.x);
+    int blk = w % a.nblk;
+    const int rest = w / a.nblk, split = rest % a.splits, bh = rest / a.splits, b = bh / a.H, h = bh - b * a.H, hk = h / a.G;
+    if (a.causal) blk = a.nblk - 1 - blk;                       // the longest rows first
+    const bf16_t* kp = a.k + (long)b * a.k_bs + (long)hk * a.k_hs;
+    const bf16_t* vp = a.v + (long)b * a.v_bs + (long)hk * a.v_hs;
+    const int* docs = a.doc_k ? a.doc_k + (long)b * a.Nk : nullptr;
+    const int4* tab = a.doc_k ? a.tab_k + (long)b * a.ntk : nullptr;
+    const float* posk = BIAS ? a.pos_k + (long)b * a.Nk * a.axes : nullptr;
+    const int off = a.Nk - a.Nq;
+    const int pre = a.causal ? (a.prefix ? min(max(a.prefix[b], 0), a.Nk) : 0) : a.Nk;
+    // this lane's query (rows behind the last one repeat it and are not stored)
+    const int q0 = blk * 32 * NW + wave * 32, qr = min(q0 + (lane & 31), a.Nq - 1);
+    const bool active = q0 < a.Nq;
+    const bf16_t* qp = a.q + (long)b * a.q_bs + (long)qr * a.q_rs + (long)h * a.q_hs;
+    bf16x8 qf[KS];
+#pragma unroll
+    for (int kk = 0; kk < KS; ++kk) qf[kk] = *reinterpret_cast<const bf16x8*>(qp + kk * 16 + 8 * (lane >> 5));
+    const int lim = max(pre, min(qr + off + 1, a.Nk));          // keys below it are visible as far as order goes (qr + off + 1 may be <= 0)
+    const int mydoc = a.doc_q ? a.doc_q[(long)b * a.Nq + qr] : 0;
+    float mine[3] = {0.f, 0.f, 0.f};
+    float slope2 = 0.f;
+    if (BIAS) {
+        slope2 = a.slopes[h] * LOG2E_F;
+        for (int ax = 0; ax < a.axes; ++ax) mine[ax] = a.pos_q[((long)b * a.Nq + qr) * a.axes + ax];
+    }
+    const int wlim_lo = __builtin_amdgcn_readfirstlane(wave_min_i(lim)), wlim_hi = __builtin_amdgcn_readfirstlane(wave_max_i(lim));
+    int wlo = 0, whi = 0;
+    bool pure = true;
+    if (docs) {
+        wlo = __builtin_amdgcn_readfirstlane(wave_min_i(mydoc < 0 ? 0x7fffffff : mydoc));
+        whi = __builtin_amdgcn_readfirstlane(wave_max_i(mydoc));
+        pure = wlo == whi && __builtin_amdgcn_ballot_w64(mydoc < 0) == 0;
+    }
+    // the workgroup's ranges: over its 64-row document tiles, and by its first and last row
+    const int g0 = blk * 32 * NW, g1 = min(g0 + 32 * NW, a.Nq) - 1;
+    const int glim_lo = max(pre, min(g0 + off + 1, a.Nk)), glim_hi = max(pre, min(g1 + off + 1, a.Nk));
+    int glo = 0, ghi = 0;
+    bool gpure = true;
+    if (docs) {
+        glo = 0x7fffffff; ghi = -1;
+        for (int t = g0 / TT; t <= g1 / TT; ++t) {
+            const int4 e = a.tab_q[(long)b * a.ntq + t];
+            glo = min(glo, e.x); ghi = max(ghi, e.y);
+            gpure &= e.z == min(TT, a.Nq - t * TT);
+        }
+        gpure &= glo == ghi;
+    }
+    const int t_lo = (int)((long)split * a.ntk / a.splits), t_hi = (int)((long)(split + 1) * a.ntk / a.splits);
+    Walk wk;
+    auto group = [&](int base) {
+        const int t = base + lane;
+        bool see = t < t_hi && t * TT < glim_hi, whole = t * TT + TT <= glim_lo;
+        if (docs && see) {
+            const int4 e = tab[t];
+            see = e.x <= ghi && e.y >= glo;
+            whole = whole && gpure && e.x == e.y && e.x == glo && e.z == TT;
+        }
+        wk.base = base;
+        wk.see = __builtin_amdgcn_ballot_w64(see);
+        wk.part = __builtin_amdgcn_ballot_w64(see && !whole);
+    };
+    auto next = [&](bool& partial) {                             // the next seen tile, or -1
+        while (wk.see == 0) {
+            if (wk.base + 64 >= t_hi) return -1;
+            group(wk.base + 64);
+        }
+        const int i = __builtin_ctzll(wk.see);
+        wk.see &= wk.see - 1;
+        partial = (wk.part >> i) & 1;
+        return wk.base + i;
+    };
+    group(t_lo);
+    f32x16 o[DJ];
+#pragma unroll
+    for (int dj = 0; dj < DJ; ++dj) o[dj] = zero16();
+    float m_run = -INFINITY, l_run = 0.f;
+    bool poisoned = false;
+    constexpr bool RAW = !CAP && !BIAS;                          // scores stay q.k and the exponent takes the factor
+    const float unit = RAW ? a.scale * LOG2E_F : 1.f;
+
+    Stage<HD, NT> st;
+    float pv = 0.f; int dv = 0;
+    auto fetch = [&](int t, bool partial) {
+        st.load(kp, a.k_rs, vp, a.v_rs, partial ? docs : nullptr, t * TT, a.Nk, tid);
+        if (NW == 1) return;
+        // waves 0 .. 2: one axis each, wave 3: the documents
+        const int r = min(t * TT + lane, a.Nk - 1);
+        if (BIAS && wave < a.axes) pv = posk[(long)r * a.axes + wave];
+        if (docs && wave == NW - 1) dv = docs[r];
+    };
+    auto put = [&](int t, int buf, int slot, bool partial) {
+        st.template store<false, true>(ldsK[buf], ldsV[buf], &noted[slot], partial, tid);
+        if (NW == 1) {
+            const int r = min(t * TT + lane, a.Nk - 1);
+            if (BIAS) for (int ax = 0; ax < a.axes; ++ax) ldsP[buf][ax * TT + lane] = posk[(long)r * a.axes + ax];
+            if (docs) ldsD[buf][lane] = docs[r];
+        } else {
+            if (BIAS && wave < a.axes) ldsP[buf][wave * TT + lane] = pv;
+            if (docs && wave == NW - 1) ldsD[buf][lane] = dv;
+        }
+    };
+    if (tid < 3) noted[tid] = 0;
+    __syncthreads();
+    bool partial = false, partial_n = false;
+    int t = next(partial), buf = 0, slot = 0;
+    if (t >= 0) { fetch(t, partial); put(t, 0, 0, partial); }
+    __syncthreads();
+    while (t >= 0) {
+        const int tn = next(partial_n);
+        if (tn >= 0) fetch(tn, partial_n);
+        const int slot_n = slot == 2 ? 0 : slot + 1;
+        if (tid == 0) noted[slot_n == 2 ? 0 : slot_n + 1] = 0;   // read during the tile before this one, written during the next one
+        const int j0 = t * TT;
+        bool see = active && j0 < wlim_hi, whole = j0 + TT <= wlim_lo;
+        if (docs) {
+            const int4 e = tab[t];
+            see = see && e.x <= whi && e.y >= wlo;
+            whole = whole && pure && e.x == e.y && e.x == wlo && e.z == TT;
+        }
+        if (see) {
+            f32x16 s[2];
+            float mx = -INFINITY;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                s[kb] = zero16();
+#pragma unroll
+                for (int kk = 0; kk < KS; ++kk) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_row<HD>(ldsK[buf], kb * 32, kk, lane), qf[kk], s[kb], 0, 0, 0);
+                f32x16 none;
+                modify<CAP, BIAS, false>(s[kb], none, a, mine, ldsP[buf], kb * 32, slope2, lane);
+                if (!whole) {
+                    asm volatile("" ::: "memory");               // keeps the test per score a branch
+#pragma unroll
+                    for (int g = 0; g < 4; ++g) {
+                        const int jr = kb * 32 + 8 * g + 4 * (lane >> 5);
+                        int4 d = make_int4(mydoc, mydoc, mydoc, mydoc);
+                        if (docs) d = *reinterpret_cast<const int4*>(&ldsD[buf][jr]);
+                        const int lj = lim - j0 - jr;
+                        const bool on = mydoc >= 0;
+                        if (!(on && lj > 0 && d.x == mydoc)) s[kb][4 * g] = -INFINITY;
+                        if (!(on && lj > 1 && d.y == mydoc)) s[kb][4 * g + 1] = -INFINITY;
+                        if (!(on && lj > 2 && d.z == mydoc)) s[kb][4 * g + 2] = -INFINITY;
+                        if (!(on && lj > 3 && d.w == mydoc)) s[kb][4 * g + 3] = -INFINITY;
+                    }
+                }
+#pragma unroll
+                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
+            }
+            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
+            // the reference point moves only when some row of the wave outgrew it by 2^8 (p <= 256 instead of 1): most tiles then skip the
+            // rescale of the 16 HD / 32 output registers
+            const float m_new = fmaxf(m_run, mx);
+            if (__builtin_amdgcn_ballot_w64((m_new - m_run) * unit > 8.f)) {
+                const float alpha = m_run == -INFINITY ? 0.f : fast_exp2((m_run - m_new) * unit);
+                m_run = m_new;
+                l_run *= alpha;
+#pragma unroll
+                for (int dj = 0; dj < DJ; ++dj)
+#pragma unroll
+                    for (int r = 0; r < 16; ++r) o[dj][r] *= alpha;
+            }
+            const float mu = m_run == -INFINITY ? 0.f : m_run * unit;
+            float l0 = 0.f, l1 = 0.f;
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int r = 0; r < 16; r += 2) {
+                    s[kb][r] = fast_exp2(RAW ? fmaf(s[kb][r], unit, -mu) : s[kb][r] - mu);
+                    s[kb][r + 1] = fast_exp2(RAW ? fmaf(s[kb][r + 1], unit, -mu) : s[kb][r + 1] - mu);
+                    l0 += s[kb][r]; l1 += s[kb][r + 1];
+                }
+            l_run += l0 + l1;
+            const uint32_t vb = lds_addr(ldsV[buf]);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb)
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    const bf16x8 p = pack_half(s[kb], m);
+#pragma unroll
+                    for (int dj = 0; dj < DJ; ++dj) o[dj] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_col<HD>(vb, kb * 32, m, dj, lane), p, o[dj], 0, 0, 0);
+                }
+            unsigned long long nt = noted[slot];
+            while (nt) {
+                const int r = __builtin_ctzll(nt);
+                nt &= nt - 1;
+                if (j0 + r < lim && (!docs || (mydoc >= 0 && ldsD[buf][r] == mydoc))) poisoned = true;
+            }
+        }
+        if (tn >= 0) put(tn, buf ^ 1, slot_n, partial_n);
+        __syncthreads();
+        t = tn; buf ^= 1; slot = slot_n;
+    }
+    l_run += __shfl_xor(l_run, 32, 64);
+    if (poisoned) l_run = NAN;
+    const int row = q0 + (lane & 31);
+    if (row >= a.Nq) return;
+    if (a.splits > 1) {
+        const long rows = (long)a.B * a.H * a.Nq, at = ((long)split * rows + ((long)b * a.H + h) * a.Nq + row);
+#pragma unroll
+        for (int dj = 0; dj < DJ; ++dj)
+#pragma unroll
+            for (int g = 0; g < 4; ++g)
+                *reinterpret_cast<float4*>(a.part + at * HD + dj * 32 + 8 * g + 4 * (lane >> 5)) = make_float4(o[dj][4 * g], o[dj][4 * g + 1], o[dj][4 * g + 2], o[dj][4 * g + 3]);
+        if (lane < 32) *reinterpret_cast<float2*>(a.part_ml + at * 2) = make_float2(m_run * unit, l_run);
+        return;
+    }
+    const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
+    bf16_t* op = a.o + (long)b * a.o_bs + (long)row * a.o_rs + (long)h * a.o_hs;
+#pragma unroll
+    for (int dj = 0; dj < DJ; ++dj)
+#pragma unroll
+        for (int g = 0; g < 4; ++g)
+            *reinterpret_cast<uint2*>(op + dj * 32 + 8 * g + 4 * (lane >> 5)) =
+                make_uint2(pack_bf2(o[dj][4 * g] * inv, o[dj][4 * g + 1] * inv), pack_bf2(o[dj][4 * g + 2] * inv, o[dj][4 * g + 3] * inv));
+    if (a.lse && lane < 32) a.lse[((long)b * a.H + h) * a.Nq + row] = l_run == 0.f ? -INFINITY : (m_run * unit + __log2f(l_run)) * LN2_F;
+}
+
+// joins the splits of a row: weights 2^(m_s - max m), one thread per 4 elements
+__global__ __launch_bounds__(256) void attn_mod_join_kernel(const ModArgs a, int HD) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    const int cpr = HD / 4;
+    const long rows = (long)a.B * a.H * a.Nq, r = i / cpr;
+    if (r >= rows) return;
+    const int c = (int)(i - r * cpr) * 4;
+    float m = -INFINITY;
+    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[(s * rows + r) * 2]);
+    float l = 0.f;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < a.splits; ++s) {
+        const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (s * rows + r) * 2);
+        if (ml.x == -INFINITY && ml.y == 0.f) continue;
+        const float f = ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - m);
+        const float4 v = *reinterpret_cast<const float4*>(a.part + (s * rows + r) * HD + c);
+        l = fmaf(ml.y, f, l);
+        acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
+    }
+    const float inv = l == 0.f ? 0.f : 1.f / l;
+    const long bh = r / a.Nq;
+    const int row = (int)(r - bh * a.Nq), b = (int)(bh / a.H), h = (int)(bh - (long)b * a.H);
+    *reinterpret_cast<uint2*>(a.o + (long)b * a.o_bs + (long)row * a.o_rs + (long)h * a.o_hs + c) = make_uint2(pack_bf2(acc.x * inv, acc.y * inv), pack_bf2(acc.z * inv, acc.w * inv));
+    if (a.lse && c == 0) a.lse[r] = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2_F;
+}
+
+// ================================================ backward ==============================================
+// The two owner kernels share the walk, the staging and the arithmetic of a 32 x 32 block:
+//   OWN_Q: lane = query, tiles of keys:  S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T          (7 of the 10 hd flop a pair twice: 14 hd in all)
+//   OWN_K: lane = key, tiles of queries: S = Q K^T,  dP = dO V^T,  dV^T += dO^T P, dK^T += Q^T dS
+// X, Y: the staged matrices (K, V or Q, dO); own fragments: (Q, dO) or (K, V).  OWN_Q also forms sum(do o), which OWN_K reads.
+template <int HD, bool OWN_Q, bool CAP, bool BIAS>
+__global__ __launch_bounds__(256, 2) void attn_mod_bwd_kernel(const ModArgs a) {
+    constexpr int KS = HD / 16, DJ = HD / 32, TB = TT * HD * 2;
+    __shared__ __attribute__((aligned(16))) char ldsX[2][TB];
+    __shared__ __attribute__((aligned(16))) char ldsY[2][TB];
+    __shared__ __attribute__((aligned(16))) float ldsP[2][BIAS ? 3 * TT : 4];
+    __shared__ __attribute__((aligned(16))) int ldsD[2][TT];
+    __shared__ __attribute__((aligned(16))) float ldsL[2][OWN_Q ? 4 : 2 * TT];      // lse (log2 units) and sum(do o) of the staged queries
+    __shared__ unsigned long long noted[3];
+    const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
+    const int w = die_range(blockIdx.x, gridDim.x);
+    int blk = w % a.nblk;
+    const int rest = w / a.nblk, split = rest % a.splits, bo = rest / a.splits;
+    const int OH = OWN_Q ? a.H : a.Hk, b = bo / OH, ho = bo - b * OH;                 // the owner's head: a query head or a key head
+    if (OWN_Q && a.causal) blk = a.nblk - 1 - blk;                                   // the longest rows first (keys: the first are the longest)
+    const int NO = OWN_Q ? a.Nq : a.Nk, NS = OWN_Q ? a.Nk : a.Nq;                    // rows of the owner's side and of the staged side
+    const int off = a.Nk - a.Nq;
+    const int pre = a.causal ? (a.prefix ? min(max(a.prefix[b], 0), a.Nk) : 0) : a.Nk;
+    const bool bydoc = a.doc_k != nullptr;
+    const int* doc_o = bydoc ? (OWN_Q ? a.doc_q : a.doc_k) + (long)b * NO : nullptr;
+    const int* doc_s = bydoc ? (OWN_Q ? a.doc_k : a.doc_q) + (long)b * NS : nullptr;
+    const int nts = OWN_Q ? a.ntk : a.ntq, nto = OWN_Q ? a.ntq : a.ntk;
+    const int4* tab_s = bydoc ? (OWN_Q ? a.tab_k : a.tab_q) + (long)b * nts : nullptr;
+    const int4* tab_o = bydoc ? (OWN_Q ? a.tab_q : a.tab_k) + (long)b * nto : nullptr;
+    const float* pos_s = BIAS ? (OWN_Q ? a.pos_k : a.pos_q) + (long)b * NS * a.axes : nullptr;
+    const int r0 = blk * 128 + wave * 32, ro = min(r0 + (lane & 31), NO - 1), row = r0 + (lane & 31);
+    const bool active = r0 < NO;
+    // own fragments
+    bf16x8 fa[KS], fb[KS];
+    float lse2 = 0.f, D = 0.f;
+    {
+        const bf16_t* pa = OWN_Q ? a.q + (long)b * a.q_bs + (long)ro * a.q_rs + (long)ho * a.q_hs : a.k + (long)b * a.k_bs + (long)ro * a.k_rs + (long)ho * a.k_hs;
+        const bf16_t* pb = OWN_Q ? a.d_o + (long)b * a.do_bs + (long)ro * a.do_rs + (long)ho * a.do_hs : a.v + (long)b * a.v_bs + (long)ro * a.v_rs + (long)ho * a.v_hs;
+#pragma unroll
+        for (int kk = 0; kk < KS; ++kk) {
+            fa[kk] = *reinterpret_cast<const bf16x8*>(pa + kk * 16 + 8 * (lane >> 5));
+            fb[kk] = *reinterpret_cast<const bf16x8*>(pb + kk * 16 + 8 * (lane >> 5));
+        }
+        if (OWN_Q) {
+            const bf16_t* po = a.o + (long)b * a.o_bs + (long)ro * a.o_rs + (long)ho * a.o_hs;
+#pragma unroll
+            for (int kk = 0; kk < KS; ++kk) {
+                const bf16x8 fo = *reinterpret_cast<const bf16x8*>(po + kk * 16 + 8 * (lane >> 5));
+#pragma unroll
+                for (int e = 0; e < 8; ++e) D = fmaf(bf2f((bf16_t)fo[e]), bf2f((bf16_t)fb[kk][e]), D);
+            }
+            D += __shfl_xor(D, 32, 64);
+            const long at = ((long)b * a.H + ho) * a.Nq + ro;
+            lse2 = a.lse[at] * LOG2E_F;
+            if (lse2 == -INFINITY) { lse2 = INFINITY; D = 0.f; }                     // a row that saw nothing: p = 2^(s - inf) = 0
+            if (split == 0 && lane < 32 && row < NO) a.dsum[at] = D;
+        }
+    }
+    const int mydoc = bydoc ? doc_o[ro] : 0;
+    float mine[3] = {0.f, 0.f, 0.f};
+    if (BIAS) for (int ax = 0; ax < a.axes; ++ax) mine[ax] = (OWN_Q ? a.pos_q : a.pos_k)[((long)b * NO + ro) * a.axes + ax];
+    // order: the staged index must be below `edge` (OWN_Q) or at least `edge` (OWN_K); first and last row of the wave and of the workgroup
+    auto edge_of = [&](int r) { return OWN_Q ? max(pre, min(r + off + 1, a.Nk)) : (r < pre ? 0 : r - off); };
+    const int edge = edge_of(ro);
+    const int w1 = min(r0 + 32, NO) - 1, g0 = blk * 128, g1 = min(g0 + 128, NO) - 1;
+    const int wedge0 = edge_of(min(r0, NO - 1)), wedge1 = edge_of(w1), gedge0 = edge_of(g0), gedge1 = edge_of(g1);
+    int wlo = 0, whi = 0, glo = 0, ghi = 0;
+    bool pure = true, gpure = true;
+    if (bydoc) {
+        wlo = __builtin_amdgcn_readfirstlane(wave_min_i(mydoc < 0 ? 0x7fffffff : mydoc));
+        whi = __builtin_amdgcn_readfirstlane(wave_max_i(mydoc));
+        pure = wlo == whi && __builtin_amdgcn_ballot_w64(mydoc < 0) == 0;
+        glo = 0x7fffffff; ghi = -1;
+        for (int t = g0 / TT; t <= g1 / TT; ++t) {
+            const int4 e = tab_o[t];
+            glo = min(glo, e.x); ghi = max(ghi, e.y);
+            gpure &= e.z == min(TT, NO - t * TT);
+        }
+        gpure &= glo == ghi;
+    }
+    auto order_see = [&](int t, int e0, int e1) { return OWN_Q ? t * TT < e1 : t * TT + TT > e0; };
+    auto order_whole = [&](int t, int e0, int e1) { return OWN_Q ? t * TT + TT <= e0 : t * TT >= e1; };
+    const int t_lo = (int)((long)split * nts / a.splits), t_hi = (int)((long)(split + 1) * nts / a.splits);
+    Walk wk;
+    int g = 0;                                                   // OWN_K: the query head of the group
+    auto group = [&](int base) {
+        const int t = base + lane;
+        bool see = t < t_hi && order_see(t, gedge0, gedge1), whole = order_whole(t, gedge0, gedge1) && t * TT + TT <= NS;
+        if (bydoc && see) {
+            const int4 e = tab_s[t];
+            see = e.x <= ghi && e.y >= glo;
+            whole = whole && gpure && e.x == e.y && e.x == glo && e.z == TT;
+        }
+        wk.base = base;
+        wk.see = __builtin_amdgcn_ballot_w64(see);
+        wk.part = __builtin_amdgcn_ballot_w64(see && !whole);
+    };
+    auto next = [&](bool& partial) {
+        while (wk.see == 0) {
+            if (wk.base + 64 < t_hi) group(wk.base + 64);
+            else if (!OWN_Q && g + 1 < a.G) { ++g; group(t_lo); }
+            else return -1;
+        }
+        const int i = __builtin_ctzll(wk.see);
+        wk.see &= wk.see - 1;
+        partial = (wk.part >> i) & 1;
+        return wk.base + i;
+    };
+    group(t_lo);
+    f32x16 ga[DJ], gb[OWN_Q ? 1 : DJ];                           // dQ^T, or dK^T and dV^T
+#pragma unroll
+    for (int dj = 0; dj < DJ; ++dj) { ga[dj] = zero16(); if (!OWN_Q) gb[dj] = zero16(); }
+    bool poisoned = false;
+    constexpr bool RAW = !CAP && !BIAS;
+    const float unit = RAW ? a.scale * LOG2E_F : 1.f;
+
+    Stage<HD, 256> st;
+    float pv = 0.f, lv = 0.f; int dv = 0;
+    auto fetch = [&](int t, int h, bool partial) {
+        const bf16_t* X = OWN_Q ? a.k + (long)b * a.k_bs + (long)(ho / a.G) * a.k_hs : a.q + (long)b * a.q_bs + (long)h * a.q_hs;
+        const bf16_t* Y = OWN_Q ? a.v + (long)b * a.v_bs + (long)(ho / a.G) * a.v_hs : a.d_o + (long)b * a.do_bs + (long)h * a.do_hs;
+        st.load(X, OWN_Q ? a.k_rs : a.q_rs, Y, OWN_Q ? a.v_rs : a.do_rs, partial ? doc_s : nullptr, t * TT, NS, tid);
+        const int r = min(t * TT + lane, NS - 1);
+        if (BIAS && wave < a.axes) pv = pos_s[(long)r * a.axes + wave];
+        if (bydoc && wave == 3) dv = doc_s[r];
+        if (!OWN_Q && wave < 2) lv = (wave ? a.dsum : a.lse)[((long)b * a.H + h) * a.Nq + r];
+    };
+    auto put = [&](int t, int buf, int slot, bool partial) {
+        st.template store<true, !OWN_Q>(ldsX[buf], ldsY[buf], &noted[slot], partial, tid);
+        if (BIAS && wave < a.axes) ldsP[buf][wave * TT + lane] = pv;
+        if (bydoc && wave == 3) ldsD[buf][lane] = dv;
+        if (!OWN_Q && wave < 2) {
+            const bool in = t * TT + lane < NS;                  // behind the last query: p = 0
+            if (wave == 0) ldsL[buf][lane] = (in && lv != -INFINITY) ? lv * LOG2E_F : INFINITY;
+            else ldsL[buf][TT + lane] = in ? lv : 0.f;
+        }
+    };
+    if (tid < 3) noted[tid] = 0;
+    __syncthreads();
+    bool partial = false, partial_n = false;
+    int t = next(partial), buf = 0, slot = 0;
+    int h = OWN_Q ? ho : ho * a.G + g;
+    if (t >= 0) { fetch(t, h, partial); put(t, 0, 0, partial); }
+    __syncthreads();
+    while (t >= 0) {
+        const int tn = next(partial_n);
+        const int hn = OWN_Q ? ho : ho * a.G + g;
+        if (tn >= 0) fetch(tn, hn, partial_n);
+        const int slot_n = slot == 2 ? 0 : slot + 1;
+        if (tid == 0) noted[slot_n == 2 ? 0 : slot_n + 1] = 0;   // read during the tile before this one, written during the next one
+        const int j0 = t * TT;
+        bool see = active && order_see(t, wedge0, wedge1), whole = order_whole(t, wedge0, wedge1);
+        if (OWN_Q) whole = whole && j0 + TT <= NS;
+        if (bydoc) {
+            const int4 e = tab_s[t];
+            see = see && e.x <= whi && e.y >= wlo;
+            whole = whole && pure && e.x == e.y && e.x == wlo && e.z == TT;
+        }
+        if (see) {
+            const float slope2 = BIAS ? a.slopes[h] * LOG2E_F : 0.f;
+            const uint32_t xb = lds_addr(ldsX[buf]), yb = lds_addr(ldsY[buf]);
+#pragma unroll
+            for (int kb = 0; kb < 2; ++kb) {
+                f32x16 s = zero16(), dp = zero16(), steep;
+#pragma unroll
+                for (int kk = 0; kk < KS; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_row<HD>(ldsX[buf], kb * 32, kk, lane), fa[kk], s, 0, 0, 0);
+#pragma unroll
+                for (int kk = 0; kk < KS; ++kk) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_row<HD>(ldsY[buf], kb * 32, kk, lane), fb[kk], dp, 0, 0, 0);
+                modify<CAP, BIAS, true>(s, steep, a, mine, ldsP[buf], kb * 32, slope2, lane);
+#pragma unroll
+                for (int q = 0; q < 4; ++q) {
+                    const int jr = kb * 32 + 8 * q + 4 * (lane >> 5);
+                    float4 L = make_float4(lse2, lse2, lse2, lse2), E = make_float4(D, D, D, D);
+                    if (!OWN_Q) { L = *reinterpret_cast<const float4*>(&ldsL[buf][jr]); E = *reinterpret_cast<const float4*>(&ldsL[buf][TT + jr]); }
+                    const float Ls[4] = {L.x, L.y, L.z, L.w}, Es[4] = {E.x, E.y, E.z, E.w};
+#pragma unroll
+                    for (int e = 0; e < 4; ++e) {
+                        const int r = 4 * q + e;
+                        s[r] = fast_exp2(RAW ? fmaf(s[r], unit, -Ls[e]) : s[r] - Ls[e]);
+                        dp[r] = s[r] * (dp[r] - Es[e]);
+                        if (CAP) dp[r] *= steep[r];
+                    }
+                }
+                if (!whole) {
+                    asm volatile("" ::: "memory");               // keeps the test per score a branch
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int jr = kb * 32 + 8 * q + 4 * (lane >> 5);
+                        int4 d = make_int4(mydoc, mydoc, mydoc, mydoc);
+                        if (bydoc) d = *reinterpret_cast<const int4*>(&ldsD[buf][jr]);
+                        const int ds[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+                        for (int e = 0; e < 4; ++e) {
+                            const int j = j0 + jr + e;
+                            const bool on = (OWN_Q ? j < edge : (j >= edge && j < NS)) && mydoc >= 0 && ds[e] == mydoc;
+                            if (!on) s[4 * q + e] = dp[4 * q + e] = 0.f;
+                        }
+                    }
+                }
+#pragma unroll
+                for (int m = 0; m < 2; ++m) {
+                    const bf16x8 ds = pack_half(dp, m);
+#pragma unroll
+                    for (int dj = 0; dj < DJ; ++dj) ga[dj] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_col<HD>(xb, kb * 32, m, dj, lane), ds, ga[dj], 0, 0, 0);
+                    if (!OWN_Q) {
+                        const bf16x8 p = pack_half(s, m);
+#pragma unroll
+                        for (int dj = 0; dj < DJ; ++dj) gb[dj] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_col<HD>(yb, kb * 32, m, dj, lane), p, gb[dj], 0, 0, 0);
+                    }
+                }
+            }
+            unsigned long long nt = noted[slot];
+            while (nt) {
+                const int r = __builtin_ctzll(nt), j = j0 + r;
+                nt &= nt - 1;
+                if ((OWN_Q ? j < edge : j >= edge) && (!bydoc || (mydoc >= 0 && ldsD[buf][r] == mydoc))) poisoned = true;
+            }
+        }
+        if (tn >= 0) put(tn, buf ^ 1, slot_n, partial_n);
+        __syncthreads();
+        t = tn; h = hn; buf ^= 1; slot = slot_n;
+    }
+    if (row >= NO) return;
+    const float fa_out = poisoned ? NAN : a.scale, fb_out = poisoned ? NAN : 1.f;
+    if (a.splits > 1) {
+        const long rows = (long)a.B * OH * NO;
+        float* base = a.part + (((long)split * rows + ((long)b * OH + ho) * NO + row) * (OWN_Q ? 1 : 2)) * HD;
+#pragma unroll
+        for (int dj = 0; dj < DJ; ++dj)
+#pragma unroll
+            for (int q = 0; q < 4; ++q) {
+                const int d = dj * 32 + 8 * q + 4 * (lane >> 5);
+                *reinterpret_cast<float4*>(base + d) = make_float4(ga[dj][4 * q] * fa_out, ga[dj][4 * q + 1] * fa_out, ga[dj][4 * q + 2] * fa_out, ga[dj][4 * q + 3] * fa_out);
+                if (!OWN_Q) *reinterpret_cast<float4*>(base + HD + d) = make_float4(gb[dj][4 * q] * fb_out, gb[dj][4 * q + 1] * fb_out, gb[dj][4 * q + 2] * fb_out, gb[dj][4 * q + 3] * fb_out);
+            }
+        return;
+    }
+    bf16_t* pa = OWN_Q ? a.dq + (long)b * a.dq_bs + (long)row * a.dq_rs + (long)ho * a.dq_hs : a.dk + (long)b * a.dk_bs + (long)row * a.dk_rs + (long)ho * a.dk_hs;
+    bf16_t* pb = OWN_Q ? nullptr : a.dv + (long)b * a.dv_bs + (long)row * a.dv_rs + (long)ho * a.dv_hs;
+#pragma unroll
+    for (int dj = 0; dj < DJ; ++dj)
+#pragma unroll
+        for (int q = 0; q < 4; ++q) {
+            const int d = dj * 32 + 8 * q + 4 * (lane >> 5);
+            *reinterpret_cast<uint2*>(pa + d) = make_uint2(pack_bf2(ga[dj][4 * q] * fa_out, ga[dj][4 * q + 1] * fa_out), pack_bf2(ga[dj][4 * q + 2] * fa_out, ga[dj][4 * q + 3] * fa_out));
+            if (!OWN_Q) *reinterpret_cast<uint2*>(pb + d) = make_uint2(pack_bf2(gb[dj][4 * q] * fb_out, gb[dj][4 * q + 1] * fb_out), pack_bf2(gb[dj][4 * q + 2] * fb_out, gb[dj][4 * q + 3] * fb_out));
+        }
+}
+
+// adds the splits of gradient rows in order: [split][rows][sides][HD] fp32 -> bf16, one thread per 4 elements
+struct JoinOut { bf16_t* p; long bs, rs, hs; };
+__global__ __launch_bounds__(256) void attn_mod_sum_kernel(const float* __restrict__ part, int splits, long rows, int sides, int HD, int OH, int NO, JoinOut o0, JoinOut o1) {
+    const long i = (long)blockIdx.x * 256 + threadIdx.x;
+    const int per = sides * HD / 4;
+    const long r = i / per;
+    if (r >= rows) return;
+    const int e = (int)(i - r * per) * 4, side = e / HD, c = e - side * HD;
+    float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
+    for (int s = 0; s < splits; ++s) {
+        const float4 v = *reinterpret_cast<const float4*>(part + (s * rows + r) * sides * HD + e);
+        acc.x += v.x; acc.y += v.y; acc.z += v.z; acc.w += v.w;
+    }
+    const long bh = r / NO;
+    const int row = (int)(r - bh * NO), b = (int)(bh / OH), h = (int)(bh - (long)b * OH);
+    const JoinOut& o = side ? o1 : o0;
+    *reinterpret_cast<uint2*>(o.p + (long)b * o.bs + (long)row * o.rs + (long)h * o.hs + c) = make_uint2(pack_bf2(acc.x, acc.y), pack_bf2(acc.z, acc.w));
+}
+
+// ================================================ host ==================================================
+struct Plan {
+    int ntq, ntk, nw, nblk, splits, dq_splits, dkv_splits;
+    long tab_q, tab_k, dsum, part, part_ml, bytes;             // byte offsets into the workspace
+};
+
+int splits_for(long blocks, long want, int tiles, int least) {  // enough workgroups for the chip, but `least` tiles for each
+    if (blocks <= 0 || blocks >= want || tiles < 2 * least) return 1;
+    long s = (want + blocks - 1) / blocks;
+    if (s > tiles / least) s = tiles / least;
+    if (s > MAX_SPLITS) s = MAX_SPLITS;
+    return (int)s;
+}
+
+Plan plan_for(const mrg_attn_mod_desc* d, bool backward) {
+    Plan p = {};
+    p.ntq = (d->Nq + TT - 1) / TT; p.ntk = (d->Nk + TT - 1) / TT;
+    long at = 0;
+    auto take = [&](long bytes) { const long o = at; at += (bytes + 255) / 256 * 256; return o; };
+    if (d->doc_k) { p.tab_q = take(16l * d->B * p.ntq); p.tab_k = take(16l * d->B * p.ntk); }
+    const long rows_q = (long)d->B * d->H * d->Nq, rows_k = (long)d->B * d->Hk * d->Nk;
+    if (!backward) {
+        // up to 32 queries: workgroups of one wave, four resident per CU, and the keys cut until every CU has its four
+        p.nw = d->Nq <= 32 ? 1 : 4;
+        p.nblk = (d->Nq + 32 * p.nw - 1) / (32 * p.nw);
+        p.splits = splits_for((long)d->B * d->H * p.nblk, p.nw == 1 ? 1024 : 512, p.ntk, 4);
+        if (p.splits > 1) { p.part = take(4l * p.splits * rows_q * d->head_dim); p.part_ml = take(8l * p.splits * rows_q); }
+    } else {
+        p.dsum = take(4l * rows_q);
+        p.dq_splits = splits_for((long)d->B * d->H * ((d->Nq + 127) / 128), 512, p.ntk, 4);
+        p.dkv_splits = splits_for((long)d->B * d->Hk * ((d->Nk + 127) / 128), 512, p.ntq, 4);
+        long part = 0;
+        if (p.dq_splits > 1) part = 4l * p.dq_splits * rows_q * d->head_dim;
+        if (p.dkv_splits > 1 && 8l * p.dkv_splits * rows_k * d->head_dim > part) part = 8l * p.dkv_splits * rows_k * d->head_dim;
+        p.part = take(part);                                    // used by dq first, by dk / dv behind it
+    }
+    p.bytes = at;
+    return p;
+}
+
+int mod_check(const mrg_attn_mod_desc* d, const char* who) {
+    MRG_REQUIRE(d != nullptr, MRG_ERR_ARG, "%s: null descriptor", who);
+    MRG_REQUIRE(d->head_dim == 32 || d->head_dim == 64, MRG_ERR_UNSUPPORTED, "%s: head_dim %d not in (32, 64)", who, d->head_dim);
+    MRG_REQUIRE(d->B >= 0 && d->H > 0 && d->Hk > 0 && d->Nq >= 0 && d->Nk >= 0 && d->H % d->Hk == 0, MRG_ERR_SHAPE, "%s: bad sizes B %d H %d Hk %d Nq %d Nk %d", who,
+                d->B, d->H, d->Hk, d->Nq, d->Nk);
+    MRG_REQUIRE(d->Nq <= (1 << 26) && d->Nk <= (1 << 26) && (long)d->B * d->H * (((long)(d->Nq > d->Nk ? d->Nq : d->Nk) + 31) / 32) * MAX_SPLITS <= 0x7fffffffl,
+                MRG_ERR_SHAPE, "%s: too many rows for one launch", who);
+    MRG_REQUIRE(d->scale > 0.f && d->scale < 1e30f, MRG_ERR_ARG, "%s: scale %g must be positive and finite", who, d->scale);
+    MRG_REQUIRE(d->cap >= 0.f && d->cap < 1e30f, MRG_ERR_ARG, "%s: cap %g must be 0 (none) or positive", who, d->cap);
+    const bool some = d->B > 0 && d->Nq > 0 && d->Nk > 0;        // (tensors without elements may have no address)
+    MRG_REQUIRE(!some || ((d->slopes != nullptr) == (d->pos_q != nullptr) && (d->slopes != nullptr) == (d->pos_k != nullptr)), MRG_ERR_ARG, "%s: a distance bias needs slopes, pos_q and pos_k", who);
+    MRG_REQUIRE(!d->slopes || (d->axes >= 1 && d->axes <= MRG_MAX_AXES), MRG_ERR_SHAPE, "%s: %d axes (1 to %d)", who, d->axes, MRG_MAX_AXES);
+    MRG_REQUIRE(!some || (d->doc_q != nullptr) == (d->doc_k != nullptr), MRG_ERR_ARG, "%s: documents of the queries and of the keys come together", who);
+    MRG_REQUIRE(!d->prefix || d->causal, MRG_ERR_ARG, "%s: a prefix without causal order has no effect", who);
+    return MRG_OK;
+}
+
+bool aligned8(const void* p, long a, long b, long c) { return (uintptr_t)p % 16 == 0 && (a | b | c) % 8 == 0; }
+
+ModArgs mod_args(const mrg_attn_mod_desc* d, const Plan& p) {
+    ModArgs a = {};
+    a.q = (const bf16_t*)d->q; a.k = (const bf16_t*)d->k; a.v = (const bf16_t*)d->v; a.o = (bf16_t*)d->o; a.lse = d->lse;
+    a.q_bs = d->q_bs; a.q_rs = d->q_rs; a.q_hs = d->q_hs; a.k_bs = d->k_bs; a.k_rs = d->k_rs; a.k_hs = d->k_hs;
+    a.v_bs = d->v_bs; a.v_rs = d->v_rs; a.v_hs = d->v_hs; a.o_bs = d->o_bs; a.o_rs = d->o_rs; a.o_hs = d->o_hs;
+    a.B = d->B; a.H = d->H; a.Hk = d->Hk; a.G = d->H / d->Hk; a.Nq = d->Nq; a.Nk = d->Nk; a.scale = d->scale; a.cap = d->cap;
+    a.slopes = d->slopes; a.pos_q = d->pos_q; a.pos_k = d->pos_k; a.axes = d->slopes ? d->axes : 0;
+    a.doc_q = d->doc_q; a.doc_k = d->doc_k;
+    char* ws = (char*)d->ws;
+    a.tab_q = (const int4*)(ws + p.tab_q); a.tab_k = (const int4*)(ws + p.tab_k); a.ntq = p.ntq; a.ntk = p.ntk;
+    a.causal = d->causal != 0; a.prefix = d->prefix;
+    a.d_o = (const bf16_t*)d->d_o; a.do_bs = d->do_bs; a.do_rs = d->do_rs; a.do_hs = d->do_hs;
+    a.dq = (bf16_t*)d->dq; a.dk = (bf16_t*)d->dk; a.dv = (bf16_t*)d->dv;
+    a.dq_bs = d->dq_bs; a.dq_rs = d->dq_rs; a.dq_hs = d->dq_hs; a.dk_bs = d->dk_bs; a.dk_rs = d->dk_rs; a.dk_hs = d->dk_hs;
+    a.dv_bs = d->dv_bs; a.dv_rs = d->dv_rs; a.dv_hs = d->dv_hs;
+    a.dsum = (float*)(ws + p.dsum); a.part = (float*)(ws + p.part); a.part_ml = (float*)(ws + p.part_ml);
+    return a;
+}
+
+void doc_tables(const mrg_attn_mod_desc* d, const ModArgs& a, hipStream_t st) {
+    if (!d->doc_k) return;
+    if (a.ntq) hipLaunchKernelGGL(doc_tiles_kernel, dim3((d->B * a.ntq + 3) / 4), dim3(256), 0, st, d->doc_q, (int4*)a.tab_q, d->B, d->Nq, a.ntq);
+    if (a.ntk) hipLaunchKernelGGL(doc_tiles_kernel, dim3((d->B * a.ntk + 3) / 4), dim3(256), 0, st, d->doc_k, (int4*)a.tab_k, d->B, d->Nk, a.ntk);
+}
+
+template <int HD, int NW>
+void fwd_go(const ModArgs& a, dim3 grid, hipStream_t st) {
+    const bool bias = a.slopes != nullptr;
+    if (a.cap > 0.f) {
+        if (bias) hipLaunchKernelGGL((attn_mod_fwd_kernel<HD, NW, true, true>), grid, dim3(64 * NW), 0, st, a);
+        else hipLaunchKernelGGL((attn_mod_fwd_kernel<HD, NW, true, false>), grid, dim3(64 * NW), 0, st, a);
+    } else {
+        if (bias) hipLaunchKernelGGL((attn_mod_fwd_kernel<HD, NW, false, true>), grid, dim3(64 * NW), 0, st, a);
+        else hipLaunchKernelGGL((attn_mod_fwd_kernel<HD, NW, false, false>), grid, dim3(64 * NW), 0, st, a);
+    }
+}
+template <int HD, bool OWN_Q>
+void bwd_go(const ModArgs& a, dim3 grid, hipStream_t st) {
+    const bool bias = a.slopes != nullptr;
+    if (a.cap > 0.f) {
+        if (bias) hipLaunchKernelGGL((attn_mod_bwd_kernel<HD, OWN_Q, true, true>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((attn_mod_bwd_kernel<HD, OWN_Q, true, false>), grid, dim3(256), 0, st, a);
+    } else {
+        if (bias) hipLaunchKernelGGL((attn_mod_bwd_kernel<HD, OWN_Q, false, true>), grid, dim3(256), 0, st, a);
+        else hipLaunchKernelGGL((attn_mod_bwd_kernel<HD, OWN_Q, false, false>), grid, dim3(256), 0, st, a);
+    }
+}
+template <bool OWN_Q>
+void bwd_side(ModArgs a, int splits, int HD, hipStream_t st) {
+    const int NO = OWN_Q ? a.Nq : a.Nk, OH = OWN_Q ? a.H : a.Hk;
+    if (NO == 0) return;
+    a.splits = splits;
+    a.nblk = (NO + 127) / 128;
+    const dim3 grid((unsigned)((long)a.B * OH * a.nblk * splits));
+    if (HD == 64) bwd_go<64, OWN_Q>(a, grid, st); else bwd_go<32, OWN_Q>(a, grid, st);
+    if (splits > 1) {
+        const long rows = (long)a.B * OH * NO, threads = rows * (OWN_Q ? 1 : 2) * HD / 4;
+        const JoinOut o0 = OWN_Q ? JoinOut{a.dq, a.dq_bs, a.dq_rs, a.dq_hs} : JoinOut{a.dk, a.dk_bs, a.dk_rs, a.dk_hs}, o1 = JoinOut{a.dv, a.dv_bs, a.dv_rs, a.dv_hs};
+        hipLaunchKernelGGL(attn_mod_sum_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, st, a.part, splits, rows, OWN_Q ? 1 : 2, HD, OH, NO, o0, o1);
+    }
+}
+
+}  // namespace
+
+extern "C" long mrg_attn_mod_ws_bytes(const mrg_attn_mod_desc* d, int backward) {
+    if (mod_check(d, "mrg_attn_mod_ws_bytes")) return -1;
+    return plan_for(d, backward != 0).bytes;
+}
+
+extern "C" int mrg_attn_mod_fwd(const mrg_attn_mod_desc* d, hipStream_t stream) {
+    const int rc = mod_check(d, "mrg_attn_mod_fwd");
+    if (rc) return rc;
+    if (d->B == 0 || d->Nq == 0) return MRG_OK;
+    const Plan p = plan_for(d, false);
+    MRG_REQUIRE(d->q && d->o && (d->Nk == 0 || (d->k && d->v)) && (p.bytes == 0 || d->ws), MRG_ERR_ARG, "mrg_attn_mod_fwd: null pointer");
+    MRG_REQUIRE(aligned8(d->q, d->q_bs, d->q_rs, d->q_hs) && aligned8(d->k, d->k_bs, d->k_rs, d->k_hs) && aligned8(d->v, d->v_bs, d->v_rs, d->v_hs)
+                && aligned8(d->o, d->o_bs, d->o_rs, d->o_hs), MRG_ERR_ARG, "mrg_attn_mod_fwd: operands and their strides must be multiples of 16 bytes");
+    ModArgs a = mod_args(d, p);
+    a.nblk = p.nblk; a.splits = p.splits;
+    doc_tables(d, a, stream);
+    const dim3 grid((unsigned)((long)a.B * a.H * a.nblk * a.splits));
+    if (d->head_dim == 64) { if (p.nw == 1) fwd_go<64, 1>(a, grid, stream); else fwd_go<64, 4>(a, grid, stream); }
+    else { if (p.nw == 1) fwd_go<32, 1>(a, grid, stream); else fwd_go<32, 4>(a, grid, stream); }
+    if (a.splits > 1) {
+        const long threads = (long)a.B * a.H * a.Nq * d->head_dim / 4;
+        hipLaunchKernelGGL(attn_mod_join_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, a, d->head_dim);
+    }
+    return mrg_check_launch("mrg_attn_mod_fwd");
+}
+
+extern "C" int mrg_attn_mod_bwd(const mrg_attn_mod_desc* d, hipStream_t stream) {
+    const int rc = mod_check(d, "mrg_attn_mod_bwd");
+    if (rc) return rc;
+    if (d->B == 0 || (d->Nq == 0 && d->Nk == 0)) return MRG_OK;
+    const Plan p = plan_for(d, true);
+    MRG_REQUIRE((d->Nq == 0 || (d->q && d->o && d->lse && d->d_o && d->dq)) && (d->Nk == 0 || (d->k && d->v && d->dk && d->dv)) && (p.bytes == 0 || d->ws), MRG_ERR_ARG,
+                "mrg_attn_mod_bwd: null pointer");
+    MRG_REQUIRE(aligned8(d->q, d->q_bs, d->q_rs, d->q_hs) && aligned8(d->k, d->k_bs, d->k_rs, d->k_hs) && aligned8(d->v, d->v_bs, d->v_rs, d->v_hs)
+                && aligned8(d->o, d->o_bs, d->o_rs, d->o_hs) && aligned8(d->d_o, d->do_bs, d->do_rs, d->do_hs) && aligned8(d->dq, d->dq_bs, d->dq_rs, d->dq_hs)
+                && aligned8(d->dk, d->dk_bs, d->dk_rs, d->dk_hs) && aligned8(d->dv, d->dv_bs, d->dv_rs, d->dv_hs), MRG_ERR_ARG,
+                "mrg_attn_mod_bwd: operands and their strides must be multiples of 16 bytes");
+    ModArgs a = mod_args(d, p);
+    doc_tables(d, a, stream);
+    bwd_side<true>(a, p.dq_splits, d->head_dim, stream);
+    bwd_side<false>(a, p.dkv_splits, d->head_dim, stream);
+    return mrg_check_launch("mrg_attn_mod_bwd");
+}
