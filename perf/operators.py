@@ -303,10 +303,12 @@ def _plain_attn(s):
 # ------------------------------------------------------------------------------------------------------------------ the framework's calls
 def _own_rotary(s):
     from mirage_amd import kernels as K
-    q, k = K.rotary_axes(s["q"], s["k"], s["pos"], s["freqs"], s["sections"], pairing=s["pairing"])
+    # fp32 tensors are turned where they lie, as the plain form turns them; bf16 ones into new tensors
+    at = (lambda q, k: dict(out_q=s[q], out_k=s[k])) if s["dtype"] == "fp32" else (lambda q, k: {})  # noqa: E731
+    q, k = K.rotary_axes(s["q"], s["k"], s["pos"], s["freqs"], s["sections"], pairing=s["pairing"], **at("q", "k"))
     out = {"q": q, "k": k}
     if s["train"]:
-        out["dq"], out["dk"] = K.rotary_axes(s["dq"], s["dk"], s["pos"], s["freqs"], s["sections"], pairing=s["pairing"], inverse=True)
+        out["dq"], out["dk"] = K.rotary_axes(s["dq"], s["dk"], s["pos"], s["freqs"], s["sections"], pairing=s["pairing"], inverse=True, **at("dq", "dk"))
     return out
 
 
