@@ -13,8 +13,10 @@
 //
 // Masks by tiles.  A first small launch leaves the smallest and largest document and the count of valid tokens of every 64-token tile; a
 // workgroup tests 64 tiles at a time (one per lane, one ballot) and walks only tiles that some row of it may see.  Per wave a tile is skipped,
-// whole (no test per score) or partial.  Sums, maxima, lse and all products accumulate in fp32; p and ds are rounded to bf16 as operands of
-// the second products (relative 2^-9 each, averaging over the row), the sum of p is taken before the rounding.
+// whole (no test per score) or partial.  Sums, maxima, lse and all products accumulate in fp32.  p is rounded to bf16 as an operand of the
+// second product (at most 2^-8 of each weight, averaging over the row; its sum is taken before the rounding).  ds goes into its product as
+// two bf16 parts: rounded once, dq and dk were 0.0028 from the 64-bit gradient instead of 0.0022 (0.0017 is the rounding of the result
+// itself), because the rounding of ds adds to what the stored o carries into sum(do o).
 //
 // Values that are not finite behind a mask: 0 * inf would reach the products, so in partial tiles the rows of the second product's left
 // operand that hold such values are replaced by zeros in LDS and noted; a row that SEES one of them is NaN in full.
@@ -67,6 +69,15 @@ template <int HD> __device__ __forceinline__ bf16x8 frag_col(uint32_t t, int row
 __device__ __forceinline__ bf16x8 pack_half(const f32x16& s, int m) {
     const uint4 w = make_uint4(pack_bf2(s[8 * m], s[8 * m + 1]), pack_bf2(s[8 * m + 2], s[8 * m + 3]), pack_bf2(s[8 * m + 4], s[8 * m + 5]), pack_bf2(s[8 * m + 6], s[8 * m + 7]));
     return __builtin_bit_cast(bf16x8, w);
+}
+// what the rounding of s to bf16 (pack_half) left out, itself in bf16: a product with both parts sees s to 2^-17
+__device__ __forceinline__ bf16x8 pack_rest(const f32x16& s, int m, const bf16x8& hi) {
+    const uint4 h = __builtin_bit_cast(uint4, hi);
+    const uint32_t w[4] = {h.x, h.y, h.z, h.w};
+    uint32_t r[4];
+#pragma unroll
+    for (int i = 0; i < 4; ++i) r[i] = pack_bf2(s[8 * m + 2 * i] - __uint_as_float(w[i] << 16), s[8 * m + 2 * i + 1] - __uint_as_float(w[i] & 0xffff0000u));
+    return __builtin_bit_cast(bf16x8, make_uint4(r[0], r[1], r[2], r[3]));
 }
 __device__ __forceinline__ f32x16 zero16() { f32x16 z; for (int i = 0; i < 16; ++i) z[i] = 0.f; return z; }
 __device__ __forceinline__ int reg_row(int r, int lane) { return (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5); }
@@ -630,9 +641,13 @@ __global__ __launch_bounds__(256, 2) void attn_mod_bwd_kernel(const ModArgs a) {
                 }
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
-                    const bf16x8 ds = pack_half(dp, m);
+                    const bf16x8 ds = pack_half(dp, m), rest = pack_rest(dp, m, ds);
 #pragma unroll
-                    for (int dj = 0; dj < DJ; ++dj) ga[dj] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_col<HD>(xb, kb * 32, m, dj, lane), ds, ga[dj], 0, 0, 0);
+                    for (int dj = 0; dj < DJ; ++dj) {
+                        const bf16x8 x = frag_col<HD>(xb, kb * 32, m, dj, lane);
+                        ga[dj] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, ds, ga[dj], 0, 0, 0);
+                        ga[dj] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, rest, ga[dj], 0, 0, 0);
+                    }
                     if (!OWN_Q) {
                         const bf16x8 p = pack_half(s, m);
 #pragma unroll
