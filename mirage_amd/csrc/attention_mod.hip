@@ -8,8 +8,8 @@
 // of them: S^T = K Q^T leaves lane = query and registers = keys, so row maximum, sum and rescale are lane-local (one exchange between the
 // wave's halves), and the same registers, packed to bf16, are the right operand of the next product (O^T = V^T P^T): its contraction index
 // may come in any order as long as both operands agree, and V^T fragments read from LDS with ds_read_b64_tr_b16 take the accumulator's
-// order.  Scores never leave the registers.  Tiles of 64 keys go global -> registers -> LDS one tile ahead of the products, double-buffered,
-// one barrier per tile.
+// order.  Scores never leave the registers.  Tiles of 64 keys go global -> LDS by DMA one tile ahead of the products, double-buffered, one
+// barrier per tile.
 //
 // Masks by tiles.  A first small launch leaves the smallest and largest document and the count of valid tokens of every 64-token tile; a
 // workgroup tests 64 tiles at a time (one per lane, one ballot) and walks only tiles that some row of it may see.  Per wave a tile is skipped,
@@ -22,7 +22,7 @@
 // operand that hold such values are replaced by zeros in LDS and noted; a row that SEES one of them is NaN in full.
 //
 // No atomics on results: dq is owned by queries, dk / dv by keys (the scores are computed twice), split rows are joined in a fixed order.
-#include "common.h"
+#include "gemm_common.h"
 #include "mirage_hip.h"
 
 namespace {
@@ -30,6 +30,10 @@ namespace {
 constexpr float LOG2E_F = 1.4426950408889634f, LN2_F = 0.6931471805599453f;
 constexpr int TT = 64;                        // tokens of a staged tile
 constexpr int MAX_SPLITS = 64;
+#ifndef FWD_OCC
+#define FWD_OCC 3
+#define BWD_OCC 2
+#endif
 
 struct ModArgs {
     const bf16_t* q; const bf16_t* k; const bf16_t* v; bf16_t* o; float* lse;
@@ -49,23 +53,40 @@ struct ModArgs {
 };
 
 // byte offset of 16-byte chunk c of row r in a [TT][HD] bf16 tile; the XOR spreads the rows that one instruction reads over the banks
-template <int HD> __device__ __forceinline__ int toff(int r, int c) {
-    if (HD == 64) return r * 128 + ((c ^ ((r >> 1) & 7)) << 4);
-    return r * 64 + ((c ^ ((r >> 2) & 3)) << 4);
+template <int HD> __device__ __forceinline__ int swz(int r) { return HD == 64 ? (r >> 1) & 7 : (r >> 2) & 3; }
+template <int HD> __device__ __forceinline__ int toff(int r, int c) { return r * HD * 2 + ((c ^ swz<HD>(r)) << 4); }
+__device__ __forceinline__ bf16x8 lds_read16(uint32_t addr, int byte_off) {
+    typedef __attribute__((address_space(3))) bf16x8 lds_v;
+    return *((lds_v*)(uintptr_t)addr + (byte_off >> 4));
 }
-// operand with the contraction along hd: lane -> row row0 + (lane & 31), chunk 2 kk + (lane >> 5)
-template <int HD> __device__ __forceinline__ bf16x8 frag_row(const char* t, int row0, int kk, int lane) {
-    return *reinterpret_cast<const bf16x8*>(t + toff<HD>(row0 + (lane & 31), 2 * kk + (lane >> 5)));
-}
-// operand with the contraction along the tile's rows in accumulator order (rows base + 0..3, base + 8..11, base = row0 + 16 m + 4 (lane >> 5)),
-// lane -> hd element 32 dj + (lane & 31)
-template <int HD> __device__ __forceinline__ bf16x8 frag_col(uint32_t t, int row0, int m, int dj, int lane) {
-    const int i = lane & 15, d = dj * 32 + (lane & 16) + ((i & 3) << 2);
-    const int r = row0 + 16 * m + 4 * (lane >> 5) + (i >> 2);
-    const s16x4 a = lds_read_tr16(t + toff<HD>(r, d >> 3) + ((d & 4) << 1));
-    const s16x4 b = lds_read_tr16(t + toff<HD>(r + 8, d >> 3) + ((d & 4) << 1));
-    return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
-}
+// operand with the contraction along hd: lane -> row (lane & 31) of a block of 32, chunk 2 kk + (lane >> 5); one LDS address per kk, the block of
+// rows is an immediate offset
+template <int HD> struct RowFrag {
+    uint32_t at[HD / 16];
+    __device__ __forceinline__ void init(int lane) {
+#pragma unroll
+        for (int kk = 0; kk < HD / 16; ++kk) at[kk] = (uint32_t)toff<HD>(lane & 31, 2 * kk + (lane >> 5));
+    }
+    __device__ __forceinline__ bf16x8 read(uint32_t tile, int row0, int kk) const { return lds_read16(tile + at[kk], row0 * HD * 2); }
+};
+// operand with the contraction along the tile's rows in accumulator order (rows base + 0..3, base + 8..11, base = row0 + 4 (lane >> 5), row0 a multiple
+// of 16), lane -> hd element 32 dj + (lane & 31)
+template <int HD> struct ColFrag {
+    uint32_t at[HD / 32][2];
+    __device__ __forceinline__ void init(int lane) {
+        const int i = lane & 15, r = 4 * (lane >> 5) + (i >> 2);
+#pragma unroll
+        for (int dj = 0; dj < HD / 32; ++dj) {
+            const int d = dj * 32 + (lane & 16) + ((i & 3) << 2);
+            at[dj][0] = (uint32_t)(toff<HD>(r, d >> 3) + ((d & 4) << 1));
+            at[dj][1] = (uint32_t)(toff<HD>(r + 8, d >> 3) + ((d & 4) << 1));
+        }
+    }
+    __device__ __forceinline__ bf16x8 read(uint32_t tile, int row0, int dj) const {
+        const s16x4 a = lds_read_tr16_off(tile + at[dj][0], row0 * HD * 2), b = lds_read_tr16_off(tile + at[dj][1], row0 * HD * 2);
+        return __builtin_shufflevector(a, b, 0, 1, 2, 3, 4, 5, 6, 7);
+    }
+};
 __device__ __forceinline__ bf16x8 pack_half(const f32x16& s, int m) {
     const uint4 w = make_uint4(pack_bf2(s[8 * m], s[8 * m + 1]), pack_bf2(s[8 * m + 2], s[8 * m + 3]), pack_bf2(s[8 * m + 4], s[8 * m + 5]), pack_bf2(s[8 * m + 6], s[8 * m + 7]));
     return __builtin_bit_cast(bf16x8, w);
@@ -80,7 +101,11 @@ __device__ __forceinline__ bf16x8 pack_rest(const f32x16& s, int m, const bf16x8
     return __builtin_bit_cast(bf16x8, make_uint4(r[0], r[1], r[2], r[3]));
 }
 __device__ __forceinline__ f32x16 zero16() { f32x16 z; for (int i = 0; i < 16; ++i) z[i] = 0.f; return z; }
-__device__ __forceinline__ int reg_row(int r, int lane) { return (r & 3) + 8 * (r >> 2) + 4 * (lane >> 5); }
+// the value of this lane and of its partner in the other half of the wave
+__device__ __forceinline__ float2 halves(float v) {
+    const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
+    return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
+}
 __device__ __forceinline__ int wave_min_i(int v) { for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64)); return v; }
 __device__ __forceinline__ int wave_max_i(int v) { for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64)); return v; }
 
@@ -93,44 +118,60 @@ __device__ __forceinline__ bool not_finite(const uint4 w) {
     return m[0] >= 0x7f80 || m[1] >= 0x7f80;
 }
 
-// ---- staging: a tile of two matrices (X, Y) and of the per-token vectors, global -> registers -> LDS
-template <int HD, int NT>                      // NT threads
-struct Stage {
-    static constexpr int CPR = HD / 8, CH = TT * CPR / NT;      // chunks per row, chunks per thread and matrix
-    uint4 x[CH], y[CH];
-    unsigned bad;                              // bit i / 16 + i: chunk i of x / y lies in a row that does not take part
-    // doc: of the tile's tokens, or null where all of them take part
-    __device__ __forceinline__ void load(const bf16_t* X, long xrs, const bf16_t* Y, long yrs, const int* doc, int row0, int n, int tid) {
-        bad = 0;
+// ---- staging: a tile goes global -> LDS by DMA, 1 KiB (64 chunks of 16 bytes, whole rows) an instruction; the swizzle is applied to the
+// address a lane reads from.  Rows behind the last one repeat it.  NW waves share the blocks of a tile; a wave's are 2 NW apart in parity
+// pairs, so that one offset register per parity serves all of them (the swizzle has a period of 16 rows).
+template <int HD, int NW>
+struct Dma {
+    static constexpr int CPR = HD / 8, RPB = 64 / CPR, NB = TT / RPB, PER = NB / NW;      // rows per block, blocks per tile and per wave
+    static constexpr int PAR = (HD == 64 && NW == 1) ? 2 : 1;
+    uint32_t off[PAR];
+    int rs2, r0, c16;
+    __device__ __forceinline__ int block(int j, int wave) const {                          // j-th block of this wave
+        if (NW == 1) return j;
+        return HD == 64 ? (wave & 1) + 4 * (wave >> 1) + 2 * j : wave;
+    }
+    __device__ __forceinline__ void init(long rs, int lane, int wave) {
+        rs2 = (int)rs * 2;
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const int c = tid + NT * i, r = row0 + c / CPR, e = (c % CPR) * 8;
-            const int rc = min(r, n - 1);
-            x[i] = *reinterpret_cast<const uint4*>(X + (long)rc * xrs + e);
-            y[i] = *reinterpret_cast<const uint4*>(Y + (long)rc * yrs + e);
-            if (r >= n || (doc && doc[rc] < 0)) bad |= 1u << i;
+        for (int p = 0; p < PAR; ++p) {
+            const int r = (PAR == 2 ? p : (HD == 64 ? wave & 1 : 0)) * RPB + lane / CPR;
+            off[p] = (uint32_t)(r * rs2 + (((lane % CPR) ^ swz<HD>(r)) << 4));
         }
     }
-    // CX / CY: replace rows that are not finite by zeros and note them (partial tiles only)
-    template <bool CX, bool CY>
-    __device__ __forceinline__ void store(char* lx, char* ly, unsigned long long* noted, bool partial, int tid) {
-        const uint4 z = make_uint4(0, 0, 0, 0);
+    // rows row0 .. row0 + TT - 1 of `base` (uniform) into `lds`; n: rows there are
+    __device__ __forceinline__ void fetch(const bf16_t* base, int row0, int n, const char* lds, int lane, int wave) const {
+        const char* tile = reinterpret_cast<const char*>(base) + (long)row0 * rs2;
+        const uint32_t dst = lds_addr(lds);
+        if (row0 + TT <= n) {
 #pragma unroll
-        for (int i = 0; i < CH; ++i) {
-            const int c = tid + NT * i, r = c / CPR;
-            uint4 a = x[i], b = y[i];
-            if (partial) {
-                if ((bad >> i) & 1) a = b = z;
-                const bool na = CX && not_finite(a), nb = CY && not_finite(b);
-                if (na) a = z;
-                if (nb) b = z;
-                if (na || nb) atomicOr(noted, 1ull << r);
+            for (int j = 0; j < PER; ++j) {
+                const int b = block(j, wave), odd = HD == 64 ? b & 1 : 0;
+                glds16_s(uniform_ptr(tile + (long)(b - odd) * RPB * rs2), off[PAR == 2 ? odd : 0], __builtin_amdgcn_readfirstlane(dst + b * 1024));
             }
-            *reinterpret_cast<uint4*>(lx + toff<HD>(r, c % CPR)) = a;
-            *reinterpret_cast<uint4*>(ly + toff<HD>(r, c % CPR)) = b;
+        } else {
+#pragma unroll
+            for (int j = 0; j < PER; ++j) {
+                const int b = block(j, wave), r = b * RPB + lane / CPR;
+                const uint32_t o = (uint32_t)(min(r, n - 1 - row0) * rs2 + (((lane % CPR) ^ swz<HD>(r)) << 4));
+                glds16_s(uniform_ptr(tile), o, __builtin_amdgcn_readfirstlane(dst + b * 1024));
+            }
+        }
+    }
+    // this wave's part of a landed tile: values that are not finite become zero, their rows are noted
+    __device__ __forceinline__ void tidy(char* lds, unsigned long long* noted, int lane, int wave) const {
+#pragma unroll
+        for (int j = 0; j < PER; ++j) {
+            const int b = block(j, wave);
+            uint4* at = reinterpret_cast<uint4*>(lds + b * 1024 + lane * 16);
+            if (not_finite(*at)) {
+                *at = make_uint4(0, 0, 0, 0);
+                atomicOr(noted, 1ull << (b * RPB + lane / CPR));
+            }
         }
     }
 };
+__device__ __forceinline__ void dma_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
 // smallest / largest document and number of valid tokens of every 64-token tile of a batch row
 __global__ __launch_bounds__(256) void doc_tiles_kernel(const int* __restrict__ doc, int4* __restrict__ tab, int B, int N, int nt) {
@@ -185,11 +226,30 @@ __device__ __forceinline__ void modify(f32x16& s, f32x16& steep, const ModArgs& 
     }
 }
 
+// scores a lane may not see: registers r with staged row >= left (BELOW) or < left, or another document; `left` and `doc` count from the lane's
+// first row.  x and y take `value` there
+template <bool BELOW>
+__device__ __forceinline__ void hide(f32x16& x, f32x16& y, int left, int mydoc, const int* doc, float value) {
+    asm volatile("" ::: "memory");                               // keeps the test per score behind its branch
+    if (doc) {
+#pragma unroll
+        for (int g = 0; g < 4; ++g) {
+            const int4 d = *reinterpret_cast<const int4*>(doc + 8 * g);
+            const int ds[4] = {d.x, d.y, d.z, d.w};
+#pragma unroll
+            for (int e = 0; e < 4; ++e) if (!((BELOW ? 8 * g + e < left : 8 * g + e >= left) && ds[e] == mydoc)) x[4 * g + e] = y[4 * g + e] = value;
+        }
+    } else {
+#pragma unroll
+        for (int r = 0; r < 16; ++r) if (!(BELOW ? 8 * (r >> 2) + (r & 3) < left : 8 * (r >> 2) + (r & 3) >= left)) x[r] = y[r] = value;
+    }
+}
+
 // ================================================ forward ===============================================
 // NW waves of 32 queries.  NW = 1 serves up to 32 queries (a pooled or a single new token): every workgroup is one wave, and the keys are
 // split over many of them.
 template <int HD, int NW, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * NW, 2) void attn_mod_fwd_kernel(const ModArgs a) {
+__global__ __launch_bounds__(64 * NW, FWD_OCC) void attn_mod_fwd_kernel(const ModArgs a) {
     constexpr int KS = HD / 16, DJ = HD / 32, NT = 64 * NW, TB = TT * HD * 2;
     __shared__ __attribute__((aligned(16))) char ldsK[2][TB];
     __shared__ __attribute__((aligned(16))) char ldsV[2][TB];
@@ -215,15 +275,16 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_mod_fwd_kernel(const ModArgs 
     bf16x8 qf[KS];
 #pragma unroll
     for (int kk = 0; kk < KS; ++kk) qf[kk] = *reinterpret_cast<const bf16x8*>(qp + kk * 16 + 8 * (lane >> 5));
-    const int lim = max(pre, min(qr + off + 1, a.Nk));          // keys below it are visible as far as order goes (qr + off + 1 may be <= 0)
-    const int mydoc = a.doc_q ? a.doc_q[(long)b * a.Nq + qr] : 0;
     float mine[3] = {0.f, 0.f, 0.f};
     float slope2 = 0.f;
     if (BIAS) {
         slope2 = a.slopes[h] * LOG2E_F;
         for (int ax = 0; ax < a.axes; ++ax) mine[ax] = a.pos_q[((long)b * a.Nq + qr) * a.axes + ax];
     }
-    const int wlim_lo = __builtin_amdgcn_readfirstlane(wave_min_i(lim)), wlim_hi = __builtin_amdgcn_readfirstlane(wave_max_i(lim));
+    auto lim_of = [&](int i) { return max(pre, min(i + off + 1, a.Nk)); };               // keys below it are visible as far as order goes (may be <= 0)
+    const int mydoc = a.doc_q ? a.doc_q[(long)b * a.Nq + qr] : 0;
+    const int lim = mydoc < 0 ? 0 : lim_of(qr);                  // padding sees nothing
+    const int wlim_lo = lim_of(min(q0, a.Nq - 1)), wlim_hi = lim_of(min(q0 + 31, a.Nq - 1));      // (documents are tested apart)
     int wlo = 0, whi = 0;
     bool pure = true;
     if (docs) {
@@ -233,7 +294,7 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_mod_fwd_kernel(const ModArgs 
     }
     // the workgroup's ranges: over its 64-row document tiles, and by its first and last row
     const int g0 = blk * 32 * NW, g1 = min(g0 + 32 * NW, a.Nq) - 1;
-    const int glim_lo = max(pre, min(g0 + off + 1, a.Nk)), glim_hi = max(pre, min(g1 + off + 1, a.Nk));
+    const int glim_lo = lim_of(g0), glim_hi = lim_of(g1);
     int glo = 0, ghi = 0;
     bool gpure = true;
     if (docs) {
@@ -278,36 +339,43 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_mod_fwd_kernel(const ModArgs 
     constexpr bool RAW = !CAP && !BIAS;                          // scores stay q.k and the exponent takes the factor
     const float unit = RAW ? a.scale * LOG2E_F : 1.f;
 
-    Stage<HD, NT> st;
-    float pv = 0.f; int dv = 0;
-    auto fetch = [&](int t, bool partial) {
-        st.load(kp, a.k_rs, vp, a.v_rs, partial ? docs : nullptr, t * TT, a.Nk, tid);
-        if (NW == 1) return;
-        // waves 0 .. 2: one axis each, wave 3: the documents
+    RowFrag<HD> fk; fk.init(lane);
+    ColFrag<HD> fv; fv.init(lane);
+    Dma<HD, NW> dk, dv;
+    dk.init(a.k_rs, lane, wave); dv.init(a.v_rs, lane, wave);
+    float pv[NW == 1 ? 3 : 1] = {}; int dc = 0;
+    auto fetch = [&](int t, int buf) {
+        dk.fetch(kp, t * TT, a.Nk, ldsK[buf], lane, wave);
+        dv.fetch(vp, t * TT, a.Nk, ldsV[buf], lane, wave);
         const int r = min(t * TT + lane, a.Nk - 1);
-        if (BIAS && wave < a.axes) pv = posk[(long)r * a.axes + wave];
-        if (docs && wave == NW - 1) dv = docs[r];
-    };
-    auto put = [&](int t, int buf, int slot, bool partial) {
-        st.template store<false, true>(ldsK[buf], ldsV[buf], &noted[slot], partial, tid);
         if (NW == 1) {
-            const int r = min(t * TT + lane, a.Nk - 1);
-            if (BIAS) for (int ax = 0; ax < a.axes; ++ax) ldsP[buf][ax * TT + lane] = posk[(long)r * a.axes + ax];
-            if (docs) ldsD[buf][lane] = docs[r];
-        } else {
-            if (BIAS && wave < a.axes) ldsP[buf][wave * TT + lane] = pv;
-            if (docs && wave == NW - 1) ldsD[buf][lane] = dv;
+            if (BIAS) for (int ax = 0; ax < 3; ++ax) if (ax < a.axes) pv[ax] = posk[(long)r * a.axes + ax];
+            if (docs) dc = docs[r];
+        } else {                                                 // waves 0 .. 2: one axis each, wave 3: the documents
+            if (BIAS && wave < a.axes) pv[0] = posk[(long)r * a.axes + wave];
+            if (docs && wave == NW - 1) dc = docs[r];
         }
+    };
+    auto land = [&](int buf, int slot, bool partial) {
+        if (NW == 1) {
+            if (BIAS) for (int ax = 0; ax < 3; ++ax) if (ax < a.axes) ldsP[buf][ax * TT + lane] = pv[ax];
+            if (docs) ldsD[buf][lane] = dc;
+        } else {
+            if (BIAS && wave < a.axes) ldsP[buf][wave * TT + lane] = pv[0];
+            if (docs && wave == NW - 1) ldsD[buf][lane] = dc;
+        }
+        dma_landed();
+        if (partial) dv.tidy(ldsV[buf], &noted[slot], lane, wave);
     };
     if (tid < 3) noted[tid] = 0;
     __syncthreads();
     bool partial = false, partial_n = false;
     int t = next(partial), buf = 0, slot = 0;
-    if (t >= 0) { fetch(t, partial); put(t, 0, 0, partial); }
+    if (t >= 0) { fetch(t, 0); land(0, 0, partial); }
     __syncthreads();
     while (t >= 0) {
         const int tn = next(partial_n);
-        if (tn >= 0) fetch(tn, partial_n);
+        if (tn >= 0) fetch(tn, buf ^ 1);
         const int slot_n = slot == 2 ? 0 : slot + 1;
         if (tid == 0) noted[slot_n == 2 ? 0 : slot_n + 1] = 0;   // read during the tile before this one, written during the next one
         const int j0 = t * TT;
@@ -318,78 +386,59 @@ __global__ __launch_bounds__(64 * NW, 2) void attn_mod_fwd_kernel(const ModArgs 
             whole = whole && pure && e.x == e.y && e.x == wlo && e.z == TT;
         }
         if (see) {
-            f32x16 s[2];
-            float mx = -INFINITY;
+            const uint32_t kt = lds_addr(ldsK[buf]), vt = lds_addr(ldsV[buf]);
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
-                s[kb] = zero16();
+                f32x16 s = zero16();
 #pragma unroll
-                for (int kk = 0; kk < KS; ++kk) s[kb] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_row<HD>(ldsK[buf], kb * 32, kk, lane), qf[kk], s[kb], 0, 0, 0);
-                f32x16 none;
-                modify<CAP, BIAS, false>(s[kb], none, a, mine, ldsP[buf], kb * 32, slope2, lane);
-                if (!whole) {
-                    asm volatile("" ::: "memory");               // keeps the test per score a branch
+                for (int kk = 0; kk < KS; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fk.read(kt, kb * 32, kk), qf[kk], s, 0, 0, 0);
+                modify<CAP, BIAS, false>(s, s, a, mine, ldsP[buf], kb * 32, slope2, lane);
+                if (!whole) hide<true>(s, s, lim - j0 - kb * 32 - 4 * (lane >> 5), mydoc, docs ? &ldsD[buf][kb * 32 + 4 * (lane >> 5)] : nullptr, -INFINITY);
+                float mx = s[0];
 #pragma unroll
-                    for (int g = 0; g < 4; ++g) {
-                        const int jr = kb * 32 + 8 * g + 4 * (lane >> 5);
-                        int4 d = make_int4(mydoc, mydoc, mydoc, mydoc);
-                        if (docs) d = *reinterpret_cast<const int4*>(&ldsD[buf][jr]);
-                        const int lj = lim - j0 - jr;
-                        const bool on = mydoc >= 0;
-                        if (!(on && lj > 0 && d.x == mydoc)) s[kb][4 * g] = -INFINITY;
-                        if (!(on && lj > 1 && d.y == mydoc)) s[kb][4 * g + 1] = -INFINITY;
-                        if (!(on && lj > 2 && d.z == mydoc)) s[kb][4 * g + 2] = -INFINITY;
-                        if (!(on && lj > 3 && d.w == mydoc)) s[kb][4 * g + 3] = -INFINITY;
-                    }
+                for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
+                const float2 mh = halves(mx);
+                // the reference point moves only when some row of the wave outgrew it by 2^8 (p <= 256 instead of 1): most blocks then skip
+                // the rescale of the 16 HD / 32 output registers
+                const float m_new = fmaxf(m_run, fmaxf(mh.x, mh.y));
+                if (__builtin_amdgcn_ballot_w64((m_new - m_run) * unit > 8.f)) {
+                    const float alpha = m_run == -INFINITY ? 0.f : fast_exp2((m_run - m_new) * unit);
+                    m_run = m_new;
+                    l_run *= alpha;
+#pragma unroll
+                    for (int dj = 0; dj < DJ; ++dj)
+#pragma unroll
+                        for (int r = 0; r < 16; ++r) o[dj][r] *= alpha;
                 }
-#pragma unroll
-                for (int r = 0; r < 16; ++r) mx = fmaxf(mx, s[kb][r]);
-            }
-            mx = fmaxf(mx, __shfl_xor(mx, 32, 64));
-            // the reference point moves only when some row of the wave outgrew it by 2^8 (p <= 256 instead of 1): most tiles then skip the
-            // rescale of the 16 HD / 32 output registers
-            const float m_new = fmaxf(m_run, mx);
-            if (__builtin_amdgcn_ballot_w64((m_new - m_run) * unit > 8.f)) {
-                const float alpha = m_run == -INFINITY ? 0.f : fast_exp2((m_run - m_new) * unit);
-                m_run = m_new;
-                l_run *= alpha;
-#pragma unroll
-                for (int dj = 0; dj < DJ; ++dj)
-#pragma unroll
-                    for (int r = 0; r < 16; ++r) o[dj][r] *= alpha;
-            }
-            const float mu = m_run == -INFINITY ? 0.f : m_run * unit;
-            float l0 = 0.f, l1 = 0.f;
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+                const float mu = m_run == -INFINITY ? 0.f : m_run * unit;
+                float l0 = 0.f, l1 = 0.f;
 #pragma unroll
                 for (int r = 0; r < 16; r += 2) {
-                    s[kb][r] = fast_exp2(RAW ? fmaf(s[kb][r], unit, -mu) : s[kb][r] - mu);
-                    s[kb][r + 1] = fast_exp2(RAW ? fmaf(s[kb][r + 1], unit, -mu) : s[kb][r + 1] - mu);
-                    l0 += s[kb][r]; l1 += s[kb][r + 1];
+                    s[r] = fast_exp2(RAW ? fmaf(s[r], unit, -mu) : s[r] - mu);
+                    s[r + 1] = fast_exp2(RAW ? fmaf(s[r + 1], unit, -mu) : s[r + 1] - mu);
+                    l0 += s[r]; l1 += s[r + 1];
                 }
-            l_run += l0 + l1;
-            const uint32_t vb = lds_addr(ldsV[buf]);
-#pragma unroll
-            for (int kb = 0; kb < 2; ++kb)
+                l_run += l0 + l1;
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
-                    const bf16x8 p = pack_half(s[kb], m);
+                    const bf16x8 p = pack_half(s, m);
 #pragma unroll
-                    for (int dj = 0; dj < DJ; ++dj) o[dj] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_col<HD>(vb, kb * 32, m, dj, lane), p, o[dj], 0, 0, 0);
+                    for (int dj = 0; dj < DJ; ++dj) o[dj] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fv.read(vt, kb * 32 + 16 * m, dj), p, o[dj], 0, 0, 0);
                 }
+            }
             unsigned long long nt = noted[slot];
             while (nt) {
                 const int r = __builtin_ctzll(nt);
                 nt &= nt - 1;
-                if (j0 + r < lim && (!docs || (mydoc >= 0 && ldsD[buf][r] == mydoc))) poisoned = true;
+                if (j0 + r < lim && (!docs || ldsD[buf][r] == mydoc)) poisoned = true;
             }
         }
-        if (tn >= 0) put(tn, buf ^ 1, slot_n, partial_n);
+        if (tn >= 0) land(buf ^ 1, slot_n, partial_n);
         __syncthreads();
         t = tn; buf ^= 1; slot = slot_n;
     }
-    l_run += __shfl_xor(l_run, 32, 64);
+    const float2 lh = halves(l_run);
+    l_run = lh.x + lh.y;
     if (poisoned) l_run = NAN;
     const int row = q0 + (lane & 31);
     if (row >= a.Nq) return;
@@ -446,7 +495,7 @@ __global__ __launch_bounds__(256) void attn_mod_join_kernel(const ModArgs a, int
 //   OWN_K: lane = key, tiles of queries: S = Q K^T,  dP = dO V^T,  dV^T += dO^T P, dK^T += Q^T dS
 // X, Y: the staged matrices (K, V or Q, dO); own fragments: (Q, dO) or (K, V).  OWN_Q also forms sum(do o), which OWN_K reads.
 template <int HD, bool OWN_Q, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, 2) void attn_mod_bwd_kernel(const ModArgs a) {
+__global__ __launch_bounds__(256, BWD_OCC) void attn_mod_bwd_kernel(const ModArgs a) {
     constexpr int KS = HD / 16, DJ = HD / 32, TB = TT * HD * 2;
     __shared__ __attribute__((aligned(16))) char ldsX[2][TB];
     __shared__ __attribute__((aligned(16))) char ldsY[2][TB];
@@ -491,7 +540,8 @@ __global__ __launch_bounds__(256, 2) void attn_mod_bwd_kernel(const ModArgs a) {
 #pragma unroll
                 for (int e = 0; e < 8; ++e) D = fmaf(bf2f((bf16_t)fo[e]), bf2f((bf16_t)fb[kk][e]), D);
             }
-            D += __shfl_xor(D, 32, 64);
+            const float2 dh = halves(D);
+            D = dh.x + dh.y;
             const long at = ((long)b * a.H + ho) * a.Nq + ro;
             lse2 = a.lse[at] * LOG2E_F;
             if (lse2 == -INFINITY) { lse2 = INFINITY; D = 0.f; }                     // a row that saw nothing: p = 2^(s - inf) = 0
@@ -503,7 +553,7 @@ __global__ __launch_bounds__(256, 2) void attn_mod_bwd_kernel(const ModArgs a) {
     if (BIAS) for (int ax = 0; ax < a.axes; ++ax) mine[ax] = (OWN_Q ? a.pos_q : a.pos_k)[((long)b * NO + ro) * a.axes + ax];
     // order: the staged index must be below `edge` (OWN_Q) or at least `edge` (OWN_K); first and last row of the wave and of the workgroup
     auto edge_of = [&](int r) { return OWN_Q ? max(pre, min(r + off + 1, a.Nk)) : (r < pre ? 0 : r - off); };
-    const int edge = edge_of(ro);
+    const int edge = mydoc >= 0 ? edge_of(ro) : (OWN_Q ? 0 : 1 << 30);                // padding sees nothing and is seen by nothing
     const int w1 = min(r0 + 32, NO) - 1, g0 = blk * 128, g1 = min(g0 + 128, NO) - 1;
     const int wedge0 = edge_of(min(r0, NO - 1)), wedge1 = edge_of(w1), gedge0 = edge_of(g0), gedge1 = edge_of(g1);
     int wlo = 0, whi = 0, glo = 0, ghi = 0;
@@ -556,25 +606,33 @@ __global__ __launch_bounds__(256, 2) void attn_mod_bwd_kernel(const ModArgs a) {
     constexpr bool RAW = !CAP && !BIAS;
     const float unit = RAW ? a.scale * LOG2E_F : 1.f;
 
-    Stage<HD, 256> st;
-    float pv = 0.f, lv = 0.f; int dv = 0;
-    auto fetch = [&](int t, int h, bool partial) {
+    RowFrag<HD> fr; fr.init(lane);
+    ColFrag<HD> fc; fc.init(lane);
+    Dma<HD, 4> dx, dy;
+    dx.init(OWN_Q ? a.k_rs : a.q_rs, lane, wave); dy.init(OWN_Q ? a.v_rs : a.do_rs, lane, wave);
+    float pv = 0.f, lv = 0.f; int dc = 0;
+    auto fetch = [&](int t, int h, int buf) {
         const bf16_t* X = OWN_Q ? a.k + (long)b * a.k_bs + (long)(ho / a.G) * a.k_hs : a.q + (long)b * a.q_bs + (long)h * a.q_hs;
         const bf16_t* Y = OWN_Q ? a.v + (long)b * a.v_bs + (long)(ho / a.G) * a.v_hs : a.d_o + (long)b * a.do_bs + (long)h * a.do_hs;
-        st.load(X, OWN_Q ? a.k_rs : a.q_rs, Y, OWN_Q ? a.v_rs : a.do_rs, partial ? doc_s : nullptr, t * TT, NS, tid);
+        dx.fetch(X, t * TT, NS, ldsX[buf], lane, wave);
+        dy.fetch(Y, t * TT, NS, ldsY[buf], lane, wave);
         const int r = min(t * TT + lane, NS - 1);
         if (BIAS && wave < a.axes) pv = pos_s[(long)r * a.axes + wave];
-        if (bydoc && wave == 3) dv = doc_s[r];
+        if (bydoc && wave == 3) dc = doc_s[r];
         if (!OWN_Q && wave < 2) lv = (wave ? a.dsum : a.lse)[((long)b * a.H + h) * a.Nq + r];
     };
-    auto put = [&](int t, int buf, int slot, bool partial) {
-        st.template store<true, !OWN_Q>(ldsX[buf], ldsY[buf], &noted[slot], partial, tid);
+    auto land = [&](int t, int buf, int slot, bool partial) {
         if (BIAS && wave < a.axes) ldsP[buf][wave * TT + lane] = pv;
-        if (bydoc && wave == 3) ldsD[buf][lane] = dv;
+        if (bydoc && wave == 3) ldsD[buf][lane] = dc;
         if (!OWN_Q && wave < 2) {
             const bool in = t * TT + lane < NS;                  // behind the last query: p = 0
             if (wave == 0) ldsL[buf][lane] = (in && lv != -INFINITY) ? lv * LOG2E_F : INFINITY;
             else ldsL[buf][TT + lane] = in ? lv : 0.f;
+        }
+        dma_landed();
+        if (partial) {
+            dx.tidy(ldsX[buf], &noted[slot], lane, wave);
+            if (!OWN_Q) dy.tidy(ldsY[buf], &noted[slot], lane, wave);
         }
     };
     if (tid < 3) noted[tid] = 0;
@@ -582,12 +640,12 @@ __global__ __launch_bounds__(256, 2) void attn_mod_bwd_kernel(const ModArgs a) {
     bool partial = false, partial_n = false;
     int t = next(partial), buf = 0, slot = 0;
     int h = OWN_Q ? ho : ho * a.G + g;
-    if (t >= 0) { fetch(t, h, partial); put(t, 0, 0, partial); }
+    if (t >= 0) { fetch(t, h, 0); land(t, 0, 0, partial); }
     __syncthreads();
     while (t >= 0) {
         const int tn = next(partial_n);
         const int hn = OWN_Q ? ho : ho * a.G + g;
-        if (tn >= 0) fetch(tn, hn, partial_n);
+        if (tn >= 0) fetch(tn, hn, buf ^ 1);
         const int slot_n = slot == 2 ? 0 : slot + 1;
         if (tid == 0) noted[slot_n == 2 ? 0 : slot_n + 1] = 0;   // read during the tile before this one, written during the next one
         const int j0 = t * TT;
@@ -605,9 +663,9 @@ __global__ __launch_bounds__(256, 2) void attn_mod_bwd_kernel(const ModArgs a) {
             for (int kb = 0; kb < 2; ++kb) {
                 f32x16 s = zero16(), dp = zero16(), steep;
 #pragma unroll
-                for (int kk = 0; kk < KS; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_row<HD>(ldsX[buf], kb * 32, kk, lane), fa[kk], s, 0, 0, 0);
+                for (int kk = 0; kk < KS; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.read(xb, kb * 32, kk), fa[kk], s, 0, 0, 0);
 #pragma unroll
-                for (int kk = 0; kk < KS; ++kk) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_row<HD>(ldsY[buf], kb * 32, kk, lane), fb[kk], dp, 0, 0, 0);
+                for (int kk = 0; kk < KS; ++kk) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.read(yb, kb * 32, kk), fb[kk], dp, 0, 0, 0);
                 modify<CAP, BIAS, true>(s, steep, a, mine, ldsP[buf], kb * 32, slope2, lane);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
@@ -623,35 +681,20 @@ __global__ __launch_bounds__(256, 2) void attn_mod_bwd_kernel(const ModArgs a) {
                         if (CAP) dp[r] *= steep[r];
                     }
                 }
-                if (!whole) {
-                    asm volatile("" ::: "memory");               // keeps the test per score a branch
-#pragma unroll
-                    for (int q = 0; q < 4; ++q) {
-                        const int jr = kb * 32 + 8 * q + 4 * (lane >> 5);
-                        int4 d = make_int4(mydoc, mydoc, mydoc, mydoc);
-                        if (bydoc) d = *reinterpret_cast<const int4*>(&ldsD[buf][jr]);
-                        const int ds[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-                        for (int e = 0; e < 4; ++e) {
-                            const int j = j0 + jr + e;
-                            const bool on = (OWN_Q ? j < edge : (j >= edge && j < NS)) && mydoc >= 0 && ds[e] == mydoc;
-                            if (!on) s[4 * q + e] = dp[4 * q + e] = 0.f;
-                        }
-                    }
-                }
+                if (!whole) hide<OWN_Q>(s, dp, edge - j0 - kb * 32 - 4 * (lane >> 5), mydoc, bydoc ? &ldsD[buf][kb * 32 + 4 * (lane >> 5)] : nullptr, 0.f);
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
                     const bf16x8 ds = pack_half(dp, m), rest = pack_rest(dp, m, ds);
 #pragma unroll
                     for (int dj = 0; dj < DJ; ++dj) {
-                        const bf16x8 x = frag_col<HD>(xb, kb * 32, m, dj, lane);
+                        const bf16x8 x = fc.read(xb, kb * 32 + 16 * m, dj);
                         ga[dj] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, ds, ga[dj], 0, 0, 0);
                         ga[dj] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(x, rest, ga[dj], 0, 0, 0);
                     }
                     if (!OWN_Q) {
                         const bf16x8 p = pack_half(s, m);
 #pragma unroll
-                        for (int dj = 0; dj < DJ; ++dj) gb[dj] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(frag_col<HD>(yb, kb * 32, m, dj, lane), p, gb[dj], 0, 0, 0);
+                        for (int dj = 0; dj < DJ; ++dj) gb[dj] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fc.read(yb, kb * 32 + 16 * m, dj), p, gb[dj], 0, 0, 0);
                     }
                 }
             }
@@ -659,10 +702,10 @@ __global__ __launch_bounds__(256, 2) void attn_mod_bwd_kernel(const ModArgs a) {
             while (nt) {
                 const int r = __builtin_ctzll(nt), j = j0 + r;
                 nt &= nt - 1;
-                if ((OWN_Q ? j < edge : j >= edge) && (!bydoc || (mydoc >= 0 && ldsD[buf][r] == mydoc))) poisoned = true;
+                if ((OWN_Q ? j < edge : (j >= edge && j < NS)) && (!bydoc || ldsD[buf][r] == mydoc)) poisoned = true;
             }
         }
-        if (tn >= 0) put(tn, buf ^ 1, slot_n, partial_n);
+        if (tn >= 0) land(tn, buf ^ 1, slot_n, partial_n);
         __syncthreads();
         t = tn; h = hn; buf ^= 1; slot = slot_n;
     }
@@ -759,6 +802,8 @@ int mod_check(const mrg_attn_mod_desc* d, const char* who) {
                 d->B, d->H, d->Hk, d->Nq, d->Nk);
     MRG_REQUIRE(d->Nq <= (1 << 26) && d->Nk <= (1 << 26) && (long)d->B * d->H * (((long)(d->Nq > d->Nk ? d->Nq : d->Nk) + 31) / 32) * MAX_SPLITS <= 0x7fffffffl,
                 MRG_ERR_SHAPE, "%s: too many rows for one launch", who);
+    // a tile's rows are addressed by 32-bit offsets from its first one
+    MRG_REQUIRE((d->Nq <= 1 || (d->q_rs <= (1 << 23) && d->do_rs <= (1 << 23))) && (d->Nk <= 1 || (d->k_rs <= (1 << 23) && d->v_rs <= (1 << 23))), MRG_ERR_SHAPE, "%s: row strides above 2^23 elements", who);
     MRG_REQUIRE(d->scale > 0.f && d->scale < 1e30f, MRG_ERR_ARG, "%s: scale %g must be positive and finite", who, d->scale);
     MRG_REQUIRE(d->cap >= 0.f && d->cap < 1e30f, MRG_ERR_ARG, "%s: cap %g must be 0 (none) or positive", who, d->cap);
     const bool some = d->B > 0 && d->Nq > 0 && d->Nk > 0;        // (tensors without elements may have no address)
