@@ -30,9 +30,14 @@ namespace {
 constexpr float LOG2E_F = 1.4426950408889634f, LN2_F = 0.6931471805599453f;
 constexpr int TT = 64;                        // tokens of a staged tile
 constexpr int MAX_SPLITS = 64;
-#ifndef FWD_OCC
-#define FWD_OCC 3
-#define BWD_OCC 2
+#ifndef WANT1
+#define WANT1 1024
+#define WANTF 512
+#define WANTQ 512
+#define WANTK 512
+#endif
+#ifndef BOCC
+#define BOCC (OWN_Q && !BIAS ? 3 : 2)
 #endif
 
 struct ModArgs {
@@ -173,15 +178,21 @@ struct Dma {
 };
 __device__ __forceinline__ void dma_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// smallest / largest document and number of valid tokens of every 64-token tile of a batch row
-__global__ __launch_bounds__(256) void doc_tiles_kernel(const int* __restrict__ doc, int4* __restrict__ tab, int B, int N, int nt) {
-    const int t = blockIdx.x * 4 + (threadIdx.x >> 6), lane = threadIdx.x & 63;
+// smallest / largest document and number of valid tokens of every 64-token tile of a batch row: the queries' tiles, then the keys' (0 tiles of
+// queries where both sides are the same tokens)
+__global__ __launch_bounds__(256) void doc_tiles_kernel(const int* __restrict__ doc_q, const int* __restrict__ doc_k, int4* __restrict__ tab_q, int4* __restrict__ tab_k,
+                                                        int B, int Nq, int Nk, int ntq, int ntk) {
+    int t = blockIdx.x * 4 + (threadIdx.x >> 6);
+    const int lane = threadIdx.x & 63;
+    const bool ofk = t >= B * ntq;
+    if (ofk) t -= B * ntq;
+    const int nt = ofk ? ntk : ntq, N = ofk ? Nk : Nq;
     if (t >= B * nt) return;
     const int b = t / nt, j = (t - b * nt) * TT + lane;
-    const int d = j < N ? doc[(long)b * N + j] : -1;
+    const int d = j < N ? (ofk ? doc_k : doc_q)[(long)b * N + j] : -1;
     const int lo = wave_min_i(d < 0 ? 0x7fffffff : d), hi = wave_max_i(d);
     const int n = __popcll(__builtin_amdgcn_ballot_w64(d >= 0));
-    if (lane == 0) tab[t] = make_int4(lo, hi, n, 0);
+    if (lane == 0) (ofk ? tab_k : tab_q)[t] = make_int4(lo, hi, n, 0);
 }
 
 // blocks are dispatched round-robin over the 8 dies: give each die one contiguous range of work, so that the row blocks of one head find its
@@ -191,11 +202,10 @@ __device__ __forceinline__ int die_range(int blk, int n) {
     return (die < r ? die * (q + 1) : r * (q + 1) + (die - r) * q) + idx;
 }
 
-// ---- the tiles an owner block walks: 64 at a time, one per lane
-struct Walk {
-    unsigned long long see, part;              // of the current group of 64 tiles: seen by some row; seen, but not whole
-    int base;                                  // first tile of the group
-};
+// ---- the tiles a row block walks, 64 at a time, one per lane: seen by some row of the workgroup; of those, not by every row in whole; seen by
+// the wave; seen by every row of the wave in whole
+struct Walk { unsigned long long see, part, wsee, wwhole; };
+__device__ __forceinline__ int take_tile(unsigned long long& see) { const int i = __builtin_ctzll(see); see &= see - 1; return i; }
 
 // scores in registers -> log2 units (CAP, BIAS) or left raw; steep: 1 - tanh^2
 template <bool CAP, bool BIAS, bool STEEP>
@@ -226,22 +236,27 @@ __device__ __forceinline__ void modify(f32x16& s, f32x16& steep, const ModArgs& 
     }
 }
 
-// scores a lane may not see: registers r with staged row >= left (BELOW) or < left, or another document; `left` and `doc` count from the lane's
-// first row.  x and y take `value` there
-template <bool BELOW>
+// scores a lane may not see take `value` (x; with BOTH, y as well): register r stands for the staged row 8 (r >> 2) + (r & 3) behind the lane's
+// first one, `left` and `doc` (null: order alone decides) count from there; visible below `left` (BELOW) or from it on.  One group of four at
+// a time: all 16 conditions at once are 32 scalar registers that the kernels do not have
+template <bool BELOW, bool BOTH>
 __device__ __forceinline__ void hide(f32x16& x, f32x16& y, int left, int mydoc, const int* doc, float value) {
-    asm volatile("" ::: "memory");                               // keeps the test per score behind its branch
-    if (doc) {
+    asm volatile("" : "+v"(left));                               // the conditions are formed here, not ahead of the branch that rarely comes here
 #pragma unroll
-        for (int g = 0; g < 4; ++g) {
+    for (int g = 0; g < 4; ++g) {
+        bool on[4];
+#pragma unroll
+        for (int e = 0; e < 4; ++e) on[e] = BELOW ? 8 * g + e < left : 8 * g + e >= left;
+        if (doc) {
             const int4 d = *reinterpret_cast<const int4*>(doc + 8 * g);
-            const int ds[4] = {d.x, d.y, d.z, d.w};
-#pragma unroll
-            for (int e = 0; e < 4; ++e) if (!((BELOW ? 8 * g + e < left : 8 * g + e >= left) && ds[e] == mydoc)) x[4 * g + e] = y[4 * g + e] = value;
+            on[0] &= d.x == mydoc; on[1] &= d.y == mydoc; on[2] &= d.z == mydoc; on[3] &= d.w == mydoc;
         }
-    } else {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) if (!(BELOW ? 8 * (r >> 2) + (r & 3) < left : 8 * (r >> 2) + (r & 3) >= left)) x[r] = y[r] = value;
+        for (int e = 0; e < 4; ++e) {
+            x[4 * g + e] = on[e] ? x[4 * g + e] : value;
+            if (BOTH) y[4 * g + e] = on[e] ? y[4 * g + e] : value;
+        }
+        __builtin_amdgcn_sched_barrier(0);
     }
 }
 
@@ -249,7 +264,7 @@ __device__ __forceinline__ void hide(f32x16& x, f32x16& y, int left, int mydoc, 
 // NW waves of 32 queries.  NW = 1 serves up to 32 queries (a pooled or a single new token): every workgroup is one wave, and the keys are
 // split over many of them.
 template <int HD, int NW, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * NW, FWD_OCC) void attn_mod_fwd_kernel(const ModArgs a) {
+__global__ __launch_bounds__(64 * NW, 3) void attn_mod_fwd_kernel(const ModArgs a) {
     constexpr int KS = HD / 16, DJ = HD / 32, NT = 64 * NW, TB = TT * HD * 2;
     __shared__ __attribute__((aligned(16))) char ldsK[2][TB];
     __shared__ __attribute__((aligned(16))) char ldsV[2][TB];
@@ -306,31 +321,6 @@ __global__ __launch_bounds__(64 * NW, FWD_OCC) void attn_mod_fwd_kernel(const Mo
         }
         gpure &= glo == ghi;
     }
-    const int t_lo = (int)((long)split * a.ntk / a.splits), t_hi = (int)((long)(split + 1) * a.ntk / a.splits);
-    Walk wk;
-    auto group = [&](int base) {
-        const int t = base + lane;
-        bool see = t < t_hi && t * TT < glim_hi, whole = t * TT + TT <= glim_lo;
-        if (docs && see) {
-            const int4 e = tab[t];
-            see = e.x <= ghi && e.y >= glo;
-            whole = whole && gpure && e.x == e.y && e.x == glo && e.z == TT;
-        }
-        wk.base = base;
-        wk.see = __builtin_amdgcn_ballot_w64(see);
-        wk.part = __builtin_amdgcn_ballot_w64(see && !whole);
-    };
-    auto next = [&](bool& partial) {                             // the next seen tile, or -1
-        while (wk.see == 0) {
-            if (wk.base + 64 >= t_hi) return -1;
-            group(wk.base + 64);
-        }
-        const int i = __builtin_ctzll(wk.see);
-        wk.see &= wk.see - 1;
-        partial = (wk.part >> i) & 1;
-        return wk.base + i;
-    };
-    group(t_lo);
     f32x16 o[DJ];
 #pragma unroll
     for (int dj = 0; dj < DJ; ++dj) o[dj] = zero16();
@@ -369,31 +359,49 @@ __global__ __launch_bounds__(64 * NW, FWD_OCC) void attn_mod_fwd_kernel(const Mo
     };
     if (tid < 3) noted[tid] = 0;
     __syncthreads();
-    bool partial = false, partial_n = false;
-    int t = next(partial), buf = 0, slot = 0;
-    if (t >= 0) { fetch(t, 0); land(0, 0, partial); }
+    int buf = 0, slot = 0;
+    // a split walks every splits-th tile (runs of neighbouring tiles would be unequal under an order or documents)
+    const int nmine = (a.ntk - split + a.splits - 1) / a.splits;
+    for (int base = 0; base < nmine; base += 64) {
+    Walk wk;
+    {
+        const int i = base + lane, t = split + i * a.splits;
+        bool see = i < nmine && t * TT < glim_hi, whole = t * TT + TT <= glim_lo;
+        bool ws = see && active && t * TT < wlim_hi, ww = t * TT + TT <= wlim_lo;
+        if (docs && see) {
+            const int4 e = tab[t];
+            see = e.x <= ghi && e.y >= glo;
+            whole = whole && gpure && e.x == e.y && e.x == glo && e.z == TT;
+            ws = ws && e.x <= whi && e.y >= wlo;
+            ww = ww && pure && e.x == e.y && e.x == wlo && e.z == TT;
+        }
+        wk.see = __builtin_amdgcn_ballot_w64(see);
+        wk.part = __builtin_amdgcn_ballot_w64(see && !whole);
+        wk.wsee = __builtin_amdgcn_ballot_w64(ws);
+        wk.wwhole = __builtin_amdgcn_ballot_w64(ww);
+    }
+    if (wk.see == 0) continue;
+    int i = take_tile(wk.see);
+    fetch(split + (base + i) * a.splits, buf);
+    land(buf, slot, (wk.part >> i) & 1);
     __syncthreads();
-    while (t >= 0) {
-        const int tn = next(partial_n);
-        if (tn >= 0) fetch(tn, buf ^ 1);
+    while (true) {
+        const int in = wk.see ? take_tile(wk.see) : -1;
+        if (in >= 0) fetch(split + (base + in) * a.splits, buf ^ 1);
         const int slot_n = slot == 2 ? 0 : slot + 1;
         if (tid == 0) noted[slot_n == 2 ? 0 : slot_n + 1] = 0;   // read during the tile before this one, written during the next one
-        const int j0 = t * TT;
-        bool see = active && j0 < wlim_hi, whole = j0 + TT <= wlim_lo;
-        if (docs) {
-            const int4 e = tab[t];
-            see = see && e.x <= whi && e.y >= wlo;
-            whole = whole && pure && e.x == e.y && e.x == wlo && e.z == TT;
-        }
+        const int j0 = (split + (base + i) * a.splits) * TT;
+        const bool see = (wk.wsee >> i) & 1, whole = (wk.wwhole >> i) & 1;
         if (see) {
             const uint32_t kt = lds_addr(ldsK[buf]), vt = lds_addr(ldsV[buf]);
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
+                if (j0 + kb * 32 >= wlim_hi) break;
                 f32x16 s = zero16();
 #pragma unroll
                 for (int kk = 0; kk < KS; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fk.read(kt, kb * 32, kk), qf[kk], s, 0, 0, 0);
                 modify<CAP, BIAS, false>(s, s, a, mine, ldsP[buf], kb * 32, slope2, lane);
-                if (!whole) hide<true>(s, s, lim - j0 - kb * 32 - 4 * (lane >> 5), mydoc, docs ? &ldsD[buf][kb * 32 + 4 * (lane >> 5)] : nullptr, -INFINITY);
+                if (!whole) hide<true, false>(s, s, lim - j0 - kb * 32 - 4 * (lane >> 5), mydoc, docs ? &ldsD[buf][kb * 32 + 4 * (lane >> 5)] : nullptr, -INFINITY);
                 float mx = s[0];
 #pragma unroll
                 for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
@@ -433,9 +441,12 @@ __global__ __launch_bounds__(64 * NW, FWD_OCC) void attn_mod_fwd_kernel(const Mo
                 if (j0 + r < lim && (!docs || ldsD[buf][r] == mydoc)) poisoned = true;
             }
         }
-        if (tn >= 0) land(buf ^ 1, slot_n, partial_n);
+        if (in >= 0) land(buf ^ 1, slot_n, (wk.part >> in) & 1);
         __syncthreads();
-        t = tn; buf ^= 1; slot = slot_n;
+        buf ^= 1; slot = slot_n;
+        if (in < 0) break;
+        i = in;
+    }
     }
     const float2 lh = halves(l_run);
     l_run = lh.x + lh.y;
@@ -495,7 +506,7 @@ __global__ __launch_bounds__(256) void attn_mod_join_kernel(const ModArgs a, int
 //   OWN_K: lane = key, tiles of queries: S = Q K^T,  dP = dO V^T,  dV^T += dO^T P, dK^T += Q^T dS
 // X, Y: the staged matrices (K, V or Q, dO); own fragments: (Q, dO) or (K, V).  OWN_Q also forms sum(do o), which OWN_K reads.
 template <int HD, bool OWN_Q, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, BWD_OCC) void attn_mod_bwd_kernel(const ModArgs a) {
+__global__ __launch_bounds__(256, BOCC) void attn_mod_bwd_kernel(const ModArgs a) {
     constexpr int KS = HD / 16, DJ = HD / 32, TB = TT * HD * 2;
     __shared__ __attribute__((aligned(16))) char ldsX[2][TB];
     __shared__ __attribute__((aligned(16))) char ldsY[2][TB];
@@ -572,33 +583,6 @@ __global__ __launch_bounds__(256, BWD_OCC) void attn_mod_bwd_kernel(const ModArg
     }
     auto order_see = [&](int t, int e0, int e1) { return OWN_Q ? t * TT < e1 : t * TT + TT > e0; };
     auto order_whole = [&](int t, int e0, int e1) { return OWN_Q ? t * TT + TT <= e0 : t * TT >= e1; };
-    const int t_lo = (int)((long)split * nts / a.splits), t_hi = (int)((long)(split + 1) * nts / a.splits);
-    Walk wk;
-    int g = 0;                                                   // OWN_K: the query head of the group
-    auto group = [&](int base) {
-        const int t = base + lane;
-        bool see = t < t_hi && order_see(t, gedge0, gedge1), whole = order_whole(t, gedge0, gedge1) && t * TT + TT <= NS;
-        if (bydoc && see) {
-            const int4 e = tab_s[t];
-            see = e.x <= ghi && e.y >= glo;
-            whole = whole && gpure && e.x == e.y && e.x == glo && e.z == TT;
-        }
-        wk.base = base;
-        wk.see = __builtin_amdgcn_ballot_w64(see);
-        wk.part = __builtin_amdgcn_ballot_w64(see && !whole);
-    };
-    auto next = [&](bool& partial) {
-        while (wk.see == 0) {
-            if (wk.base + 64 < t_hi) group(wk.base + 64);
-            else if (!OWN_Q && g + 1 < a.G) { ++g; group(t_lo); }
-            else return -1;
-        }
-        const int i = __builtin_ctzll(wk.see);
-        wk.see &= wk.see - 1;
-        partial = (wk.part >> i) & 1;
-        return wk.base + i;
-    };
-    group(t_lo);
     f32x16 ga[DJ], gb[OWN_Q ? 1 : DJ];                           // dQ^T, or dK^T and dV^T
 #pragma unroll
     for (int dj = 0; dj < DJ; ++dj) { ga[dj] = zero16(); if (!OWN_Q) gb[dj] = zero16(); }
@@ -611,23 +595,24 @@ __global__ __launch_bounds__(256, BWD_OCC) void attn_mod_bwd_kernel(const ModArg
     Dma<HD, 4> dx, dy;
     dx.init(OWN_Q ? a.k_rs : a.q_rs, lane, wave); dy.init(OWN_Q ? a.v_rs : a.do_rs, lane, wave);
     float pv = 0.f, lv = 0.f; int dc = 0;
-    auto fetch = [&](int t, int h, int buf) {
-        const bf16_t* X = OWN_Q ? a.k + (long)b * a.k_bs + (long)(ho / a.G) * a.k_hs : a.q + (long)b * a.q_bs + (long)h * a.q_hs;
-        const bf16_t* Y = OWN_Q ? a.v + (long)b * a.v_bs + (long)(ho / a.G) * a.v_hs : a.d_o + (long)b * a.do_bs + (long)h * a.do_hs;
+    const bf16_t *X = nullptr, *Y = nullptr;
+    const float* rowv = nullptr;                                 // OWN_K: wave 0 reads lse, wave 1 sum(do o)
+    auto fetch = [&](int t, int buf) {
         dx.fetch(X, t * TT, NS, ldsX[buf], lane, wave);
         dy.fetch(Y, t * TT, NS, ldsY[buf], lane, wave);
         const int r = min(t * TT + lane, NS - 1);
         if (BIAS && wave < a.axes) pv = pos_s[(long)r * a.axes + wave];
         if (bydoc && wave == 3) dc = doc_s[r];
-        if (!OWN_Q && wave < 2) lv = (wave ? a.dsum : a.lse)[((long)b * a.H + h) * a.Nq + r];
+        if (!OWN_Q && wave < 2) lv = rowv[r];
     };
     auto land = [&](int t, int buf, int slot, bool partial) {
         if (BIAS && wave < a.axes) ldsP[buf][wave * TT + lane] = pv;
         if (bydoc && wave == 3) ldsD[buf][lane] = dc;
         if (!OWN_Q && wave < 2) {
-            const bool in = t * TT + lane < NS;                  // behind the last query: p = 0
-            if (wave == 0) ldsL[buf][lane] = (in && lv != -INFINITY) ? lv * LOG2E_F : INFINITY;
-            else ldsL[buf][TT + lane] = in ? lv : 0.f;
+            // negated: raw scores and dp start from them in the accumulators; behind the last query and in rows that saw nothing p = 0
+            const bool in = t * TT + lane < NS;
+            if (wave == 0) ldsL[buf][lane] = (in && lv != -INFINITY) ? lv * (-LOG2E_F / unit) : -INFINITY;
+            else ldsL[buf][TT + lane] = in ? -lv : 0.f;
         }
         dma_landed();
         if (partial) {
@@ -637,31 +622,59 @@ __global__ __launch_bounds__(256, BWD_OCC) void attn_mod_bwd_kernel(const ModArg
     };
     if (tid < 3) noted[tid] = 0;
     __syncthreads();
-    bool partial = false, partial_n = false;
-    int t = next(partial), buf = 0, slot = 0;
-    int h = OWN_Q ? ho : ho * a.G + g;
-    if (t >= 0) { fetch(t, h, 0); land(t, 0, 0, partial); }
+    int buf = 0, slot = 0;
+    const int nmine = (nts - split + a.splits - 1) / a.splits;   // a split walks every splits-th tile
+    for (int g = 0; g < (OWN_Q ? 1 : a.G); ++g) {
+    const int h = OWN_Q ? ho : ho * a.G + g;
+    X = OWN_Q ? a.k + (long)b * a.k_bs + (long)(ho / a.G) * a.k_hs : a.q + (long)b * a.q_bs + (long)h * a.q_hs;
+    Y = OWN_Q ? a.v + (long)b * a.v_bs + (long)(ho / a.G) * a.v_hs : a.d_o + (long)b * a.do_bs + (long)h * a.do_hs;
+    if (!OWN_Q) rowv = (wave ? a.dsum : a.lse) + ((long)b * a.H + h) * a.Nq;
+    for (int base = 0; base < nmine; base += 64) {
+    Walk wk;
+    {
+        const int i = base + lane, t = split + i * a.splits;
+        bool see = i < nmine && order_see(t, gedge0, gedge1), whole = order_whole(t, gedge0, gedge1) && t * TT + TT <= NS;
+        bool ws = see && active && order_see(t, wedge0, wedge1), ww = order_whole(t, wedge0, wedge1) && (!OWN_Q || t * TT + TT <= NS);
+        if (bydoc && see) {
+            const int4 e = tab_s[t];
+            see = e.x <= ghi && e.y >= glo;
+            whole = whole && gpure && e.x == e.y && e.x == glo && e.z == TT;
+            ws = ws && e.x <= whi && e.y >= wlo;
+            ww = ww && pure && e.x == e.y && e.x == wlo && e.z == TT;
+        }
+        wk.see = __builtin_amdgcn_ballot_w64(see);
+        wk.part = __builtin_amdgcn_ballot_w64(see && !whole);
+        wk.wsee = __builtin_amdgcn_ballot_w64(ws);
+        wk.wwhole = __builtin_amdgcn_ballot_w64(ww);
+    }
+    if (wk.see == 0) continue;
+    int i = take_tile(wk.see);
+    { const int t = split + (base + i) * a.splits; fetch(t, buf); land(t, buf, slot, (wk.part >> i) & 1); }
     __syncthreads();
-    while (t >= 0) {
-        const int tn = next(partial_n);
-        const int hn = OWN_Q ? ho : ho * a.G + g;
-        if (tn >= 0) fetch(tn, hn, buf ^ 1);
+    while (true) {
+        const int in = wk.see ? take_tile(wk.see) : -1, tn = split + (base + in) * a.splits;
+        if (in >= 0) fetch(tn, buf ^ 1);
         const int slot_n = slot == 2 ? 0 : slot + 1;
         if (tid == 0) noted[slot_n == 2 ? 0 : slot_n + 1] = 0;   // read during the tile before this one, written during the next one
-        const int j0 = t * TT;
-        bool see = active && order_see(t, wedge0, wedge1), whole = order_whole(t, wedge0, wedge1);
-        if (OWN_Q) whole = whole && j0 + TT <= NS;
-        if (bydoc) {
-            const int4 e = tab_s[t];
-            see = see && e.x <= whi && e.y >= wlo;
-            whole = whole && pure && e.x == e.y && e.x == wlo && e.z == TT;
-        }
+        const int j0 = (split + (base + i) * a.splits) * TT;
+        const bool see = (wk.wsee >> i) & 1, whole = (wk.wwhole >> i) & 1;
         if (see) {
             const float slope2 = BIAS ? a.slopes[h] * LOG2E_F : 0.f;
             const uint32_t xb = lds_addr(ldsX[buf]), yb = lds_addr(ldsY[buf]);
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
+                if (OWN_Q ? j0 + kb * 32 >= wedge1 : j0 + kb * 32 >= NS) break;
+                if (!OWN_Q && j0 + kb * 32 + 32 <= wedge0) continue;
                 f32x16 s = zero16(), dp = zero16(), steep;
+                if (!OWN_Q) {
+#pragma unroll
+                    for (int q = 0; q < 4; ++q) {
+                        const int jr = kb * 32 + 8 * q + 4 * (lane >> 5);
+                        if (RAW) { const float4 L = *reinterpret_cast<const float4*>(&ldsL[buf][jr]); s[4 * q] = L.x; s[4 * q + 1] = L.y; s[4 * q + 2] = L.z; s[4 * q + 3] = L.w; }
+                        const float4 E = *reinterpret_cast<const float4*>(&ldsL[buf][TT + jr]);
+                        dp[4 * q] = E.x; dp[4 * q + 1] = E.y; dp[4 * q + 2] = E.z; dp[4 * q + 3] = E.w;
+                    }
+                }
 #pragma unroll
                 for (int kk = 0; kk < KS; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.read(xb, kb * 32, kk), fa[kk], s, 0, 0, 0);
 #pragma unroll
@@ -669,19 +682,22 @@ __global__ __launch_bounds__(256, BWD_OCC) void attn_mod_bwd_kernel(const ModArg
                 modify<CAP, BIAS, true>(s, steep, a, mine, ldsP[buf], kb * 32, slope2, lane);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
-                    const int jr = kb * 32 + 8 * q + 4 * (lane >> 5);
-                    float4 L = make_float4(lse2, lse2, lse2, lse2), E = make_float4(D, D, D, D);
-                    if (!OWN_Q) { L = *reinterpret_cast<const float4*>(&ldsL[buf][jr]); E = *reinterpret_cast<const float4*>(&ldsL[buf][TT + jr]); }
-                    const float Ls[4] = {L.x, L.y, L.z, L.w}, Es[4] = {E.x, E.y, E.z, E.w};
+                    float4 L = make_float4(-lse2, -lse2, -lse2, -lse2);
+                    if (!OWN_Q && !RAW) L = *reinterpret_cast<const float4*>(&ldsL[buf][kb * 32 + 8 * q + 4 * (lane >> 5)]);
+                    const float Ls[4] = {L.x, L.y, L.z, L.w};
 #pragma unroll
                     for (int e = 0; e < 4; ++e) {
                         const int r = 4 * q + e;
-                        s[r] = fast_exp2(RAW ? fmaf(s[r], unit, -Ls[e]) : s[r] - Ls[e]);
-                        dp[r] = s[r] * (dp[r] - Es[e]);
+                        s[r] = fast_exp2(!RAW ? s[r] + Ls[e] : (OWN_Q ? fmaf(s[r], unit, Ls[e]) : s[r] * unit));
+                        dp[r] = OWN_Q ? s[r] * (dp[r] - D) : s[r] * dp[r];
                         if (CAP) dp[r] *= steep[r];
                     }
                 }
-                if (!whole) hide<OWN_Q>(s, dp, edge - j0 - kb * 32 - 4 * (lane >> 5), mydoc, bydoc ? &ldsD[buf][kb * 32 + 4 * (lane >> 5)] : nullptr, 0.f);
+                if (!whole) {
+                    const int left = edge - j0 - kb * 32 - 4 * (lane >> 5);
+                    const int* doc = bydoc ? &ldsD[buf][kb * 32 + 4 * (lane >> 5)] : nullptr;
+                    hide<OWN_Q, !OWN_Q>(dp, s, left, mydoc, doc, 0.f);
+                }
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
                     const bf16x8 ds = pack_half(dp, m), rest = pack_rest(dp, m, ds);
@@ -705,9 +721,13 @@ __global__ __launch_bounds__(256, BWD_OCC) void attn_mod_bwd_kernel(const ModArg
                 if ((OWN_Q ? j < edge : (j >= edge && j < NS)) && (!bydoc || ldsD[buf][r] == mydoc)) poisoned = true;
             }
         }
-        if (tn >= 0) land(tn, buf ^ 1, slot_n, partial_n);
+        if (in >= 0) land(tn, buf ^ 1, slot_n, (wk.part >> in) & 1);
         __syncthreads();
-        t = tn; h = hn; buf ^= 1; slot = slot_n;
+        buf ^= 1; slot = slot_n;
+        if (in < 0) break;
+        i = in;
+    }
+    }
     }
     if (row >= NO) return;
     const float fa_out = poisoned ? NAN : a.scale, fb_out = poisoned ? NAN : 1.f;
@@ -780,12 +800,12 @@ Plan plan_for(const mrg_attn_mod_desc* d, bool backward) {
         // up to 32 queries: workgroups of one wave, four resident per CU, and the keys cut until every CU has its four
         p.nw = d->Nq <= 32 ? 1 : 4;
         p.nblk = (d->Nq + 32 * p.nw - 1) / (32 * p.nw);
-        p.splits = splits_for((long)d->B * d->H * p.nblk, p.nw == 1 ? 1024 : 512, p.ntk, 4);
+        p.splits = splits_for((long)d->B * d->H * p.nblk, p.nw == 1 ? WANT1 : WANTF, p.ntk, 4);
         if (p.splits > 1) { p.part = take(4l * p.splits * rows_q * d->head_dim); p.part_ml = take(8l * p.splits * rows_q); }
     } else {
         p.dsum = take(4l * rows_q);
-        p.dq_splits = splits_for((long)d->B * d->H * ((d->Nq + 127) / 128), 512, p.ntk, 4);
-        p.dkv_splits = splits_for((long)d->B * d->Hk * ((d->Nk + 127) / 128), 512, p.ntq, 4);
+        p.dq_splits = splits_for((long)d->B * d->H * ((d->Nq + 127) / 128), WANTQ, p.ntk, 4);
+        p.dkv_splits = splits_for((long)d->B * d->Hk * ((d->Nk + 127) / 128), WANTK, p.ntq, 4);
         long part = 0;
         if (p.dq_splits > 1) part = 4l * p.dq_splits * rows_q * d->head_dim;
         if (p.dkv_splits > 1 && 8l * p.dkv_splits * rows_k * d->head_dim > part) part = 8l * p.dkv_splits * rows_k * d->head_dim;
@@ -835,10 +855,12 @@ ModArgs mod_args(const mrg_attn_mod_desc* d, const Plan& p) {
     return a;
 }
 
-void doc_tables(const mrg_attn_mod_desc* d, const ModArgs& a, hipStream_t st) {
+void doc_tables(const mrg_attn_mod_desc* d, const Plan& p, ModArgs& a, hipStream_t st) {
     if (!d->doc_k) return;
-    if (a.ntq) hipLaunchKernelGGL(doc_tiles_kernel, dim3((d->B * a.ntq + 3) / 4), dim3(256), 0, st, d->doc_q, (int4*)a.tab_q, d->B, d->Nq, a.ntq);
-    if (a.ntk) hipLaunchKernelGGL(doc_tiles_kernel, dim3((d->B * a.ntk + 3) / 4), dim3(256), 0, st, d->doc_k, (int4*)a.tab_k, d->B, d->Nk, a.ntk);
+    const bool same = d->doc_q == d->doc_k && d->Nq == d->Nk;
+    if (same) a.tab_q = a.tab_k;
+    const int ntq = same || !d->doc_q ? 0 : p.ntq, tiles = d->B * (ntq + p.ntk);
+    if (tiles) hipLaunchKernelGGL(doc_tiles_kernel, dim3((tiles + 3) / 4), dim3(256), 0, st, d->doc_q, d->doc_k, (int4*)a.tab_q, (int4*)a.tab_k, d->B, d->Nq, d->Nk, ntq, p.ntk);
 }
 
 template <int HD, int NW>
@@ -895,7 +917,7 @@ extern "C" int mrg_attn_mod_fwd(const mrg_attn_mod_desc* d, hipStream_t stream) 
                 && aligned8(d->o, d->o_bs, d->o_rs, d->o_hs), MRG_ERR_ARG, "mrg_attn_mod_fwd: operands and their strides must be multiples of 16 bytes");
     ModArgs a = mod_args(d, p);
     a.nblk = p.nblk; a.splits = p.splits;
-    doc_tables(d, a, stream);
+    doc_tables(d, p, a, stream);
     const dim3 grid((unsigned)((long)a.B * a.H * a.nblk * a.splits));
     if (d->head_dim == 64) { if (p.nw == 1) fwd_go<64, 1>(a, grid, stream); else fwd_go<64, 4>(a, grid, stream); }
     else { if (p.nw == 1) fwd_go<32, 1>(a, grid, stream); else fwd_go<32, 4>(a, grid, stream); }
@@ -918,7 +940,7 @@ extern "C" int mrg_attn_mod_bwd(const mrg_attn_mod_desc* d, hipStream_t stream) 
                 && aligned8(d->dk, d->dk_bs, d->dk_rs, d->dk_hs) && aligned8(d->dv, d->dv_bs, d->dv_rs, d->dv_hs), MRG_ERR_ARG,
                 "mrg_attn_mod_bwd: operands and their strides must be multiples of 16 bytes");
     ModArgs a = mod_args(d, p);
-    doc_tables(d, a, stream);
+    doc_tables(d, p, a, stream);
     bwd_side<true>(a, p.dq_splits, d->head_dim, stream);
     bwd_side<false>(a, p.dkv_splits, d->head_dim, stream);
     return mrg_check_launch("mrg_attn_mod_bwd");
