@@ -35,6 +35,7 @@ constexpr int MAX_SPLITS = 64;
 #define WANTF 512
 #define WANTQ 512
 #define WANTK 512
+#define WANTKC 1024
 #endif
 #ifndef BOCC
 #define BOCC (OWN_Q && !BIAS ? 3 : 2)
@@ -195,11 +196,15 @@ __global__ __launch_bounds__(256) void doc_tiles_kernel(const int* __restrict__ 
     if (lane == 0) (ofk ? tab_k : tab_q)[t] = make_int4(lo, hi, n, 0);
 }
 
-// blocks are dispatched round-robin over the 8 dies: give each die one contiguous range of work, so that the row blocks of one head find its
-// keys in their own L2
-__device__ __forceinline__ int die_range(int blk, int n) {
-    const int q = n >> 3, r = n & 7, die = blk & 7, idx = blk >> 3;
-    return (die < r ? die * (q + 1) : r * (q + 1) + (die - r) * q) + idx;
+// Work of a launch: `heads` (batch, head) pairs of `per` row blocks each.  Workgroups are dispatched round-robin over the 8 dies; a die gets whole
+// heads (where they divide by 8), so that a head's keys stay in its own L2.  Under an order the blocks differ in length, `longest` first: then
+// all heads' longest blocks start first and the short ones fill the end (one head after the other left a quarter of the chip idle behind the
+// last head's long blocks); otherwise a head's blocks follow each other.
+__device__ __forceinline__ void place(int id, int heads, int per, bool by_length, int& head, int& blk) {
+    const int dies = heads % 8 == 0 ? 8 : 1, mine = heads / dies;
+    const int die = id % dies, idx = id / dies;
+    if (by_length) { head = die * mine + idx % mine; blk = idx / mine; }
+    else { head = die * mine + idx / per; blk = idx % per; }
 }
 
 // ---- the tiles a row block walks, 64 at a time, one per lane: seen by some row of the workgroup; of those, not by every row in whole; seen by
@@ -272,10 +277,11 @@ __global__ __launch_bounds__(64 * NW, 3) void attn_mod_fwd_kernel(const ModArgs 
     __shared__ __attribute__((aligned(16))) int ldsD[2][TT];
     __shared__ unsigned long long noted[3];                      // of tile n: slot n % 3
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int w = die_range(blockIdx.x, gridDim.x);
-    int blk = w % a.nblk;
-    const int rest = w / a.nblk, split = rest % a.splits, bh = rest / a.splits, b = bh / a.H, h = bh - b * a.H, hk = h / a.G;
-    if (a.causal) blk = a.nblk - 1 - blk;                       // the longest rows first
+    int bh, blk;
+    place(blockIdx.x, a.B * a.H, a.nblk * a.splits, a.causal, bh, blk);
+    const int split = blk % a.splits, b = bh / a.H, h = bh - b * a.H, hk = h / a.G;
+    blk /= a.splits;
+    if (a.causal) blk = a.nblk - 1 - blk;                       // the last queries see the most
     const bf16_t* kp = a.k + (long)b * a.k_bs + (long)hk * a.k_hs;
     const bf16_t* vp = a.v + (long)b * a.v_bs + (long)hk * a.v_hs;
     const int* docs = a.doc_k ? a.doc_k + (long)b * a.Nk : nullptr;
@@ -515,11 +521,12 @@ __global__ __launch_bounds__(256, BOCC) void attn_mod_bwd_kernel(const ModArgs a
     __shared__ __attribute__((aligned(16))) float ldsL[2][OWN_Q ? 4 : 2 * TT];      // lse (log2 units) and sum(do o) of the staged queries
     __shared__ unsigned long long noted[3];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
-    const int w = die_range(blockIdx.x, gridDim.x);
-    int blk = w % a.nblk;
-    const int rest = w / a.nblk, split = rest % a.splits, bo = rest / a.splits;
-    const int OH = OWN_Q ? a.H : a.Hk, b = bo / OH, ho = bo - b * OH;                 // the owner's head: a query head or a key head
-    if (OWN_Q && a.causal) blk = a.nblk - 1 - blk;                                   // the longest rows first (keys: the first are the longest)
+    const int OH = OWN_Q ? a.H : a.Hk;                                               // the owner's head: a query head or a key head
+    int bo, blk;
+    place(blockIdx.x, a.B * OH, a.nblk * a.splits, a.causal, bo, blk);
+    const int split = blk % a.splits, b = bo / OH, ho = bo - b * OH;
+    blk /= a.splits;
+    if (OWN_Q && a.causal) blk = a.nblk - 1 - blk;                                   // the last queries see the most, the first keys are seen the most
     const int NO = OWN_Q ? a.Nq : a.Nk, NS = OWN_Q ? a.Nk : a.Nq;                    // rows of the owner's side and of the staged side
     const int off = a.Nk - a.Nq;
     const int pre = a.causal ? (a.prefix ? min(max(a.prefix[b], 0), a.Nk) : 0) : a.Nk;
@@ -805,7 +812,7 @@ Plan plan_for(const mrg_attn_mod_desc* d, bool backward) {
     } else {
         p.dsum = take(4l * rows_q);
         p.dq_splits = splits_for((long)d->B * d->H * ((d->Nq + 127) / 128), WANTQ, p.ntk, 4);
-        p.dkv_splits = splits_for((long)d->B * d->Hk * ((d->Nk + 127) / 128), WANTK, p.ntq, 4);
+        p.dkv_splits = splits_for((long)d->B * d->Hk * ((d->Nk + 127) / 128), d->causal ? WANTKC : WANTK, p.ntq, 4);
         long part = 0;
         if (p.dq_splits > 1) part = 4l * p.dq_splits * rows_q * d->head_dim;
         if (p.dkv_splits > 1 && 8l * p.dkv_splits * rows_k * d->head_dim > part) part = 8l * p.dkv_splits * rows_k * d->head_dim;
