@@ -30,8 +30,11 @@ namespace {
 constexpr float LOG2E_F = 1.4426950408889634f, LN2_F = 0.6931471805599453f;
 constexpr int TT = 64;                        // tokens of a staged tile
 constexpr int MAX_SPLITS = 64;
+#ifndef NWF
+#define NWF 4
+#endif
 #ifndef WANT1
-#define WANT1 1024
+#define WANT1 2048
 #define WANTF 512
 #define WANTQ 512
 #define WANTK 512
@@ -135,6 +138,7 @@ struct Dma {
     int rs2, r0, c16;
     __device__ __forceinline__ int block(int j, int wave) const {                          // j-th block of this wave
         if (NW == 1) return j;
+        if (NW == 2) return wave + 2 * j;
         return HD == 64 ? (wave & 1) + 4 * (wave >> 1) + 2 * j : wave;
     }
     __device__ __forceinline__ void init(long rs, int lane, int wave) {
@@ -339,27 +343,24 @@ __global__ __launch_bounds__(64 * NW, 3) void attn_mod_fwd_kernel(const ModArgs 
     ColFrag<HD> fv; fv.init(lane);
     Dma<HD, NW> dk, dv;
     dk.init(a.k_rs, lane, wave); dv.init(a.v_rs, lane, wave);
-    float pv[NW == 1 ? 3 : 1] = {}; int dc = 0;
+    constexpr int AXW = (3 + NW - 1) / NW;                       // the waves share the axes; the last one takes the documents
+    float pv[AXW] = {}; int dc = 0;
     auto fetch = [&](int t, int buf) {
         dk.fetch(kp, t * TT, a.Nk, ldsK[buf], lane, wave);
         dv.fetch(vp, t * TT, a.Nk, ldsV[buf], lane, wave);
         const int r = min(t * TT + lane, a.Nk - 1);
-        if (NW == 1) {
-            if (BIAS) for (int ax = 0; ax < 3; ++ax) if (ax < a.axes) pv[ax] = posk[(long)r * a.axes + ax];
-            if (docs) dc = docs[r];
-        } else {                                                 // waves 0 .. 2: one axis each, wave 3: the documents
-            if (BIAS && wave < a.axes) pv[0] = posk[(long)r * a.axes + wave];
-            if (docs && wave == NW - 1) dc = docs[r];
+        if (BIAS) {
+#pragma unroll
+            for (int x = 0; x < AXW; ++x) if (wave + NW * x < a.axes) pv[x] = posk[(long)r * a.axes + wave + NW * x];
         }
+        if (docs && wave == NW - 1) dc = docs[r];
     };
     auto land = [&](int buf, int slot, bool partial) {
-        if (NW == 1) {
-            if (BIAS) for (int ax = 0; ax < 3; ++ax) if (ax < a.axes) ldsP[buf][ax * TT + lane] = pv[ax];
-            if (docs) ldsD[buf][lane] = dc;
-        } else {
-            if (BIAS && wave < a.axes) ldsP[buf][wave * TT + lane] = pv[0];
-            if (docs && wave == NW - 1) ldsD[buf][lane] = dc;
+        if (BIAS) {
+#pragma unroll
+            for (int x = 0; x < AXW; ++x) if (wave + NW * x < a.axes) ldsP[buf][(wave + NW * x) * TT + lane] = pv[x];
         }
+        if (docs && wave == NW - 1) ldsD[buf][lane] = dc;
         dma_landed();
         if (partial) dv.tidy(ldsV[buf], &noted[slot], lane, wave);
     };
@@ -805,7 +806,7 @@ Plan plan_for(const mrg_attn_mod_desc* d, bool backward) {
     const long rows_q = (long)d->B * d->H * d->Nq, rows_k = (long)d->B * d->Hk * d->Nk;
     if (!backward) {
         // up to 32 queries: workgroups of one wave, four resident per CU, and the keys cut until every CU has its four
-        p.nw = d->Nq <= 32 ? 1 : 4;
+        p.nw = d->Nq <= 32 ? 1 : NWF;
         p.nblk = (d->Nq + 32 * p.nw - 1) / (32 * p.nw);
         p.splits = splits_for((long)d->B * d->H * p.nblk, p.nw == 1 ? WANT1 : WANTF, p.ntk, 4);
         if (p.splits > 1) { p.part = take(4l * p.splits * rows_q * d->head_dim); p.part_ml = take(8l * p.splits * rows_q); }
@@ -926,8 +927,8 @@ extern "C" int mrg_attn_mod_fwd(const mrg_attn_mod_desc* d, hipStream_t stream) 
     a.nblk = p.nblk; a.splits = p.splits;
     doc_tables(d, p, a, stream);
     const dim3 grid((unsigned)((long)a.B * a.H * a.nblk * a.splits));
-    if (d->head_dim == 64) { if (p.nw == 1) fwd_go<64, 1>(a, grid, stream); else fwd_go<64, 4>(a, grid, stream); }
-    else { if (p.nw == 1) fwd_go<32, 1>(a, grid, stream); else fwd_go<32, 4>(a, grid, stream); }
+    if (d->head_dim == 64) { if (p.nw == 1) fwd_go<64, 1>(a, grid, stream); else fwd_go<64, NWF>(a, grid, stream); }
+    else { if (p.nw == 1) fwd_go<32, 1>(a, grid, stream); else fwd_go<32, NWF>(a, grid, stream); }
     if (a.splits > 1) {
         const long threads = (long)a.B * a.H * a.Nq * d->head_dim / 4;
         hipLaunchKernelGGL(attn_mod_join_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, a, d->head_dim);
