@@ -11,7 +11,8 @@
 // so a workgroup carries four sums per column instead of five, whatever the gate's shape.
 //
 // Bound: HBM.  Forward reads 4 + 2 and writes 4 + 2 bytes an element (fp32 residual, bf16 branch and y), backward reads 12 and writes 6.
-// A row is read once into registers (a wave per row up to 1024 columns, four waves beyond), all statistics in fp32: the mean first, then the
+// A row is read once into registers (forward: a wave per row up to 1024 columns, four waves beyond; backward, which carries the column sums
+// and a requested row as well: one wave per 256 columns), all statistics in fp32: the mean first, then the
 // squares of the differences, from registers.  Column sums stay in registers over a workgroup's rows, meet in LDS, and leave as one
 // partial row per workgroup that a second launch adds in a fixed order: no atomics, the same bits on every run.
 #include "common.h"
@@ -25,7 +26,7 @@ struct ResidArgs {
     float* x_new; void* y; int y_f32; float* stats;      // stats [4][M]: post mean, post rstd, pre mean, pre rstd
     int M, L, D, layer; float eps;                        // L: rows that share a gate
     // backward
-    const float* dx_new; const void* dy; int dy_f32; float* dx; void* dbranch;
+    const float* dx_new; const void* dy; int dy_f32, branch_f32; float* dx; void* dbranch;
     float* part;                                          // [grid][4][D]: dw_pre, db_pre, dw_post (or dgate), db_post
     float* gpart;                                         // [samples * parts][D] dgate of each unit
     int parts, units;
@@ -38,6 +39,13 @@ __device__ __forceinline__ float4 rn_load(const void* p, long row, int D, int c,
     if (f32) return reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + row * D)[c];
     return rn_bf4(reinterpret_cast<const uint2*>(reinterpret_cast<const bf16_t*>(p) + row * D)[c]);
 }
+// the same without opening bf16 (a requested row waits in the form it came in)
+__device__ __forceinline__ float4 rn_raw(const void* p, long row, int D, int c, bool f32) {
+    if (f32) return reinterpret_cast<const float4*>(reinterpret_cast<const float*>(p) + row * D)[c];
+    const uint2 u = reinterpret_cast<const uint2*>(reinterpret_cast<const bf16_t*>(p) + row * D)[c];
+    return make_float4(__uint_as_float(u.x), __uint_as_float(u.y), 0.f, 0.f);
+}
+__device__ __forceinline__ float4 rn_open(const float4 v, bool f32) { return f32 ? v : rn_bf4(make_uint2(__float_as_uint(v.x), __float_as_uint(v.y))); }
 __device__ __forceinline__ void rn_store(void* p, long row, int D, int c, bool f32, const float4 v) {
     if (f32) reinterpret_cast<float4*>(reinterpret_cast<float*>(p) + row * D)[c] = v;
     else reinterpret_cast<uint2*>(reinterpret_cast<bf16_t*>(p) + row * D)[c] = make_uint2(pack_bf2(v.x, v.y), pack_bf2(v.z, v.w));
@@ -53,19 +61,22 @@ __device__ __forceinline__ float4 fma4(const float4 a, const float s, const floa
     return make_float4(fmaf(a.x, s, b.x), fmaf(a.y, s, b.y), fmaf(a.z, s, b.z), fmaf(a.w, s, b.w));
 }
 
-// sum over the lanes of a row: its wave, or its four waves through `box` (two alternating sets of slots; every wave of the workgroup calls it
+// sum over the lanes of a row: its wave, or its WPR waves through `box` (two alternating sets of slots; every wave of the workgroup calls it
 // the same number of times)
 template <int WPR>
 struct RowSum {
-    float (*box)[2][4]; int turn = 0, wave;
+    float (*box)[2][WPR]; int turn = 0, wave;
     __device__ __forceinline__ float2 operator()(float a, float b) {
         a = wave_sum(a); b = wave_sum(b);
         if (WPR == 1) return make_float2(a, b);
-        float (&slot)[2][4] = box[turn];
+        float (&slot)[2][WPR] = box[turn];
         turn ^= 1;
         if ((threadIdx.x & 63) == 0) { slot[0][wave] = a; slot[1][wave] = b; }
         __syncthreads();
-        return make_float2((slot[0][0] + slot[0][1]) + (slot[0][2] + slot[0][3]), (slot[1][0] + slot[1][1]) + (slot[1][2] + slot[1][3]));
+        float2 s = make_float2(slot[0][0], slot[1][0]);
+#pragma unroll
+        for (int w = 1; w < WPR; ++w) { s.x += slot[0][w]; s.y += slot[1][w]; }
+        return s;
     }
 };
 
@@ -87,7 +98,7 @@ __device__ __forceinline__ void row_stats(const float4 (&v)[NV], const bool (&ok
 
 template <int NV, int WPR, bool BR32>
 __global__ __launch_bounds__(256) void resid_norm_fwd_kernel(const ResidArgs a) {
-    __shared__ float box[2][2][4];
+    __shared__ float box[2][2][WPR];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
     const int row = WPR == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
     if (WPR == 1 && row >= a.M) return;
@@ -134,124 +145,93 @@ __global__ __launch_bounds__(256) void resid_norm_fwd_kernel(const ResidArgs a) 
     for (int j = 0; j < NV; ++j) if (ok[j]) rn_store(a.y, row, D, c0 + step * j, a.y_f32, scale4(shift4(x[j], mu), rs) * pw[j] + pb[j]);
 }
 
-// SAMPLE: a gate per sample -- the sums A and T are closed at the end of every unit (a part of one sample's rows) into gpart and into the
-// workgroup's own dw_post / db_post; otherwise there is one gate (or none) and they are closed once
-template <int NV, int WPR, bool BR32, bool POST, bool SAMPLE>
-__global__ __launch_bounds__(256) void resid_norm_bwd_kernel(const ResidArgs a) {
-    __shared__ float box[2][2][4];
-    __shared__ __attribute__((aligned(16))) float buf[WPR == 1 ? 4 * NV * 256 : 4];
-    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+// One float4 of a row per lane, WPR waves per row (WPR = 1: four rows side by side).  SAMPLE: a gate per sample -- the sums A and T are closed at the
+// end of every unit (a part of one sample's rows) into gpart and into the workgroup's own dw_post / db_post; otherwise there is one gate (or none)
+// and they are closed once
+template <int WPR, bool POST, bool SAMPLE, bool PRE, bool B32, bool DY32>
+__global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR, 4) void resid_norm_bwd_kernel(const ResidArgs a) {
+    __shared__ float box[2][2][WPR];
+    __shared__ __attribute__((aligned(16))) float buf[WPR == 1 ? 4 * 256 : 4];
+    const int wave = threadIdx.x >> 6;
     RowSum<WPR> sum{box, 0, wave};
-    const int D = a.D, nv = D >> 2, c0 = WPR == 1 ? lane : threadIdx.x, step = 64 * WPR;
+    const int D = a.D, c = WPR == 1 ? threadIdx.x & 63 : threadIdx.x;
     const float invD = 1.f / (float)D;
-    bool ok[NV];
-    float4 pre_w[NV], post_w[NV], g[NV], sw[NV], sb[NV], A[NV], T[NV], GA[NV], GT[NV];
-#pragma unroll
-    for (int j = 0; j < NV; ++j) {
-        const int c = c0 + step * j;
-        ok[j] = c < nv;
-        pre_w[j] = (ok[j] && a.pre_w) ? reinterpret_cast<const float4*>(a.pre_w)[c] : zero4();
-        post_w[j] = (ok[j] && POST) ? reinterpret_cast<const float4*>(a.post_w)[c] : zero4();
-        g[j] = make_float4(1.f, 1.f, 1.f, 1.f);
-        if (!SAMPLE && ok[j] && a.gate) g[j] = reinterpret_cast<const float4*>(a.gate)[c];
-        sw[j] = sb[j] = A[j] = T[j] = GA[j] = GT[j] = zero4();
-    }
-    // one column sum of the workgroup: its waves' registers meet in LDS (a wave per row) or are whole already (a row over four waves)
-    auto flush = [&](const float4 (&v)[NV], float* out) {
+    const bool ok = c < (D >> 2);
+    const int cc = ok ? c : 0;                                    // lanes behind the row read its first chunk and count for nothing
+    auto vec = [&](const float* p) { return p && ok ? reinterpret_cast<const float4*>(p)[c] : zero4(); };
+    const float4 pre_w = vec(PRE ? a.pre_w : nullptr), post_w = vec(POST ? a.post_w : nullptr);
+    float4 g = make_float4(1.f, 1.f, 1.f, 1.f);
+    if (!SAMPLE && a.gate) g = vec(a.gate);
+    float4 sw = zero4(), sb = zero4(), A = zero4(), T = zero4(), GA = zero4(), GT = zero4();
+    // one column sum of the workgroup: its waves' registers meet in LDS (a wave per row) or are whole already
+    auto flush = [&](const float4 v, float* out) {
         if (WPR == 1) {
             __syncthreads();
-#pragma unroll
-            for (int j = 0; j < NV; ++j) if (ok[j]) reinterpret_cast<float4*>(buf + wave * NV * 256)[c0 + step * j] = v[j];
+            if (ok) reinterpret_cast<float4*>(buf + wave * 256)[c] = v;
             __syncthreads();
-            for (int c = threadIdx.x; c < D; c += 256) out[c] = (buf[c] + buf[NV * 256 + c]) + (buf[2 * NV * 256 + c] + buf[3 * NV * 256 + c]);
-        } else {
-#pragma unroll
-            for (int j = 0; j < NV; ++j) if (ok[j]) reinterpret_cast<float4*>(out)[c0 + step * j] = v[j];
-        }
+            for (int i = threadIdx.x; i < D; i += 256) out[i] = (buf[i] + buf[256 + i]) + (buf[512 + i] + buf[768 + i]);
+        } else if (ok) reinterpret_cast<float4*>(out)[c] = v;
     };
     // end of the rows that share a gate: dgate = w_post A + b_post T, and g A, g T towards dw_post, db_post
     auto close = [&](int slot) {
         if (a.gpart) {
-            float4 dg[NV];
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                dg[j] = POST ? A[j] * post_w[j] : A[j];
-                if (POST && ok[j] && a.post_b) dg[j] = dg[j] + T[j] * reinterpret_cast<const float4*>(a.post_b)[c0 + step * j];
-            }
+            float4 dg = POST ? A * post_w : A;
+            if (POST && a.post_b) dg = dg + T * vec(a.post_b);
             flush(dg, a.gpart + (long)slot * D);
         }
-#pragma unroll
-        for (int j = 0; j < NV; ++j) {
-            GA[j] = GA[j] + A[j] * g[j]; GT[j] = GT[j] + T[j] * g[j];
-            if (SAMPLE) A[j] = T[j] = zero4();
-        }
+        GA = GA + A * g; GT = GT + T * g;
+        if (SAMPLE) A = T = zero4();
     };
     const int u0 = (int)((long)blockIdx.x * a.units / gridDim.x), u1 = (int)((long)(blockIdx.x + 1) * a.units / gridDim.x);
     for (int u = u0; u < u1; ++u) {
         const int smp = u / a.parts, part = u - smp * a.parts;
         const int lo = smp * a.L + (int)((long)part * a.L / a.parts), hi = smp * a.L + (int)((long)(part + 1) * a.L / a.parts);
-        if (SAMPLE) {
-#pragma unroll
-            for (int j = 0; j < NV; ++j) if (ok[j]) g[j] = reinterpret_cast<const float4*>(a.gate + (long)smp * a.gate_stride)[c0 + step * j];
-        }
-        for (int row = lo + (WPR == 1 ? wave : 0); row < hi; row += (WPR == 1 ? 4 : 1)) {
-            float4 t[NV], w[NV], xh[NV], b[NV];
-#pragma unroll
-            for (int j = 0; j < NV; ++j) {
-                const int c = c0 + step * j;
-                t[j] = w[j] = xh[j] = b[j] = zero4();
-                if (ok[j]) {
-                    t[j] = rn_load(a.dx_new, row, D, c, true);
-                    b[j] = rn_load(a.branch, row, D, c, BR32);
-                    if (a.pre_w) { w[j] = rn_load(a.dy, row, D, c, a.dy_f32); xh[j] = rn_load(a.x_new, row, D, c, true); }
-                }
-            }
-            if (a.pre_w) {
-                const float mu = a.stats[2l * a.M + row], rs = a.stats[3l * a.M + row];
-                float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-                for (int j = 0; j < NV; ++j) if (ok[j]) {
-                    xh[j] = scale4(shift4(xh[j], mu), rs);
-                    sw[j] = sw[j] + w[j] * xh[j];
-                    sb[j] = sb[j] + w[j];
-                    w[j] = w[j] * pre_w[j];
-                    s1 += sum4(w[j]); s2 += dot4(w[j], xh[j]);
-                }
-                const float2 m = sum(s1, s2);
+        if (SAMPLE) g = vec(a.gate + (long)smp * a.gate_stride);
+        constexpr int RSTEP = WPR == 1 ? 4 : 1;
+        const int first = lo + (WPR == 1 ? wave : 0);
+        // the next row is requested before this one's sums and stores
+        float4 nt = zero4(), nw = zero4(), nx = zero4(), nb = zero4(), nstat = zero4();
+        auto fetch = [&](int row) {
+            nt = rn_load(a.dx_new, row, D, cc, true);
+            nb = rn_raw(a.branch, row, D, cc, B32);
+            if (PRE) { nw = rn_raw(a.dy, row, D, cc, DY32); nx = rn_load(a.x_new, row, D, cc, true); }
+            if (POST) { nstat.x = a.stats[row]; nstat.y = a.stats[(long)a.M + row]; }
+            if (PRE) { nstat.z = a.stats[2l * a.M + row]; nstat.w = a.stats[3l * a.M + row]; }
+        };
+        if (first < hi) fetch(first);
+        for (int row = first; row < hi; row += RSTEP) {
+            float4 t = nt, b = rn_open(nb, B32), w = rn_open(nw, DY32), xh = nx;
+            const float4 stat = nstat;
+            if (!ok) t = b = w = xh = zero4();
+            if (row + RSTEP < hi) fetch(row + RSTEP);
+            if (PRE) {
+                if (ok) xh = scale4(shift4(xh, stat.z), stat.w);
+                sw = sw + w * xh;
+                sb = sb + w;
+                w = w * pre_w;
+                const float2 m = sum(sum4(w), dot4(w, xh));
                 const float m1 = a.layer ? m.x * invD : 0.f, m2 = m.y * invD;
-#pragma unroll
-                for (int j = 0; j < NV; ++j) if (ok[j]) t[j] = fma4(fma4(xh[j], -m2, shift4(w[j], m1)), rs, t[j]);
+                t = fma4(fma4(xh, -m2, shift4(w, m1)), stat.w, t);
             }
-            float rs = 1.f;
+            if (POST && ok) b = scale4(shift4(b, stat.x), stat.y);
+            if (ok) rn_store(a.dx, row, D, c, true, scale4(t, a.alpha));
+            else t = zero4();
+            A = A + t * b;
+            if (POST) T = T + t;
+            t = t * g;
             if (POST) {
-                const float mu = a.stats[row];
-                rs = a.stats[(long)a.M + row];
-#pragma unroll
-                for (int j = 0; j < NV; ++j) if (ok[j]) b[j] = scale4(shift4(b[j], mu), rs);
-            }
-            float s1 = 0.f, s2 = 0.f;
-#pragma unroll
-            for (int j = 0; j < NV; ++j) if (ok[j]) {
-                rn_store(a.dx, row, D, c0 + step * j, true, scale4(t[j], a.alpha));
-                A[j] = A[j] + t[j] * b[j];
-                if (POST) T[j] = T[j] + t[j];
-                t[j] = t[j] * g[j];
-                if (POST) { t[j] = t[j] * post_w[j]; s1 += sum4(t[j]); s2 += dot4(t[j], b[j]); }
-            }
-            if (POST) {
-                const float2 m = sum(s1, s2);
+                t = t * post_w;
+                const float2 m = sum(sum4(t), dot4(t, b));
                 const float m1 = a.layer ? m.x * invD : 0.f, m2 = m.y * invD;
-#pragma unroll
-                for (int j = 0; j < NV; ++j) if (ok[j]) t[j] = scale4(fma4(b[j], -m2, shift4(t[j], m1)), rs);
+                t = scale4(fma4(b, -m2, shift4(t, m1)), stat.y);
             }
-#pragma unroll
-            for (int j = 0; j < NV; ++j) if (ok[j]) rn_store(a.dbranch, row, D, c0 + step * j, BR32, t[j]);
+            if (ok) rn_store(a.dbranch, row, D, c, B32, t);
         }
         if (SAMPLE) close(u);
     }
     if (!SAMPLE) close(blockIdx.x);
     float* out = a.part + (long)blockIdx.x * 4 * D;
-    if (a.pre_w) { flush(sw, out); if (a.pre_b) flush(sb, out + D); }
+    if (PRE) { flush(sw, out); if (a.pre_b) flush(sb, out + D); }
     if (POST) { flush(GA, out + 2 * D); if (a.post_b) flush(GT, out + 3 * D); }
 }
 
@@ -285,7 +265,7 @@ __global__ __launch_bounds__(256) void resid_norm_sum_kernel(const SumArgs a, in
 
 // units of the backward launch: the rows that share a gate, cut into `parts` so that about two workgroups per CU have work, but no part
 // below 16 rows (four per wave) where a gate has that many
-constexpr int RN_GRID = 512;
+constexpr int RN_GRID = 1024;
 int rn_parts(int samples, int L) {
     int parts = (RN_GRID + samples - 1) / samples;
     const int most = (L + 15) / 16;
@@ -293,12 +273,20 @@ int rn_parts(int samples, int L) {
 }
 int rn_grid(long units) { return (int)(units < RN_GRID ? units : RN_GRID); }
 
-template <int NV, int WPR, bool BR32>
-void rn_bwd(const ResidArgs& a, bool post, bool sample, int grid, hipStream_t st) {
-#define RN_GO(P, S) hipLaunchKernelGGL((resid_norm_bwd_kernel<NV, WPR, BR32, P, S>), dim3(grid), dim3(256), 0, st, a)
-    if (post) { if (sample) RN_GO(true, true); else RN_GO(true, false); }
+template <int WPR, bool B32, bool PRE, bool DY32>
+void rn_bwd(const ResidArgs& a, bool sample, int grid, hipStream_t st) {
+#define RN_GO(P, S) hipLaunchKernelGGL((resid_norm_bwd_kernel<WPR, P, S, PRE, B32, DY32>), dim3(grid), dim3(WPR == 1 ? 256 : 64 * WPR), 0, st, a)
+    if (a.post_w) { if (sample) RN_GO(true, true); else RN_GO(true, false); }
     else { if (sample) RN_GO(false, true); else RN_GO(false, false); }
 #undef RN_GO
+}
+// (the operands' types are part of the kernel: chosen at run time they kept the next row's loads from being issued together, 274 -> 399 us at
+// 65792 x 1024)
+template <int WPR>
+void rn_bwd(const ResidArgs& a, bool sample, int grid, hipStream_t st) {
+    if (!a.pre_w) { if (a.branch_f32) rn_bwd<WPR, true, false, false>(a, sample, grid, st); else rn_bwd<WPR, false, false, false>(a, sample, grid, st); }
+    else if (a.dy_f32) { if (a.branch_f32) rn_bwd<WPR, true, true, true>(a, sample, grid, st); else rn_bwd<WPR, false, true, true>(a, sample, grid, st); }
+    else { if (a.branch_f32) rn_bwd<WPR, true, true, false>(a, sample, grid, st); else rn_bwd<WPR, false, true, false>(a, sample, grid, st); }
 }
 
 int rn_check(const mrg_resid_norm_desc* d, const char* who) {
@@ -322,7 +310,7 @@ ResidArgs rn_args(const mrg_resid_norm_desc* d) {
     a.post_w = d->post_w; a.post_b = d->post_b; a.pre_w = d->pre_w; a.pre_b = d->pre_b;
     a.x_new = d->x_new; a.y = d->y; a.y_f32 = d->y_dtype == MRG_DT_F32; a.stats = d->stats;
     a.M = d->samples * d->rows_per_sample; a.L = d->rows_per_sample; a.D = d->D; a.layer = d->norm == MRG_NORM_LAYER; a.eps = d->eps;
-    a.dx_new = d->dx_new; a.dy = d->dy; a.dy_f32 = a.y_f32; a.dx = d->dx; a.dbranch = d->dbranch;
+    a.dx_new = d->dx_new; a.dy = d->dy; a.dy_f32 = a.y_f32; a.branch_f32 = d->branch_dtype == MRG_DT_F32; a.dx = d->dx; a.dbranch = d->dbranch;
     return a;
 }
 
@@ -379,12 +367,12 @@ extern "C" int mrg_resid_norm_bwd(const mrg_resid_norm_desc* d, hipStream_t stre
     const bool gated = d->gate_rows > 0;
     a.part = d->ws; a.gpart = gated ? d->ws + (long)grid * 4 * d->D : nullptr;
     if (a.M) {
-        const bool wide = d->D > 1024, f = d->branch_dtype == MRG_DT_F32, post = d->post_w != nullptr;
-        const int nv = wide ? (d->D + 1023) / 1024 : (d->D + 255) / 256;
-#define RN_B(NV, WPR) do { if (f) rn_bwd<NV, WPR, true>(a, post, sample, grid, stream); else rn_bwd<NV, WPR, false>(a, post, sample, grid, stream); } while (0)
-        if (wide) { if (nv == 2) RN_B(2, 4); else if (nv == 3) RN_B(3, 4); else RN_B(4, 4); }
-        else { if (nv == 1) RN_B(1, 1); else if (nv == 2) RN_B(2, 1); else if (nv == 3) RN_B(3, 1); else RN_B(4, 1); }
-#undef RN_B
+        if (d->D <= 256) rn_bwd<1>(a, sample, grid, stream);
+        else if (d->D <= 512) rn_bwd<2>(a, sample, grid, stream);
+        else if (d->D <= 768) rn_bwd<3>(a, sample, grid, stream);
+        else if (d->D <= 1024) rn_bwd<4>(a, sample, grid, stream);
+        else if (d->D <= 2048) rn_bwd<8>(a, sample, grid, stream);
+        else rn_bwd<16>(a, sample, grid, stream);
     }
     // the partial rows' sums (no rows at all: every gradient is zero)
     SumArgs s = {};

@@ -675,71 +675,92 @@ def attn_bwd(q, k, v, o, lse, d_o, dq, dk, dv, B, H, Nq, Nk, hd, scale, q_stride
 
 
 # ------------------------------------------------------------------------- packed volumes: rotary positions, modified scores, gated residual
-class _On:
-    """Launch on the device the operands live on: its current stream, and the device itself when it is not the current one."""
-    __slots__ = ("dev", "stream", "guard")
-
-    def __init__(self, dev: torch.device):
-        self.dev = dev
-
-    def __enter__(self):
-        self.guard = None
-        if self.dev.index is not None and self.dev.index != torch.cuda.current_device():
-            self.guard = torch.cuda.device(self.dev)
-            self.guard.__enter__()
-        return C.c_void_p(_cur(self.dev).cuda_stream)
-
-    def __exit__(self, *exc):
-        if self.guard is not None:
-            self.guard.__exit__(*exc)
+_raw_stream = torch._C._cuda_getCurrentRawStream      # (the Stream object of torch.cuda.current_stream costs a microsecond of every call)
 
 
-def _want(t: Optional[torch.Tensor], what: str, dev, dtypes, shape=None, contiguous=True):
-    """argument check of the operators below: device, dtype, exact shape, layout"""
-    if t is None:
+def _launch(fn, d, dev: torch.device, what: str):
+    """one C entry point on the device its operands live on: that device's current stream, and the device itself made current if it is not"""
+    i = dev.index
+    if i == torch.cuda.current_device():
+        rc = fn(C.byref(d), _raw_stream(i))
+    else:
+        with torch.cuda.device(dev):
+            rc = fn(C.byref(d), _raw_stream(i))
+    check(rc, what)
+
+
+def _want(t: Optional[torch.Tensor], what: str, dev, dtypes, shape):
+    """argument check of the operators below: device, dtype, exact shape, contiguous.  Accepts at once or says what is wrong"""
+    if t is None or (isinstance(t, torch.Tensor) and t.dtype in dtypes and t.shape == shape and t.device == dev and t.is_contiguous()):
         return
-    if not torch.is_tensor(t):
+    _refuse(t, what, dev, dtypes)
+    if t.shape != shape:
+        raise ValueError(f"mirage_amd: {what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
+    raise ValueError(f"mirage_amd: {what} must be contiguous")
+
+
+def _refuse(t, what: str, dev, dtypes):
+    if not isinstance(t, torch.Tensor):
         raise TypeError(f"mirage_amd: {what} must be a tensor, got {type(t).__name__}")
     _need_cuda(t, what)
     if t.device != dev:
         raise ValueError(f"mirage_amd: {what} is on {t.device}, the other operands on {dev}")
     if t.dtype not in dtypes:
         raise ValueError(f"mirage_amd: {what} must be {' or '.join(str(d) for d in dtypes)}, got {t.dtype}")
-    if shape is not None and tuple(t.shape) != tuple(shape):
-        raise ValueError(f"mirage_amd: {what} must have shape {tuple(shape)}, got {tuple(t.shape)}")
-    if contiguous and not t.is_contiguous():
-        raise ValueError(f"mirage_amd: {what} must be contiguous")
 
 
-def _heads(t: torch.Tensor, what: str, B: int, N: int, dev, dtypes):
-    """[B, N, heads, head_dim] operand with any batch / row / head strides and a contiguous head"""
-    _want(t, what, dev, dtypes, contiguous=False)
-    if t.dim() != 4 or t.shape[0] != B or t.shape[1] != N:
-        raise ValueError(f"mirage_amd: {what} must be [{B}, {N}, heads, head_dim], got {tuple(t.shape)}")
-    if t.numel() and t.shape[3] > 1 and t.stride(3) != 1:
+def _heads(t: torch.Tensor, what: str, B: int, N: int, dev, dtype):
+    """[B, N, heads, head_dim] operand with any batch / row / head strides and a contiguous head: its shape and strides"""
+    if not (isinstance(t, torch.Tensor) and t.dtype is dtype and t.device == dev):
+        _refuse(t, what, dev, (dtype,))
+    shape, stride = t.shape, t.stride()
+    if len(shape) != 4 or shape[0] != B or shape[1] != N:
+        raise ValueError(f"mirage_amd: {what} must be [{B}, {N}, heads, head_dim], got {tuple(shape)}")
+    if stride[3] != 1 and shape[3] > 1 and t.numel():
         raise ValueError(f"mirage_amd: {what}: the head dimension must be contiguous")
+    return shape, stride
 
 
-def _no_overlap(out: torch.Tensor, src: torch.Tensor, what: str):
-    """an output is its input (in place) or lies apart from it"""
-    if out.numel() == 0 or (out.data_ptr() == src.data_ptr() and out.stride() == src.stride()):
-        return
-    span = lambda t: (t.data_ptr(), t.data_ptr() + t.element_size() * (1 + sum((n - 1) * s for n, s in zip(t.shape, t.stride()))))
-    (a0, a1), (b0, b1) = span(out), span(src)
-    if a0 < b1 and b0 < a1 and out.untyped_storage().data_ptr() == src.untyped_storage().data_ptr() and not _interleaved_apart(out, src):
-        raise ValueError(f"mirage_amd: {what} overlaps an operand of another layout")
+def _out_heads(t: torch.Tensor, what: str, shape, dev, dtype):
+    """a destination: like _heads, of the given shape, no two elements in one place"""
+    got, st = _heads(t, what, shape[0], shape[1], dev, dtype)
+    if got != shape:
+        raise ValueError(f"mirage_amd: {what} must have shape {tuple(shape)}, got {tuple(got)}")
+    head = (got[2] - 1) * st[2] + got[3]
+    if st[2] < got[3] or st[1] < head or st[0] < (got[1] - 1) * st[1] + head:          # not simply batch > row > head: any order without overlap
+        room = 1
+        for n, s in sorted(((n, s) for n, s in zip(got, st) if n > 1), key=lambda ns: ns[1]):
+            if s < room:
+                raise ValueError(f"mirage_amd: {what} has elements in the same place (strides {tuple(st)})")
+            room = s * (n - 1) + room
+    return st
 
 
-def _interleaved_apart(a: torch.Tensor, b: torch.Tensor) -> bool:
-    """column blocks of the same rows (views into one fused projection buffer): same strides, and their head blocks do not meet"""
-    if a.stride() != b.stride() or a.dim() != 4:
-        return False
-    row = a.stride(1)
-    d = (b.data_ptr() - a.data_ptr()) // a.element_size() % row if row else 0
-    width = lambda t: (t.shape[2] - 1) * t.stride(2) + t.shape[3]
-    return width(a) <= d and d + width(b) <= row
+def _apart(a: torch.Tensor, b: torch.Tensor) -> bool:
+    """do two [B, N, heads, head_dim] tensors share no memory: column blocks of the same rows (views into one fused buffer), or spans that do not meet"""
+    if a.numel() == 0 or b.numel() == 0:
+        return True
+    pa, pb, sa, sb, na, nb = a.data_ptr(), b.data_ptr(), a.stride(), b.stride(), a.shape, b.shape
+    ea, eb = a.element_size(), b.element_size()
+    if sa == sb and ea == eb and sa[1] and (sa[0] % sa[1] == 0 or na[0] == 1):
+        d = (pb - pa) // ea % sa[1]
+        if (na[2] - 1) * sa[2] + na[3] <= d and d + (nb[2] - 1) * sb[2] + nb[3] <= sa[1]:
+            return True
+    end = lambda p, n, s, e: p + e * (1 + (n[0] - 1) * s[0] + (n[1] - 1) * s[1] + (n[2] - 1) * s[2] + (n[3] - 1) * s[3])  # noqa: E731
+    return end(pa, na, sa, ea) <= pb or end(pb, nb, sb, eb) <= pa
 
 
+def _need_apart(out: torch.Tensor, src: torch.Tensor, what: str):
+    if not _apart(out, src):
+        raise ValueError(f"mirage_amd: {what} overlaps another operand")
+
+
+def _in_place(out: torch.Tensor, src: torch.Tensor) -> bool:
+    return out is src or (out.data_ptr() == src.data_ptr() and out.stride() == src.stride())
+
+
+_F64, _FLOATS, _POS, _I32, _ONLY32 = (torch.float64,), (BF16, F32), (torch.int32, F32), (torch.int32,), (F32,)
+_NO_STRIDE = (0, 0, 0, 0)
 _PAIRING = {"half": L.MRG_PAIR_HALF, "interleaved": L.MRG_PAIR_INTERLEAVED, "axial": L.MRG_PAIR_AXIAL}
 
 
@@ -752,58 +773,60 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], pos: torch.Tensor, f
     or "axial" (half inside each axis' own span).  inverse: by the negative angle, which is the gradient's rotation.
     out_q / out_k: destinations (the inputs themselves for in place); default new contiguous tensors.  Returns (q', k')."""
     _need_cuda(q, "rotary q")
-    dev, dt = q.device, q.dtype
-    if q.dim() != 4 or dt not in (BF16, F32):
-        raise ValueError(f"mirage_amd: rotary q must be bf16 or fp32 [B, N, heads, head_dim], got {dt} {tuple(q.shape)}")
-    B, N, Hq, hd = q.shape
-    _heads(q, "rotary q", B, N, dev, (dt,))
-    if pairing not in _PAIRING:
+    dev, dt, shape = q.device, q.dtype, q.shape
+    if len(shape) != 4 or (dt is not BF16 and dt is not F32):
+        raise ValueError(f"mirage_amd: rotary q must be bf16 or fp32 [B, N, heads, head_dim], got {dt} {tuple(shape)}")
+    B, N, Hq, hd = shape
+    _, qs = _heads(q, "rotary q", B, N, dev, dt)
+    kind = _PAIRING.get(pairing)
+    if kind is None:
         raise ValueError(f"mirage_amd: pairing {pairing!r} is none of {sorted(_PAIRING)}")
-    sections = tuple(int(s) for s in sections)
-    if not 1 <= len(sections) <= L.MRG_MAX_AXES or min(sections) < 1 or 2 * sum(sections) > hd:
-        raise ValueError(f"mirage_amd: sections {sections}: 1 to {L.MRG_MAX_AXES} axes of at least one pair, together at most {hd // 2} pairs of a head of {hd}")
-    _want(freqs, "rotary freqs", dev, (torch.float64,), (sum(sections),))
-    _want(pos, "rotary positions", dev, (torch.int32, F32), (N, len(sections)) if pos.dim() == 2 else (B, N, len(sections)), contiguous=False)
-    if pos.numel() and len(sections) > 1 and pos.stride(-1) != 1:
+    axes = len(sections)
+    if not 1 <= axes <= L.MRG_MAX_AXES or min(sections) < 1 or 2 * sum(sections) > hd:
+        raise ValueError(f"mirage_amd: sections {tuple(sections)}: 1 to {L.MRG_MAX_AXES} axes of at least one pair, together at most {hd // 2} pairs of a head of {hd}")
+    _want(freqs, "rotary freqs", dev, _F64, (sum(sections),))
+    if not (isinstance(pos, torch.Tensor) and pos.device == dev and pos.dtype in _POS):
+        _refuse(pos, "rotary positions", dev, _POS)
+    shared = pos.dim() == 2
+    if pos.shape != ((N, axes) if shared else (B, N, axes)):
+        raise ValueError(f"mirage_amd: rotary positions must be [{B}, {N}, {axes}] or [{N}, {axes}], got {tuple(pos.shape)}")
+    ps = pos.stride()
+    if ps[-1] != 1 and axes > 1 and pos.numel():
         raise ValueError("mirage_amd: rotary positions: the axes must be contiguous")
-    d = L.RotaryDesc()
-    d.dtype, d.B, d.N, d.Hq, d.head_dim = (L.MRG_DT_BF16 if dt == BF16 else L.MRG_DT_F32), B, N, Hq, hd
     if out_q is None:
-        out_q = torch.empty((B, N, Hq, hd), dtype=dt, device=dev)
+        out_q = torch.empty(shape, dtype=dt, device=dev)
+        qos = out_q.stride()
     else:
-        _heads(out_q, "rotary out_q", B, N, dev, (dt,))
-        if out_q.shape != q.shape:
-            raise ValueError("mirage_amd: rotary out_q must have the shape of q")
-        _no_overlap(out_q, q, "rotary out_q")
-    d.q, d.q_out = q.data_ptr(), out_q.data_ptr()
-    d.q_bs, d.q_rs, d.q_hs, _ = q.stride()
-    d.qo_bs, d.qo_rs, d.qo_hs, _ = out_q.stride()
+        qos = _out_heads(out_q, "rotary out_q", shape, dev, dt)
+        if not _in_place(out_q, q):
+            _need_apart(out_q, q, "rotary out_q")
+        if k is not None:
+            _need_apart(out_q, k, "rotary out_q")
+    k_ptr = ko_ptr = None
+    Hk, ks, kos = 0, _NO_STRIDE, _NO_STRIDE
     if k is not None:
-        _heads(k, "rotary k", B, N, dev, (dt,))
-        if k.shape[3] != hd:
-            raise ValueError(f"mirage_amd: rotary k has heads of {k.shape[3]}, q of {hd}")
+        kshape, ks = _heads(k, "rotary k", B, N, dev, dt)
+        if kshape[3] != hd:
+            raise ValueError(f"mirage_amd: rotary k has heads of {kshape[3]}, q of {hd}")
+        Hk = kshape[2]
         if out_k is None:
-            out_k = torch.empty(k.shape, dtype=dt, device=dev)
+            out_k = torch.empty(kshape, dtype=dt, device=dev)
+            kos = out_k.stride()
         else:
-            _heads(out_k, "rotary out_k", B, N, dev, (dt,))
-            if out_k.shape != k.shape:
-                raise ValueError("mirage_amd: rotary out_k must have the shape of k")
-            _no_overlap(out_k, k, "rotary out_k")
-            _no_overlap(out_k, q, "rotary out_k")
-        if out_q.data_ptr() != q.data_ptr():
-            _no_overlap(out_q, k, "rotary out_q")
-        d.Hk, d.k, d.k_out = k.shape[2], k.data_ptr(), out_k.data_ptr()
-        d.k_bs, d.k_rs, d.k_hs, _ = k.stride()
-        d.ko_bs, d.ko_rs, d.ko_hs, _ = out_k.stride()
+            kos = _out_heads(out_k, "rotary out_k", kshape, dev, dt)
+            here = _in_place(out_k, k)
+            if not here:
+                _need_apart(out_k, k, "rotary out_k")
+            if not (here and out_q is q):                         # (both in place: q and k were found apart above)
+                _need_apart(out_k, q, "rotary out_k")
+                _need_apart(out_k, out_q, "rotary out_k")
+        k_ptr, ko_ptr = k.data_ptr(), out_k.data_ptr()
     elif out_k is not None:
         raise ValueError("mirage_amd: rotary out_k without k")
-    d.pos, d.pos_dtype = pos.data_ptr(), (L.MRG_POS_I32 if pos.dtype == torch.int32 else L.MRG_POS_F32)
-    d.pos_bs, d.pos_rs = (0 if pos.dim() == 2 else pos.stride(0)), pos.stride(-2)
-    d.freqs, d.axes, d.pairing, d.inverse = freqs.data_ptr(), len(sections), _PAIRING[pairing], int(bool(inverse))
-    for i, s in enumerate(sections):
-        d.sections[i] = s
-    with _On(dev) as st:
-        check(lib.mrg_rotary_axes(C.byref(d), st), "mrg_rotary_axes")
+    d = L.RotaryDesc(q.data_ptr(), k_ptr, out_q.data_ptr(), ko_ptr, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], qos[0], qos[1], qos[2], kos[0], kos[1], kos[2],
+                     L.MRG_DT_BF16 if dt is BF16 else L.MRG_DT_F32, B, N, Hq, Hk, hd, L.MRG_POS_F32 if pos.dtype is F32 else L.MRG_POS_I32, pos.data_ptr(),
+                     0 if shared else ps[0], ps[-2], freqs.data_ptr(), axes, tuple(sections), kind, 1 if inverse else 0)
+    _launch(lib.mrg_rotary_axes, d, dev, "mrg_rotary_axes")
     return out_q, out_k
 
 
@@ -811,35 +834,35 @@ _NORM_KIND = {"layer": L.MRG_NORM_LAYER, "rms": L.MRG_NORM_RMS}
 
 
 def _resid_norm_desc(rows_like, branch, gate, alpha, post, pre, kind, eps, y_dtype):
-    dev = rows_like.device
-    _want(rows_like, "resid_norm residual", dev, (F32,))
-    _want(branch, "resid_norm branch", dev, (BF16, F32), rows_like.shape)
-    if rows_like.dim() < 2 or kind not in _NORM_KIND:
-        raise ValueError(f"mirage_amd: resid_norm takes rows [..., D] and kind 'layer' or 'rms', got {tuple(rows_like.shape)}, {kind!r}")
-    D = rows_like.shape[-1]
+    dev, shape = rows_like.device, rows_like.shape
+    _want(rows_like, "resid_norm residual", dev, _ONLY32, shape)
+    _want(branch, "resid_norm branch", dev, _FLOATS, shape)
+    norm = _NORM_KIND.get(kind)
+    if len(shape) < 2 or norm is None or branch is None:
+        raise ValueError(f"mirage_amd: resid_norm takes a residual and a branch of rows [samples, ..., D] and kind 'layer' or 'rms', got {tuple(shape)}, {kind!r}")
+    S, D = shape[0], shape[-1]
     if D % 4 or not 4 <= D <= 4096:
         raise ValueError(f"mirage_amd: resid_norm rows must be a multiple of 4 and at most 4096 wide, got {D}")
-    S = rows_like.shape[0]
-    d = L.ResidNormDesc()
-    d.samples, d.rows_per_sample, d.D = S, (rows_like.numel() // (S * D) if S else 0), D
-    d.norm, d.alpha, d.eps = _NORM_KIND[kind], float(alpha), float(eps)
-    d.branch_dtype = L.MRG_DT_BF16 if branch.dtype == BF16 else L.MRG_DT_F32
-    d.y_dtype = L.MRG_DT_BF16 if y_dtype == BF16 else L.MRG_DT_F32
+    M = rows_like.numel() // D
+    vec = (D,)
+    gate_ptr, gate_rows = None, 0
     if gate is not None:
-        _want(gate, "resid_norm gate", dev, (F32,), (D,) if gate.dim() == 1 else (S, D))
-        d.gate, d.gate_rows = gate.data_ptr(), (1 if gate.dim() == 1 else S)
+        gate_rows = 1 if gate.dim() == 1 else S
+        _want(gate, "resid_norm gate", dev, _ONLY32, vec if gate.dim() == 1 else (S, D))
+        gate_ptr = gate.data_ptr()
+    ptrs = []
     for name, wb in (("post", post), ("pre", pre)):
-        if wb is None:
-            continue
-        w, b = wb
-        _want(w, f"resid_norm {name} weight", dev, (F32,), (D,))
-        _want(b, f"resid_norm {name} bias", dev, (F32,), (D,))
-        if w is None:
-            raise ValueError(f"mirage_amd: resid_norm {name} norm without a weight")
-        setattr(d, name + "_w", w.data_ptr())
-        setattr(d, name + "_b", _p(b))
-    d.branch = branch.data_ptr()
-    return d, D, S, dev
+        w = b = None
+        if wb is not None:
+            w, b = wb
+            _want(w, f"resid_norm {name} weight", dev, _ONLY32, vec)
+            _want(b, f"resid_norm {name} bias", dev, _ONLY32, vec)
+            if w is None:
+                raise ValueError(f"mirage_amd: resid_norm {name} norm without a weight")
+        ptrs += (_p(w), _p(b))
+    d = L.ResidNormDesc(S, M // S if S else 0, D, norm, L.MRG_DT_BF16 if branch.dtype is BF16 else L.MRG_DT_F32, L.MRG_DT_BF16 if y_dtype is BF16 else L.MRG_DT_F32,
+                        gate_rows, alpha, eps, None, branch.data_ptr(), gate_ptr, *ptrs)
+    return d, D, M, dev
 
 
 def resid_norm_fwd(x: torch.Tensor, branch: torch.Tensor, *, gate: Optional[torch.Tensor] = None, alpha: float = 1.0, post=None, pre=None, kind: str = "layer",
@@ -848,15 +871,19 @@ def resid_norm_fwd(x: torch.Tensor, branch: torch.Tensor, *, gate: Optional[torc
     x fp32 [samples, ..., D], branch bf16 or fp32 of the same shape, both contiguous; gate fp32 [D] or [samples, D] or None; post / pre = (weight,
     bias or None) fp32 [D] or None (no norm there; without pre there is no y).  kind: "layer" or "rms".  Returns (x', y or None, stats)."""
     _need_cuda(x, "resid_norm residual")
-    if out_dtype not in (BF16, F32):
+    if out_dtype is not BF16 and out_dtype is not F32:
         raise ValueError(f"mirage_amd: resid_norm out_dtype must be bf16 or fp32, got {out_dtype}")
-    d, D, S, dev = _resid_norm_desc(x, branch, gate, alpha, post, pre, kind, eps, out_dtype)
+    d, D, M, dev = _resid_norm_desc(x, branch, gate, alpha, post, pre, kind, eps, out_dtype)
     x_new = torch.empty_like(x)
-    y = torch.empty(x.shape, dtype=out_dtype, device=dev) if pre is not None else None
-    stats = torch.empty((4, x.numel() // D), dtype=F32, device=dev) if (pre is not None or post is not None) else None
-    d.x, d.x_new, d.y, d.stats = x.data_ptr(), x_new.data_ptr(), _p(y), _p(stats)
-    with _On(dev) as st:
-        check(lib.mrg_resid_norm_fwd(C.byref(d), st), "mrg_resid_norm_fwd")
+    d.x, d.x_new = x.data_ptr(), x_new.data_ptr()
+    y = stats = None
+    if pre is not None:
+        y = torch.empty_like(x, dtype=out_dtype)
+        d.y = y.data_ptr()
+    if pre is not None or post is not None:
+        stats = torch.empty((4, M), dtype=F32, device=dev)
+        d.stats = stats.data_ptr()
+    _launch(lib.mrg_resid_norm_fwd, d, dev, "mrg_resid_norm_fwd")
     return x_new, y, stats
 
 
@@ -869,32 +896,37 @@ def resid_norm_bwd(dx_new: torch.Tensor, dy: Optional[torch.Tensor], x_new: torc
     _need_cuda(dx_new, "resid_norm gradient")
     if (pre is None) != (dy is None):
         raise ValueError("mirage_amd: resid_norm_bwd needs dy exactly when there is a pre norm")
-    if dy is not None:
-        _want(dy, "resid_norm dy", dx_new.device, (BF16, F32), dx_new.shape)
-    d, D, S, dev = _resid_norm_desc(dx_new, branch, gate, alpha, post, pre, kind, eps, dy.dtype if dy is not None else BF16)
-    _want(x_new, "resid_norm x_new", dev, (F32,), dx_new.shape)
-    if pre is not None or post is not None:
-        if stats is None:
-            raise ValueError("mirage_amd: resid_norm_bwd needs the forward pass's stats")
-        _want(stats, "resid_norm stats", dev, (F32,), (4, dx_new.numel() // D))
+    _want(dy, "resid_norm dy", dx_new.device, _FLOATS, dx_new.shape)
+    d, D, M, dev = _resid_norm_desc(dx_new, branch, gate, alpha, post, pre, kind, eps, dy.dtype if dy is not None else BF16)
+    if x_new is None or (stats is None and (pre is not None or post is not None)):
+        raise ValueError("mirage_amd: resid_norm_bwd needs the forward pass's x_new and stats")
+    _want(x_new, "resid_norm x_new", dev, _ONLY32, dx_new.shape)
+    _want(stats, "resid_norm stats", dev, _ONLY32, (4, M))
     dx, dbranch = torch.empty_like(dx_new), torch.empty_like(branch)
     made: Dict[str, torch.Tensor] = {}
+    todo = []                                                     # (name, descriptor field) of the vectors without a given destination
     for name, field, src in (("gate", "d_gate", gate), ("post_weight", "d_post_w", post and post[0]), ("post_bias", "d_post_b", post and post[1]),
                              ("pre_weight", "d_pre_w", pre and pre[0]), ("pre_bias", "d_pre_b", pre and pre[1])):
         if src is None:
             continue
         g = grads.get(name) if grads is not None else None
+        if g is None and src.dim() == 1:
+            todo.append((name, field))
+            continue
         if g is None:
             g = torch.empty_like(src)
         else:
-            _want(g, f"resid_norm gradient {name}", dev, (F32,), src.shape)
+            _want(g, f"resid_norm gradient {name}", dev, _ONLY32, src.shape)
         made[name] = g
         setattr(d, field, g.data_ptr())
+    if todo:
+        for (name, field), g in zip(todo, torch.empty((len(todo), D), dtype=F32, device=dev).unbind(0)):
+            made[name] = g
+            setattr(d, field, g.data_ptr())
     ws = torch.empty(lib.mrg_resid_norm_ws_floats(C.byref(d)), dtype=F32, device=dev)
     d.x_new, d.stats, d.dx_new, d.dy, d.dx, d.dbranch, d.ws = (x_new.data_ptr(), _p(stats), dx_new.data_ptr(), _p(dy), dx.data_ptr(), dbranch.data_ptr(),
                                                                ws.data_ptr())
-    with _On(dev) as st:
-        check(lib.mrg_resid_norm_bwd(C.byref(d), st), "mrg_resid_norm_bwd")
+    _launch(lib.mrg_resid_norm_bwd, d, dev, "mrg_resid_norm_bwd")
     return dx, dbranch, made
 
 
@@ -923,48 +955,48 @@ class ScoreMod:
 def _attn_mod_desc(q, k, v, scale, mod: Optional[ScoreMod]):
     _need_cuda(q, "attention q")
     dev = q.device
-    if q.dim() != 4 or k.dim() != 4:
-        raise ValueError(f"mirage_amd: attention operands are [B, N, heads, head_dim], got {tuple(q.shape)} and {tuple(k.shape)}")
+    if q.dim() != 4 or not isinstance(k, torch.Tensor) or k.dim() != 4:
+        raise ValueError("mirage_amd: attention operands are [B, N, heads, head_dim] tensors")
     B, Nq, H, hd = q.shape
     Nk, Hk = k.shape[1], k.shape[2]
-    for t, what, n in ((q, "attention q", Nq), (k, "attention k", Nk), (v, "attention v", Nk)):
-        _heads(t, what, B, n, dev, (BF16,))
-    if hd not in (32, 64):
+    _, qs = _heads(q, "attention q", B, Nq, dev, BF16)
+    kshape, ks = _heads(k, "attention k", B, Nk, dev, BF16)
+    vshape, vs = _heads(v, "attention v", B, Nk, dev, BF16)
+    if hd != 64 and hd != 32:
         raise NotImplementedError(f"mirage_amd: attention head_dim {hd} not in (32, 64)")
-    if k.shape != v.shape or k.shape[3] != hd or Hk == 0 or H == 0 or H % Hk:
-        raise ValueError(f"mirage_amd: attention q {tuple(q.shape)}, k {tuple(k.shape)}, v {tuple(v.shape)}: k and v alike, query heads a multiple of key heads")
-    d = L.AttnModDesc()
-    d.q, d.k, d.v = q.data_ptr(), k.data_ptr(), v.data_ptr()
-    d.q_bs, d.q_rs, d.q_hs, _ = q.stride()
-    d.k_bs, d.k_rs, d.k_hs, _ = k.stride()
-    d.v_bs, d.v_rs, d.v_hs, _ = v.stride()
-    d.B, d.H, d.Hk, d.Nq, d.Nk, d.head_dim, d.scale = B, H, Hk, Nq, Nk, hd, float(scale)
+    if kshape != vshape or kshape[3] != hd or Hk == 0 or H == 0 or H % Hk:
+        raise ValueError(f"mirage_amd: attention q {tuple(q.shape)}, k {tuple(kshape)}, v {tuple(vshape)}: k and v alike, query heads a multiple of key heads")
+    d = L.AttnModDesc(q.data_ptr(), k.data_ptr(), v.data_ptr(), None, None, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], vs[0], vs[1], vs[2], 0, 0, 0,
+                      B, H, Hk, Nq, Nk, hd, scale)
     if mod is not None:
-        d.cap, d.causal = mod.cap, int(mod.causal)
+        d.cap, d.causal = mod.cap, mod.causal
         if mod.slopes is not None:
             axes = mod.pos_q.shape[-1] if mod.pos_q.dim() else 0
             if not 1 <= axes <= L.MRG_MAX_AXES:
                 raise ValueError(f"mirage_amd: ScoreMod positions have {axes} axes (1 to {L.MRG_MAX_AXES})")
-            _want(mod.slopes, "ScoreMod slopes", dev, (F32,), (H,))
-            _want(mod.pos_q, "ScoreMod pos_q", dev, (F32,), (B, Nq, axes))
-            _want(mod.pos_k, "ScoreMod pos_k", dev, (F32,), (B, Nk, axes))
+            _want(mod.slopes, "ScoreMod slopes", dev, _ONLY32, (H,))
+            _want(mod.pos_q, "ScoreMod pos_q", dev, _ONLY32, (B, Nq, axes))
+            _want(mod.pos_k, "ScoreMod pos_k", dev, _ONLY32, (B, Nk, axes))
             d.slopes, d.pos_q, d.pos_k, d.axes = mod.slopes.data_ptr(), mod.pos_q.data_ptr(), mod.pos_k.data_ptr(), axes
         if mod.doc_q is not None:
-            _want(mod.doc_q, "ScoreMod doc_q", dev, (torch.int32,), (B, Nq))
-            _want(mod.doc_k, "ScoreMod doc_k", dev, (torch.int32,), (B, Nk))
+            _want(mod.doc_q, "ScoreMod doc_q", dev, _I32, (B, Nq))
+            _want(mod.doc_k, "ScoreMod doc_k", dev, _I32, (B, Nk))
             d.doc_q, d.doc_k = mod.doc_q.data_ptr(), mod.doc_k.data_ptr()
         if mod.prefix is not None:
-            _want(mod.prefix, "ScoreMod prefix", dev, (torch.int32,), (B,))
+            _want(mod.prefix, "ScoreMod prefix", dev, _I32, (B,))
             d.prefix = mod.prefix.data_ptr()
     return d, dev
 
 
 def _attn_mod_ws(d, backward: int, dev):
+    """the call's workspace (None: it needs none); stream-ordered like every tensor, so it may go as soon as the launches are queued"""
     n = lib.mrg_attn_mod_ws_bytes(C.byref(d), backward)
     if n < 0:
         check(int(n), "mrg_attn_mod_ws_bytes")
-    ws = torch.empty(n, dtype=torch.uint8, device=dev) if n else None
-    d.ws = _p(ws)
+    if not n:
+        return None
+    ws = torch.empty(n, dtype=torch.uint8, device=dev)
+    d.ws = ws.data_ptr()
     return ws
 
 
@@ -974,44 +1006,45 @@ def attn_mod_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float
     o = 0 and lse = -inf."""
     d, dev = _attn_mod_desc(q, k, v, scale, mod)
     o = torch.empty(q.shape, dtype=BF16, device=dev)
-    lse = torch.empty((d.B, d.H, d.Nq), dtype=F32, device=dev) if need_lse else None
-    d.o, d.lse = o.data_ptr(), _p(lse)
+    d.o = o.data_ptr()
     d.o_bs, d.o_rs, d.o_hs, _ = o.stride()
-    with _On(dev) as st:
-        ws = _attn_mod_ws(d, 0, dev)      # noqa: F841  (stream-ordered: lives until this call's launches are queued)
-        check(lib.mrg_attn_mod_fwd(C.byref(d), st), "mrg_attn_mod_fwd")
+    lse = None
+    if need_lse:
+        lse = torch.empty((d.B, d.H, d.Nq), dtype=F32, device=dev)
+        d.lse = lse.data_ptr()
+    ws = _attn_mod_ws(d, 0, dev)      # noqa: F841
+    _launch(lib.mrg_attn_mod_fwd, d, dev, "mrg_attn_mod_fwd")
     return o, lse
 
 
 def attn_mod_bwd(q, k, v, o, lse, d_o, scale: float, mod: Optional[ScoreMod] = None, dq=None, dk=None, dv=None):
-    """Gradients of attn_mod_fwd: (dq, dk, dv) bf16, new contiguous tensors or the destinations given (views into a fused gradient buffer)."""
+    """Gradients of attn_mod_fwd: (dq, dk, dv) bf16, new contiguous tensors or the destinations given (views into a fused gradient buffer, apart from
+    every operand and from each other)."""
     d, dev = _attn_mod_desc(q, k, v, scale, mod)
-    _heads(o, "attention o", d.B, d.Nq, dev, (BF16,))
-    _heads(d_o, "attention d_o", d.B, d.Nq, dev, (BF16,))
-    if o.shape != q.shape or d_o.shape != q.shape:
+    oshape, os_ = _heads(o, "attention o", d.B, d.Nq, dev, BF16)
+    gshape, gs = _heads(d_o, "attention d_o", d.B, d.Nq, dev, BF16)
+    if oshape != q.shape or gshape != q.shape:
         raise ValueError("mirage_amd: attention o and d_o must have the shape of q")
-    _want(lse, "attention lse", dev, (F32,), (d.B, d.H, d.Nq))
     if lse is None:
         raise ValueError("mirage_amd: attn_mod_bwd needs the forward pass's lse")
-    outs = []
-    for g, src, what, n in ((dq, q, "attention dq", d.Nq), (dk, k, "attention dk", d.Nk), (dv, v, "attention dv", d.Nk)):
+    _want(lse, "attention lse", dev, _ONLY32, (d.B, d.H, d.Nq))
+    outs, strides = [], []
+    for g, src, what in ((dq, q, "attention dq"), (dk, k, "attention dk"), (dv, v, "attention dv")):
         if g is None:
             g = torch.empty(src.shape, dtype=BF16, device=dev)
+            strides += g.stride()[:3]
         else:
-            _heads(g, what, d.B, n, dev, (BF16,))
-            if g.shape != src.shape:
-                raise ValueError(f"mirage_amd: {what} must have shape {tuple(src.shape)}, got {tuple(g.shape)}")
+            strides += _out_heads(g, what, src.shape, dev, BF16)[:3]
+            for t in (q, k, v, o, d_o, *outs):
+                _need_apart(g, t, what)
         outs.append(g)
     d.o, d.lse, d.d_o = o.data_ptr(), lse.data_ptr(), d_o.data_ptr()
-    d.o_bs, d.o_rs, d.o_hs, _ = o.stride()
-    d.do_bs, d.do_rs, d.do_hs, _ = d_o.stride()
-    d.dq, d.dk, d.dv = (g.data_ptr() for g in outs)
-    d.dq_bs, d.dq_rs, d.dq_hs, _ = outs[0].stride()
-    d.dk_bs, d.dk_rs, d.dk_hs, _ = outs[1].stride()
-    d.dv_bs, d.dv_rs, d.dv_hs, _ = outs[2].stride()
-    with _On(dev) as st:
-        ws = _attn_mod_ws(d, 1, dev)      # noqa: F841
-        check(lib.mrg_attn_mod_bwd(C.byref(d), st), "mrg_attn_mod_bwd")
+    d.o_bs, d.o_rs, d.o_hs = os_[:3]
+    d.do_bs, d.do_rs, d.do_hs = gs[:3]
+    d.dq, d.dk, d.dv = outs[0].data_ptr(), outs[1].data_ptr(), outs[2].data_ptr()
+    d.dq_bs, d.dq_rs, d.dq_hs, d.dk_bs, d.dk_rs, d.dk_hs, d.dv_bs, d.dv_rs, d.dv_hs = strides
+    ws = _attn_mod_ws(d, 1, dev)      # noqa: F841
+    _launch(lib.mrg_attn_mod_bwd, d, dev, "mrg_attn_mod_bwd")
     return tuple(outs)
 
 
