@@ -1,0 +1,271 @@
+"""Transformer blocks for packed volumes: rows that hold the tokens of several samples (stacks of scans of any size, one after the other, padded at
+the end), with rotary positions over several axes (stack, height, width) instead of the fixed 2-D table, attention that stays inside a
+sample, and norms on both sides of every branch.
+
+    y = norm1(x)
+    x, y = x + gate1 * post1(attention(y)),  norm2(x)
+    x, y = x + gate2 * post2(mlp(y)),        norm1 of the next block (x)
+
+The counterpart of utils.Block / engine.EncoderFn for such rows; the reference has no packed form (its blocks: mirage/utils.py:162-262).  Like
+there, parameters are fp32 nn.Parameters, products run on the bf16 GEMM kernels, the residual stream is fp32, and the backward pass OVERWRITES
+the parameters' gradient buffers (arena.grad_buffer): nothing has to be zeroed, and a parameter takes part once per backward pass.
+"""
+from typing import Optional, Sequence
+
+import torch
+import torch.nn as nn
+
+from . import engine as E
+from . import kernels as K
+from .arena import grad_buffer
+from .utils import Linear, Mlp
+
+BF16, F32 = torch.bfloat16, torch.float32
+
+
+# ------------------------------------------------------------------------------------------------------------- positions
+def grid_positions(sizes: Sequence[int], lead: int = 0, device=None) -> torch.Tensor:
+    """int32 [lead + prod(sizes), len(sizes)]: raster order over `sizes` (stack, height, width; the last runs fastest), behind `lead` tokens at the
+    origin (global tokens: rotary positions leave a token at the origin as it is)."""
+    axes = torch.meshgrid(*[torch.arange(n) for n in sizes], indexing="ij")
+    at = torch.stack([a.reshape(-1) for a in axes], dim=1)
+    return torch.cat([torch.zeros(lead, len(sizes), dtype=at.dtype), at]).to(device=device, dtype=torch.int32)
+
+
+def rotary_frequencies(sections: Sequence[int], theta: float = 100.0, device=None) -> torch.Tensor:
+    """float64 [sum(sections)]: theta^(-i / n) for pair i of the n pairs of each axis (radians per position unit)."""
+    return torch.cat([theta ** (-torch.arange(n, dtype=torch.float64) / n) for n in sections]).to(device)
+
+
+# ------------------------------------------------------------------------------------------------- differentiable operators
+class _RotaryFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, pos, freqs, sections, pairing):
+        ctx.save_for_backward(pos, freqs)
+        ctx.how = (sections, pairing)
+        return K.rotary_axes(q, k, pos, freqs, sections, pairing=pairing)
+
+    @staticmethod
+    def backward(ctx, dq, dk):
+        pos, freqs = ctx.saved_tensors
+        dq, dk = K.rotary_axes(dq, dk, pos, freqs, ctx.how[0], pairing=ctx.how[1], inverse=True)
+        return dq, dk, None, None, None, None
+
+
+def rotary(q, k, pos, freqs, sections, pairing: str = "axial"):
+    """kernels.rotary_axes with its gradient (q and k of [B, N, heads, head_dim], bf16 or fp32)."""
+    return _RotaryFn.apply(q, k, pos, freqs, tuple(sections), pairing)
+
+
+class _AttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, q, k, v, scale, mod):
+        need = any(ctx.needs_input_grad)
+        o, lse = K.attn_mod_fwd(q, k, v, scale, mod, need_lse=need)
+        if need:
+            ctx.save_for_backward(q, k, v, o, lse)
+            ctx.how = (scale, mod)
+        return o
+
+    @staticmethod
+    def backward(ctx, d_o):
+        q, k, v, o, lse = ctx.saved_tensors
+        if d_o.stride(-1) != 1:
+            d_o = d_o.contiguous()
+        return (*K.attn_mod_bwd(q, k, v, o, lse, d_o, *ctx.how), None, None)
+
+
+def attention(q, k, v, scale: float, mod: Optional[K.ScoreMod] = None):
+    """kernels.attn_mod_fwd with its gradient: [B, Nq, H, hd] from bf16 q [B, Nq, H, hd] and k, v [B, Nk, Hk, hd]."""
+    return _AttentionFn.apply(q, k, v, scale, mod)
+
+
+class _SeamFn(torch.autograd.Function):
+    """kernels.resid_norm_fwd; the gradients of a per-sample gate are returned, those of the parameters written into their buffers."""
+
+    @staticmethod
+    def forward(ctx, x, branch, gates, seam, pre, *params):
+        how = dict(gate=gates if gates is not None else seam.gate, alpha=seam.alpha, post=_wb(seam.post), pre=_wb(pre), kind=seam.kind, eps=seam.eps)
+        x_new, y, stats = K.resid_norm_fwd(x, branch, **how)
+        ctx.seam, ctx.pre = seam, pre
+        ctx.save_for_backward(x_new, branch, gates, stats)
+        return x_new, y
+
+    @staticmethod
+    def backward(ctx, dx_new, dy):
+        x_new, branch, gates, stats = ctx.saved_tensors
+        seam, pre = ctx.seam, ctx.pre
+        named = [("post_weight", seam.post and seam.post.weight), ("post_bias", seam.post and seam.post.bias), ("pre_weight", pre and pre.weight),
+                 ("pre_bias", pre and pre.bias)] + ([("gate", seam.gate)] if gates is None else [])
+        into = {n: grad_buffer(p) for n, p in named if p is not None}
+        dx, dbranch, grads = K.resid_norm_bwd(dx_new.contiguous(), None if pre is None else dy.contiguous(), x_new, branch, stats,
+                                              gate=gates if gates is not None else seam.gate, alpha=seam.alpha, post=_wb(seam.post), pre=_wb(pre), kind=seam.kind,
+                                              eps=seam.eps, grads={n: g for n, g in into.items() if g is not None})
+        return (dx, dbranch, grads["gate"] if gates is not None else None) + (None,) * (len(ctx.needs_input_grad) - 3)
+
+
+def _wb(norm):
+    return None if norm is None else (norm.weight, norm.bias)
+
+
+# ------------------------------------------------------------------------------------------------------------- modules
+class Norm(nn.Module):
+    """weight and bias of a norm that a seam applies; kind "layer" (with bias) or "rms" (without)"""
+
+    def __init__(self, dim: int, kind: str = "layer"):
+        super().__init__()
+        if kind not in ("layer", "rms"):
+            raise ValueError(f"mirage_amd.packed.Norm: kind {kind!r} is neither 'layer' nor 'rms'")
+        self.weight = nn.Parameter(torch.ones(dim))
+        self.bias = nn.Parameter(torch.zeros(dim)) if kind == "layer" else None
+
+
+class Seam(nn.Module):
+    """x' = alpha x + gate * post(branch), y = pre(x') in one kernel (kernels.resid_norm_fwd).  gate: a learnt row of channels (its initial value, or
+    None for no gate); forward(gates=[samples, dim]) puts one row per sample in its place."""
+
+    def __init__(self, dim: int, kind: str = "layer", post: bool = True, gate: Optional[float] = 1.0, alpha: float = 1.0, eps: float = 1e-6):
+        super().__init__()
+        self.kind, self.alpha, self.eps = kind, float(alpha), float(eps)
+        self.post = Norm(dim, kind) if post else None
+        self.gate = nn.Parameter(torch.full((dim,), float(gate))) if gate is not None else None
+
+    def forward(self, x, branch, pre: Optional[Norm] = None, gates: Optional[torch.Tensor] = None):
+        """(x', y); y is None without `pre`"""
+        params = [p for m in (self, pre) if m is not None for p in m.parameters()]
+        return _SeamFn.apply(x, branch, gates, self, pre, *params)
+
+
+class _PackedAttentionFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y16, att, pos, mod, *params):
+        B, N, _ = y16.shape
+        qkv, _, _ = E.lin_fwd(y16, att.qkv)
+        heads = qkv.view(B, N, att.num_heads + 2 * att.num_kv_heads, att.head_dim)
+        q, k, v = att.split(heads)
+        freqs = None
+        if att.sections is not None:                              # q and k are turned where the projection left them
+            freqs = att.freqs(y16.device)
+            K.rotary_axes(q, k, pos, freqs, att.sections, pairing=att.pairing, out_q=q, out_k=k)
+        need = any(ctx.needs_input_grad)
+        o, lse = K.attn_mod_fwd(q, k, v, att.scale, mod, need_lse=need)
+        branch, _, _ = E.lin_fwd(o.view(B, N, -1), att.proj)
+        if need:
+            ctx.att, ctx.mod = att, mod
+            ctx.save_for_backward(y16, qkv, o, lse, pos, freqs)
+        return branch
+
+    @staticmethod
+    def backward(ctx, dbranch):
+        y16, qkv, o, lse, pos, freqs = ctx.saved_tensors
+        att = ctx.att
+        B, N, _ = y16.shape
+        d_o, _ = E.lin_bwd(dbranch.contiguous(), o.view(B, N, -1), att.proj)
+        q, k, v = att.split(qkv.view(B, N, -1, att.head_dim))
+        d_qkv = torch.empty_like(qkv)
+        dq, dk, dv = att.split(d_qkv.view(B, N, -1, att.head_dim))
+        K.attn_mod_bwd(q, k, v, o, lse, d_o.view(o.shape), att.scale, ctx.mod, dq=dq, dk=dk, dv=dv)
+        if att.sections is not None:
+            K.rotary_axes(dq, dk, pos, freqs, att.sections, pairing=att.pairing, inverse=True, out_q=dq, out_k=dk)
+        dy, _ = E.lin_bwd(d_qkv, y16, att.qkv)
+        E.join_side_stream()
+        return (dy,) + (None,) * (len(ctx.needs_input_grad) - 1)
+
+
+class PackedAttention(nn.Module):
+    """Self attention over packed rows: one projection to q (num_heads) and k, v (num_kv_heads each, shared by groups of query heads), rotary positions
+    (sections: pairs per axis; None: no rotation), attention under `mod` (kernels.ScoreMod), output projection.  bf16 in, bf16 out."""
+
+    def __init__(self, dim: int, num_heads: int, num_kv_heads: Optional[int] = None, sections: Optional[Sequence[int]] = None, theta: float = 100.0,
+                 pairing: str = "axial", qkv_bias: bool = True):
+        super().__init__()
+        self.num_heads, self.num_kv_heads = num_heads, num_kv_heads or num_heads
+        self.head_dim = dim // num_heads
+        if dim % num_heads or self.head_dim not in (32, 64) or num_heads % self.num_kv_heads:
+            raise NotImplementedError(f"mirage_amd.PackedAttention: {num_heads} heads ({self.num_kv_heads} for keys) of {dim} channels: head_dim must be 32 or 64, "
+                                      "and the key heads must divide the query heads")
+        self.scale = self.head_dim ** -0.5
+        self.sections, self.theta, self.pairing = (None if sections is None else tuple(sections)), float(theta), pairing
+        self.qkv = Linear(dim, (num_heads + 2 * self.num_kv_heads) * self.head_dim, bias=qkv_bias)
+        self.proj = Linear(dim, dim)
+        self._freqs = {}
+
+    def freqs(self, device) -> torch.Tensor:
+        """the rotary table on `device` (float64 whatever type the module's parameters are cast to)"""
+        if device not in self._freqs:
+            self._freqs[device] = rotary_frequencies(self.sections, self.theta, device)
+        return self._freqs[device]
+
+    def split(self, heads):
+        h, k = self.num_heads, self.num_kv_heads
+        return heads[:, :, :h], heads[:, :, h:h + k], heads[:, :, h + k:]
+
+    def forward(self, y16, pos: Optional[torch.Tensor] = None, mod: Optional[K.ScoreMod] = None):
+        if y16.dtype != BF16 or y16.dim() != 3 or not y16.is_contiguous():
+            raise ValueError(f"mirage_amd.PackedAttention: needs contiguous bf16 [B, N, dim] (a norm's output), got {y16.dtype} {tuple(y16.shape)}")
+        if (pos is None) != (self.sections is None):
+            raise ValueError("mirage_amd.PackedAttention: positions go with rotary sections")
+        return _PackedAttentionFn.apply(y16, self, pos, mod, *self.parameters())
+
+
+class _PackedMlpFn(torch.autograd.Function):
+    @staticmethod
+    def forward(ctx, y16, mlp, *params):
+        need = any(ctx.needs_input_grad)
+        act, _, pre = E.lin_fwd(y16, mlp.fc1, gelu=True, save_pre=need)
+        branch, _, _ = E.lin_fwd(act, mlp.fc2)
+        if need:
+            ctx.mlp = mlp
+            ctx.save_for_backward(y16, pre, act)
+        return branch
+
+    @staticmethod
+    def backward(ctx, dbranch):
+        y16, pre, act = ctx.saved_tensors
+        d_pre, _ = E.lin_bwd(dbranch.contiguous(), act, ctx.mlp.fc2, gelu_pre=pre)
+        dy, _ = E.lin_bwd(d_pre, y16, ctx.mlp.fc1)
+        E.join_side_stream()
+        return (dy,) + (None,) * (len(ctx.needs_input_grad) - 1)
+
+
+class PackedBlock(nn.Module):
+    """Parameters of one block (module docstring); PackedEncoder runs them, because a block's last seam already applies the next block's first norm."""
+
+    def __init__(self, dim: int, num_heads: int, mlp_ratio: float = 4.0, num_kv_heads: Optional[int] = None, sections: Optional[Sequence[int]] = None,
+                 theta: float = 100.0, pairing: str = "axial", norm: str = "layer", post_norm: bool = True, gate: Optional[float] = 1.0, alpha: float = 1.0,
+                 eps: float = 1e-6):
+        super().__init__()
+        self.norm1 = Norm(dim, norm)
+        self.attn = PackedAttention(dim, num_heads, num_kv_heads, sections, theta, pairing)
+        self.seam1 = Seam(dim, norm, post_norm, gate, alpha, eps)
+        self.norm2 = Norm(dim, norm)
+        self.mlp = Mlp(dim, int(dim * mlp_ratio))
+        self.seam2 = Seam(dim, norm, post_norm, gate, alpha, eps)
+
+    def forward(self, x, y16, following: Optional[Norm], pos=None, mod=None, gates=None):
+        """one block from (x, norm1(x)): (x, following(x) or None).  gates: (attention's, mlp's) rows per sample, [samples, dim] each"""
+        g1, g2 = gates if gates is not None else (None, None)
+        x, y16 = self.seam1(x, self.attn(y16, pos, mod), self.norm2, g1)
+        return self.seam2(x, _PackedMlpFn.apply(y16, self.mlp, *self.mlp.parameters()), following, g2)
+
+
+class PackedEncoder(nn.Module):
+    """A stack of PackedBlocks with a final norm: forward(x fp32 [B, N, dim], pos, mod, gates) -> (x, norm(x) in bf16).  `mod` carries the documents of the
+    packed rows (and whatever else its scores need); padding tokens keep their residual, and what they hold reaches no other token."""
+
+    def __init__(self, dim: int, depth: int, num_heads: int, **block):
+        super().__init__()
+        if depth < 1:
+            raise ValueError("mirage_amd.PackedEncoder: depth must be at least 1")
+        self.blocks = nn.ModuleList([PackedBlock(dim, num_heads, **block) for _ in range(depth)])
+        norm, eps = block.get("norm", "layer"), block.get("eps", 1e-6)
+        self.norm = Norm(dim, norm)
+        self._first = Seam(dim, norm, post=False, gate=None, alpha=0.0, eps=eps)          # no parameters: x' = 0 x + x, y = norm1(x)
+
+    def forward(self, x, pos: Optional[torch.Tensor] = None, mod: Optional[K.ScoreMod] = None, gates=None):
+        """gates: per block (attention's, mlp's) rows per sample, or None (the blocks' learnt channel gates)"""
+        x, y16 = self._first(x, x, self.blocks[0].norm1)
+        for i, blk in enumerate(self.blocks):
+            following = self.blocks[i + 1].norm1 if i + 1 < len(self.blocks) else self.norm
+            x, y16 = blk(x, y16, following, pos, mod, None if gates is None else gates[i])
+        return x, y16
