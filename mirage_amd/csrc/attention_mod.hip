@@ -216,12 +216,12 @@ __device__ __forceinline__ void place(int id, int heads, int per, bool by_length
 struct Walk { unsigned long long see, part, wsee, wwhole; };
 __device__ __forceinline__ int take_tile(unsigned long long& see) { const int i = __builtin_ctzll(see); see &= see - 1; return i; }
 
-// scores in registers -> log2 units (CAP, BIAS) or left raw; steep: 1 - tanh^2
+// scores in registers: CAP -> log2 units, otherwise q.k stays as it is (the exponential takes the factor) and the bias comes in q.k's units.
+// kslope: slope / scale, or with CAP slope log2(e).  steep: 1 - tanh^2
 template <bool CAP, bool BIAS, bool STEEP>
-__device__ __forceinline__ void modify(f32x16& s, f32x16& steep, const ModArgs& a, const float (&mine)[3], const float* pos, int row0, float slope2, int lane) {
-    const float c1 = a.scale * LOG2E_F;
+__device__ __forceinline__ void modify(f32x16& s, f32x16& steep, const ModArgs& a, const float (&mine)[3], const float* pos, int row0, float kslope, int lane) {
     if (CAP) {
-        const float up = 2.f * c1 / a.cap, capl = a.cap * LOG2E_F;
+        const float up = 2.f * a.scale * LOG2E_F / a.cap, capl = a.cap * LOG2E_F;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
             const float th = fmaf(-2.f, __builtin_amdgcn_rcpf(fast_exp2(s[r] * up) + 1.f), 1.f);       // tanh(x) = 1 - 2 / (e^2x + 1)
@@ -230,18 +230,19 @@ __device__ __forceinline__ void modify(f32x16& s, f32x16& steep, const ModArgs& 
         }
     }
     if (BIAS) {
-        f32x16 far = zero16();
+        f32x16 far;                                              // signed for one axis: |.| is free where it is used
 #pragma unroll
         for (int ax = 0; ax < 3; ++ax) if (ax < a.axes) {
 #pragma unroll
             for (int g = 0; g < 4; ++g) {
                 const float4 p = *reinterpret_cast<const float4*>(pos + ax * TT + row0 + 8 * g + 4 * (lane >> 5));
-                far[4 * g] += fabsf(p.x - mine[ax]); far[4 * g + 1] += fabsf(p.y - mine[ax]);
-                far[4 * g + 2] += fabsf(p.z - mine[ax]); far[4 * g + 3] += fabsf(p.w - mine[ax]);
+                const float d[4] = {p.x - mine[ax], p.y - mine[ax], p.z - mine[ax], p.w - mine[ax]};
+#pragma unroll
+                for (int e = 0; e < 4; ++e) far[4 * g + e] = ax == 0 ? d[e] : fabsf(far[4 * g + e]) + fabsf(d[e]);
             }
         }
 #pragma unroll
-        for (int r = 0; r < 16; ++r) s[r] = CAP ? fmaf(far[r], -slope2, s[r]) : fmaf(far[r], -slope2, s[r] * c1);
+        for (int r = 0; r < 16; ++r) s[r] = fmaf(fabsf(far[r]), -kslope, s[r]);
     }
 }
 
@@ -301,9 +302,9 @@ __global__ __launch_bounds__(64 * NW, 3) void attn_mod_fwd_kernel(const ModArgs 
 #pragma unroll
     for (int kk = 0; kk < KS; ++kk) qf[kk] = *reinterpret_cast<const bf16x8*>(qp + kk * 16 + 8 * (lane >> 5));
     float mine[3] = {0.f, 0.f, 0.f};
-    float slope2 = 0.f;
+    float kslope = 0.f;
     if (BIAS) {
-        slope2 = a.slopes[h] * LOG2E_F;
+        kslope = CAP ? a.slopes[h] * LOG2E_F : a.slopes[h] / a.scale;
         for (int ax = 0; ax < a.axes; ++ax) mine[ax] = a.pos_q[((long)b * a.Nq + qr) * a.axes + ax];
     }
     auto lim_of = [&](int i) { return max(pre, min(i + off + 1, a.Nk)); };               // keys below it are visible as far as order goes (may be <= 0)
@@ -336,7 +337,7 @@ __global__ __launch_bounds__(64 * NW, 3) void attn_mod_fwd_kernel(const ModArgs 
     for (int dj = 0; dj < DJ; ++dj) o[dj] = zero16();
     float m_run = -INFINITY, l_run = 0.f;
     bool poisoned = false;
-    constexpr bool RAW = !CAP && !BIAS;                          // scores stay q.k and the exponent takes the factor
+    constexpr bool RAW = !CAP;                                   // scores stay in q.k's units and the exponential takes the factor
     const float unit = RAW ? a.scale * LOG2E_F : 1.f;
 
     RowFrag<HD> fk; fk.init(lane);
@@ -407,7 +408,7 @@ __global__ __launch_bounds__(64 * NW, 3) void attn_mod_fwd_kernel(const ModArgs 
                 f32x16 s = zero16();
 #pragma unroll
                 for (int kk = 0; kk < KS; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fk.read(kt, kb * 32, kk), qf[kk], s, 0, 0, 0);
-                modify<CAP, BIAS, false>(s, s, a, mine, ldsP[buf], kb * 32, slope2, lane);
+                modify<CAP, BIAS, false>(s, s, a, mine, ldsP[buf], kb * 32, kslope, lane);
                 if (!whole) hide<true, false>(s, s, lim - j0 - kb * 32 - 4 * (lane >> 5), mydoc, docs ? &ldsD[buf][kb * 32 + 4 * (lane >> 5)] : nullptr, -INFINITY);
                 float mx = s[0];
 #pragma unroll
@@ -595,7 +596,7 @@ __global__ __launch_bounds__(256, BOCC) void attn_mod_bwd_kernel(const ModArgs a
 #pragma unroll
     for (int dj = 0; dj < DJ; ++dj) { ga[dj] = zero16(); if (!OWN_Q) gb[dj] = zero16(); }
     bool poisoned = false;
-    constexpr bool RAW = !CAP && !BIAS;
+    constexpr bool RAW = !CAP;
     const float unit = RAW ? a.scale * LOG2E_F : 1.f;
 
     RowFrag<HD> fr; fr.init(lane);
@@ -667,7 +668,7 @@ __global__ __launch_bounds__(256, BOCC) void attn_mod_bwd_kernel(const ModArgs a
         const int j0 = (split + (base + i) * a.splits) * TT;
         const bool see = (wk.wsee >> i) & 1, whole = (wk.wwhole >> i) & 1;
         if (see) {
-            const float slope2 = BIAS ? a.slopes[h] * LOG2E_F : 0.f;
+            const float kslope = !BIAS ? 0.f : (CAP ? a.slopes[h] * LOG2E_F : a.slopes[h] / a.scale);
             const uint32_t xb = lds_addr(ldsX[buf]), yb = lds_addr(ldsY[buf]);
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
@@ -687,7 +688,7 @@ __global__ __launch_bounds__(256, BOCC) void attn_mod_bwd_kernel(const ModArgs a
                 for (int kk = 0; kk < KS; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.read(xb, kb * 32, kk), fa[kk], s, 0, 0, 0);
 #pragma unroll
                 for (int kk = 0; kk < KS; ++kk) dp = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fr.read(yb, kb * 32, kk), fb[kk], dp, 0, 0, 0);
-                modify<CAP, BIAS, true>(s, steep, a, mine, ldsP[buf], kb * 32, slope2, lane);
+                modify<CAP, BIAS, true>(s, steep, a, mine, ldsP[buf], kb * 32, kslope, lane);
 #pragma unroll
                 for (int q = 0; q < 4; ++q) {
                     float4 L = make_float4(-lse2, -lse2, -lse2, -lse2);
