@@ -30,6 +30,12 @@ namespace {
 constexpr float LOG2E_F = 1.4426950408889634f, LN2_F = 0.6931471805599453f;
 constexpr int TT = 64;                        // tokens of a staged tile
 constexpr int MAX_SPLITS = 64;
+#ifndef FOCC
+#define FOCC 3
+#endif
+#ifndef TABMIN
+#define TABMIN 4
+#endif
 #ifndef NWF
 #define NWF 4
 #endif
@@ -51,7 +57,7 @@ struct ModArgs {
     float scale, cap;
     const float* slopes; const float* pos_q; const float* pos_k; int axes;
     const int* doc_q; const int* doc_k;
-    const int4* tab_q; const int4* tab_k; int ntq, ntk;     // per tile {lowest, highest document, valid tokens}
+    const int4* tab_q; const int4* tab_k; int ntq, ntk;     // per tile {lowest, highest document, valid tokens}; null: every tile is looked at
     int causal; const int* prefix;
     const bf16_t* d_o; long do_bs, do_rs, do_hs;
     bf16_t* dq; bf16_t* dk; bf16_t* dv;
@@ -274,7 +280,7 @@ __device__ __forceinline__ void hide(f32x16& x, f32x16& y, int left, int mydoc, 
 // NW waves of 32 queries.  NW = 1 serves up to 32 queries (a pooled or a single new token): every workgroup is one wave, and the keys are
 // split over many of them.
 template <int HD, int NW, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * NW, 3) void attn_mod_fwd_kernel(const ModArgs a) {
+__global__ __launch_bounds__(64 * NW, FOCC) void attn_mod_fwd_kernel(const ModArgs a) {
     constexpr int KS = HD / 16, DJ = HD / 32, NT = 64 * NW, TB = TT * HD * 2;
     __shared__ __attribute__((aligned(16))) char ldsK[2][TB];
     __shared__ __attribute__((aligned(16))) char ldsV[2][TB];
@@ -290,7 +296,7 @@ __global__ __launch_bounds__(64 * NW, 3) void attn_mod_fwd_kernel(const ModArgs 
     const bf16_t* kp = a.k + (long)b * a.k_bs + (long)hk * a.k_hs;
     const bf16_t* vp = a.v + (long)b * a.v_bs + (long)hk * a.v_hs;
     const int* docs = a.doc_k ? a.doc_k + (long)b * a.Nk : nullptr;
-    const int4* tab = a.doc_k ? a.tab_k + (long)b * a.ntk : nullptr;
+    const int4* tab = a.tab_k ? a.tab_k + (long)b * a.ntk : nullptr;
     const float* posk = BIAS ? a.pos_k + (long)b * a.Nk * a.axes : nullptr;
     const int off = a.Nk - a.Nq;
     const int pre = a.causal ? (a.prefix ? min(max(a.prefix[b], 0), a.Nk) : 0) : a.Nk;
@@ -313,7 +319,7 @@ __global__ __launch_bounds__(64 * NW, 3) void attn_mod_fwd_kernel(const ModArgs 
     const int wlim_lo = lim_of(min(q0, a.Nq - 1)), wlim_hi = lim_of(min(q0 + 31, a.Nq - 1));      // (documents are tested apart)
     int wlo = 0, whi = 0;
     bool pure = true;
-    if (docs) {
+    if (tab) {
         wlo = __builtin_amdgcn_readfirstlane(wave_min_i(mydoc < 0 ? 0x7fffffff : mydoc));
         whi = __builtin_amdgcn_readfirstlane(wave_max_i(mydoc));
         pure = wlo == whi && __builtin_amdgcn_ballot_w64(mydoc < 0) == 0;
@@ -323,7 +329,7 @@ __global__ __launch_bounds__(64 * NW, 3) void attn_mod_fwd_kernel(const ModArgs 
     const int glim_lo = lim_of(g0), glim_hi = lim_of(g1);
     int glo = 0, ghi = 0;
     bool gpure = true;
-    if (docs) {
+    if (tab) {
         glo = 0x7fffffff; ghi = -1;
         for (int t = g0 / TT; t <= g1 / TT; ++t) {
             const int4 e = a.tab_q[(long)b * a.ntq + t];
@@ -376,7 +382,8 @@ __global__ __launch_bounds__(64 * NW, 3) void attn_mod_fwd_kernel(const ModArgs 
         const int i = base + lane, t = split + i * a.splits;
         bool see = i < nmine && t * TT < glim_hi, whole = t * TT + TT <= glim_lo;
         bool ws = see && active && t * TT < wlim_hi, ww = t * TT + TT <= wlim_lo;
-        if (docs && see) {
+        if (docs && !tab) whole = ww = false;
+        if (tab && see) {
             const int4 e = tab[t];
             see = e.x <= ghi && e.y >= glo;
             whole = whole && gpure && e.x == e.y && e.x == glo && e.z == TT;
@@ -482,25 +489,33 @@ __global__ __launch_bounds__(64 * NW, 3) void attn_mod_fwd_kernel(const ModArgs 
     if (a.lse && lane < 32) a.lse[((long)b * a.H + h) * a.Nq + row] = l_run == 0.f ? -INFINITY : (m_run * unit + __log2f(l_run)) * LN2_F;
 }
 
-// joins the splits of a row: weights 2^(m_s - max m), one thread per 4 elements
-__global__ __launch_bounds__(256) void attn_mod_join_kernel(const ModArgs a, int HD) {
-    const long i = (long)blockIdx.x * 256 + threadIdx.x;
-    const int cpr = HD / 4;
-    const long rows = (long)a.B * a.H * a.Nq, r = i / cpr;
+// joins the splits of a row: weights 2^(m_s - max m).  A wave per row: 4 elements a lane, the splits dealt over the 256 / HD groups of lanes (one
+// thread per 4 elements walked its splits one load after the other: 10 us for 192 rows of 11)
+template <int HD>
+__global__ __launch_bounds__(256) void attn_mod_join_kernel(const ModArgs a) {
+    constexpr int CPR = HD / 4, NG = 64 / CPR;
+    const long rows = (long)a.B * a.H * a.Nq, r = (long)blockIdx.x * 4 + (threadIdx.x >> 6);
     if (r >= rows) return;
-    const int c = (int)(i - r * cpr) * 4;
-    float m = -INFINITY;
-    for (int s = 0; s < a.splits; ++s) m = fmaxf(m, a.part_ml[(s * rows + r) * 2]);
+    const int lane = threadIdx.x & 63, c = (lane % CPR) * 4, g = lane / CPR;
+    float m = lane < a.splits ? a.part_ml[(lane * rows + r) * 2] : -INFINITY;      // at most 64 splits
+    m = wave_max(m);
     float l = 0.f;
     float4 acc = make_float4(0.f, 0.f, 0.f, 0.f);
-    for (int s = 0; s < a.splits; ++s) {
+#pragma unroll 4
+    for (int s = g; s < a.splits; s += NG) {
         const float2 ml = *reinterpret_cast<const float2*>(a.part_ml + (s * rows + r) * 2);
-        if (ml.x == -INFINITY && ml.y == 0.f) continue;
-        const float f = ml.x == -INFINITY ? 1.f : fast_exp2(ml.x - m);
         const float4 v = *reinterpret_cast<const float4*>(a.part + (s * rows + r) * HD + c);
+        // a split that saw nothing has m = -inf, l = 0 and o = 0; a row that is NaN without a maximum stays NaN
+        const float f = ml.x == -INFINITY ? (ml.y == 0.f ? 0.f : 1.f) : fast_exp2(ml.x - m);
         l = fmaf(ml.y, f, l);
         acc.x = fmaf(v.x, f, acc.x); acc.y = fmaf(v.y, f, acc.y); acc.z = fmaf(v.z, f, acc.z); acc.w = fmaf(v.w, f, acc.w);
     }
+#pragma unroll
+    for (int o = CPR; o < 64; o <<= 1) {
+        l += __shfl_xor(l, o, 64);
+        acc.x += __shfl_xor(acc.x, o, 64); acc.y += __shfl_xor(acc.y, o, 64); acc.z += __shfl_xor(acc.z, o, 64); acc.w += __shfl_xor(acc.w, o, 64);
+    }
+    if (g != 0) return;
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const long bh = r / a.Nq;
     const int row = (int)(r - bh * a.Nq), b = (int)(bh / a.H), h = (int)(bh - (long)b * a.H);
@@ -536,8 +551,8 @@ __global__ __launch_bounds__(256, BOCC) void attn_mod_bwd_kernel(const ModArgs a
     const int* doc_o = bydoc ? (OWN_Q ? a.doc_q : a.doc_k) + (long)b * NO : nullptr;
     const int* doc_s = bydoc ? (OWN_Q ? a.doc_k : a.doc_q) + (long)b * NS : nullptr;
     const int nts = OWN_Q ? a.ntk : a.ntq, nto = OWN_Q ? a.ntq : a.ntk;
-    const int4* tab_s = bydoc ? (OWN_Q ? a.tab_k : a.tab_q) + (long)b * nts : nullptr;
-    const int4* tab_o = bydoc ? (OWN_Q ? a.tab_q : a.tab_k) + (long)b * nto : nullptr;
+    const int4* tab_s = a.tab_k ? (OWN_Q ? a.tab_k : a.tab_q) + (long)b * nts : nullptr;
+    const int4* tab_o = a.tab_k ? (OWN_Q ? a.tab_q : a.tab_k) + (long)b * nto : nullptr;
     const float* pos_s = BIAS ? (OWN_Q ? a.pos_k : a.pos_q) + (long)b * NS * a.axes : nullptr;
     const int r0 = blk * 128 + wave * 32, ro = min(r0 + (lane & 31), NO - 1), row = r0 + (lane & 31);
     const bool active = r0 < NO;
@@ -578,7 +593,7 @@ __global__ __launch_bounds__(256, BOCC) void attn_mod_bwd_kernel(const ModArgs a
     const int wedge0 = edge_of(min(r0, NO - 1)), wedge1 = edge_of(w1), gedge0 = edge_of(g0), gedge1 = edge_of(g1);
     int wlo = 0, whi = 0, glo = 0, ghi = 0;
     bool pure = true, gpure = true;
-    if (bydoc) {
+    if (tab_s) {
         wlo = __builtin_amdgcn_readfirstlane(wave_min_i(mydoc < 0 ? 0x7fffffff : mydoc));
         whi = __builtin_amdgcn_readfirstlane(wave_max_i(mydoc));
         pure = wlo == whi && __builtin_amdgcn_ballot_w64(mydoc < 0) == 0;
@@ -644,7 +659,8 @@ __global__ __launch_bounds__(256, BOCC) void attn_mod_bwd_kernel(const ModArgs a
         const int i = base + lane, t = split + i * a.splits;
         bool see = i < nmine && order_see(t, gedge0, gedge1), whole = order_whole(t, gedge0, gedge1) && t * TT + TT <= NS;
         bool ws = see && active && order_see(t, wedge0, wedge1), ww = order_whole(t, wedge0, wedge1) && (!OWN_Q || t * TT + TT <= NS);
-        if (bydoc && see) {
+        if (bydoc && !tab_s) whole = ww = false;
+        if (tab_s && see) {
             const int4 e = tab_s[t];
             see = e.x <= ghi && e.y >= glo;
             whole = whole && gpure && e.x == e.y && e.x == glo && e.z == TT;
@@ -787,6 +803,7 @@ __global__ __launch_bounds__(256) void attn_mod_sum_kernel(const float* __restri
 // ================================================ host ==================================================
 struct Plan {
     int ntq, ntk, nw, nblk, splits, dq_splits, dkv_splits;
+    bool tables;
     long tab_q, tab_k, dsum, part, part_ml, bytes;             // byte offsets into the workspace
 };
 
@@ -803,16 +820,17 @@ Plan plan_for(const mrg_attn_mod_desc* d, bool backward) {
     p.ntq = (d->Nq + TT - 1) / TT; p.ntk = (d->Nk + TT - 1) / TT;
     long at = 0;
     auto take = [&](long bytes) { const long o = at; at += (bytes + 255) / 256 * 256; return o; };
-    if (d->doc_k) { p.tab_q = take(16l * d->B * p.ntq); p.tab_k = take(16l * d->B * p.ntk); }
     const long rows_q = (long)d->B * d->H * d->Nq, rows_k = (long)d->B * d->Hk * d->Nk;
     if (!backward) {
         // up to 32 queries: workgroups of one wave, four resident per CU, and the keys cut until every CU has its four
         p.nw = d->Nq <= 32 ? 1 : NWF;
         p.nblk = (d->Nq + 32 * p.nw - 1) / (32 * p.nw);
         p.splits = splits_for((long)d->B * d->H * p.nblk, p.nw == 1 ? WANT1 : WANTF, p.ntk, 4);
+        p.tables = d->doc_k && (p.nw == 1 ? p.ntk > 2 : p.ntk > TABMIN);
         if (p.splits > 1) { p.part = take(4l * p.splits * rows_q * d->head_dim); p.part_ml = take(8l * p.splits * rows_q); }
     } else {
         p.dsum = take(4l * rows_q);
+        p.tables = d->doc_k && (p.ntk > TABMIN || p.ntq > TABMIN);
         p.dq_splits = splits_for((long)d->B * d->H * ((d->Nq + 127) / 128), WANTQ, p.ntk, 4);
         p.dkv_splits = splits_for((long)d->B * d->Hk * ((d->Nk + 127) / 128), d->causal ? WANTKC : WANTK, p.ntq, 4);
         long part = 0;
@@ -820,6 +838,7 @@ Plan plan_for(const mrg_attn_mod_desc* d, bool backward) {
         if (p.dkv_splits > 1 && 8l * p.dkv_splits * rows_k * d->head_dim > part) part = 8l * p.dkv_splits * rows_k * d->head_dim;
         p.part = take(part);                                    // used by dq first, by dk / dv behind it
     }
+    if (p.tables) { p.tab_q = take(16l * d->B * p.ntq); p.tab_k = take(16l * d->B * p.ntk); }
     p.bytes = at;
     return p;
 }
@@ -854,7 +873,8 @@ ModArgs mod_args(const mrg_attn_mod_desc* d, const Plan& p) {
     a.slopes = d->slopes; a.pos_q = d->pos_q; a.pos_k = d->pos_k; a.axes = d->slopes ? d->axes : 0;
     a.doc_q = d->doc_q; a.doc_k = d->doc_k;
     char* ws = (char*)d->ws;
-    a.tab_q = (const int4*)(ws + p.tab_q); a.tab_k = (const int4*)(ws + p.tab_k); a.ntq = p.ntq; a.ntk = p.ntk;
+    if (p.tables) { a.tab_q = (const int4*)(ws + p.tab_q); a.tab_k = (const int4*)(ws + p.tab_k); }
+    a.ntq = p.ntq; a.ntk = p.ntk;
     a.causal = d->causal != 0; a.prefix = d->prefix;
     a.d_o = (const bf16_t*)d->d_o; a.do_bs = d->do_bs; a.do_rs = d->do_rs; a.do_hs = d->do_hs;
     a.dq = (bf16_t*)d->dq; a.dk = (bf16_t*)d->dk; a.dv = (bf16_t*)d->dv;
@@ -865,7 +885,7 @@ ModArgs mod_args(const mrg_attn_mod_desc* d, const Plan& p) {
 }
 
 void doc_tables(const mrg_attn_mod_desc* d, const Plan& p, ModArgs& a, hipStream_t st) {
-    if (!d->doc_k) return;
+    if (!p.tables) return;
     const bool same = d->doc_q == d->doc_k && d->Nq == d->Nk;
     if (same) a.tab_q = a.tab_k;
     const int ntq = same || !d->doc_q ? 0 : p.ntq, tiles = d->B * (ntq + p.ntk);
@@ -931,8 +951,9 @@ extern "C" int mrg_attn_mod_fwd(const mrg_attn_mod_desc* d, hipStream_t stream) 
     if (d->head_dim == 64) { if (p.nw == 1) fwd_go<64, 1>(a, grid, stream); else fwd_go<64, NWF>(a, grid, stream); }
     else { if (p.nw == 1) fwd_go<32, 1>(a, grid, stream); else fwd_go<32, NWF>(a, grid, stream); }
     if (a.splits > 1) {
-        const long threads = (long)a.B * a.H * a.Nq * d->head_dim / 4;
-        hipLaunchKernelGGL(attn_mod_join_kernel, dim3((unsigned)((threads + 255) / 256)), dim3(256), 0, stream, a, d->head_dim);
+        const dim3 rows((unsigned)(((long)a.B * a.H * a.Nq + 3) / 4));
+        if (d->head_dim == 64) hipLaunchKernelGGL(attn_mod_join_kernel<64>, rows, dim3(256), 0, stream, a);
+        else hipLaunchKernelGGL(attn_mod_join_kernel<32>, rows, dim3(256), 0, stream, a);
     }
     return mrg_check_launch("mrg_attn_mod_fwd");
 }

@@ -121,7 +121,7 @@ def test_attention_workspace_grows_with_what_it_holds():
     ws = lambda b, **kw: L.lib.mrg_attn_mod_ws_bytes(C.byref(attn_desc(**kw)), b)
     assert ws(0) == 0                                            # no documents, nothing split
     assert ws(1) >= 4 * 4 * 5                                    # sum(do o)
-    assert ws(0, doc_q=4096, doc_k=4096) >= 2 * 16
+    assert ws(0, Nq=2000, Nk=2000, doc_q=4096, doc_k=4096) >= 2 * 16 * 32 and ws(0, doc_q=4096, doc_k=4096) == 0    # tables of the documents, for long rows
     assert ws(0, Nq=1, Nk=100_000) >= 2 * 4 * 64 * 4             # a single query is cut over many workgroups
     assert ws(1, Nq=1 << 20, Nk=1 << 20) >= 4 * 4 * (1 << 20)    # sizes in 64 bits
 
