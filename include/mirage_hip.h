@@ -238,8 +238,9 @@ int mrg_resid_norm_bwd(const mrg_resid_norm_desc* d, hipStream_t stream);
  * A row that sees nothing gives o = 0, lse = -inf and no gradient.  bf16, head_dim 32 or 64; H query heads share Hk key / value heads (H a
  * multiple of Hk: head h reads h / (H / Hk)).  *_bs / *_rs / *_hs: batch, row and head strides in elements.  Rows whose document is negative
  * are never read as keys; values behind a mask do not reach the result even when they are not finite.
- *   fwd: o, lse fp32 [B, H, Nq] (may be NULL);  ws: mrg_attn_mod_ws_bytes(d, 0) bytes.
- *   bwd: reads o, lse, d_o;  writes dq, dk, dv;  ws: mrg_attn_mod_ws_bytes(d, 1) bytes. */
+ *   fwd: o, lse fp32 [B, H, Nq] (may be NULL), o_rest (may be NULL): what the rounding of o to bf16 left out, bf16 with o's strides;
+ *        ws: mrg_attn_mod_ws_bytes(d, 0) bytes.
+ *   bwd: reads o, lse, d_o and, where given, o_rest (sum(do o) then takes o to 2^-16);  writes dq, dk, dv;  ws: mrg_attn_mod_ws_bytes(d, 1) bytes. */
 typedef struct mrg_attn_mod_desc {
     const void* q; const void* k; const void* v; void* o; float* lse;
     long q_bs, q_rs, q_hs, k_bs, k_rs, k_hs, v_bs, v_rs, v_hs, o_bs, o_rs, o_hs;
@@ -250,7 +251,7 @@ typedef struct mrg_attn_mod_desc {
     const void* d_o; long do_bs, do_rs, do_hs;
     void* dq; void* dk; void* dv;
     long dq_bs, dq_rs, dq_hs, dk_bs, dk_rs, dk_hs, dv_bs, dv_rs, dv_hs;
-    void* ws;
+    void* ws; void* o_rest;
 } mrg_attn_mod_desc;
 long mrg_attn_mod_ws_bytes(const mrg_attn_mod_desc* d, int backward);
 int mrg_attn_mod_fwd(const mrg_attn_mod_desc* d, hipStream_t stream);

@@ -113,7 +113,7 @@ class AttnModDesc(C.Structure):
                 ("slopes", vp), ("pos_q", vp), ("pos_k", vp), ("axes", ci), ("doc_q", vp), ("doc_k", vp), ("causal", ci), ("prefix", vp),
                 ("d_o", vp), ("do_bs", cl), ("do_rs", cl), ("do_hs", cl), ("dq", vp), ("dk", vp), ("dv", vp),
                 ("dq_bs", cl), ("dq_rs", cl), ("dq_hs", cl), ("dk_bs", cl), ("dk_rs", cl), ("dk_hs", cl), ("dv_bs", cl), ("dv_rs", cl), ("dv_hs", cl),
-                ("ws", vp)]
+                ("ws", vp), ("o_rest", vp)]
 
 
 class AdamWDesc(C.Structure):

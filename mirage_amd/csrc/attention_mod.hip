@@ -15,8 +15,8 @@
 // workgroup tests 64 tiles at a time (one per lane, one ballot) and walks only tiles that some row of it may see.  Per wave a tile is skipped,
 // whole (no test per score) or partial.  Sums, maxima, lse and all products accumulate in fp32.  p is rounded to bf16 as an operand of the
 // second product (at most 2^-8 of each weight, averaging over the row; its sum is taken before the rounding).  ds goes into its product as
-// two bf16 parts: rounded once, dq and dk were 0.0028 from the 64-bit gradient instead of 0.0022 (0.0017 is the rounding of the result
-// itself), because the rounding of ds adds to what the stored o carries into sum(do o).
+// two bf16 parts, and sum(do o) takes o with what its rounding left out: with either rounded once, dq and dk were 0.0028 from the 64-bit
+// gradient, where 0.0017 is the rounding of the result itself.
 //
 // Values that are not finite behind a mask: 0 * inf would reach the products, so in partial tiles the rows of the second product's left
 // operand that hold such values are replaced by zeros in LDS and noted; a row that SEES one of them is NaN in full.
@@ -51,7 +51,7 @@ constexpr int MAX_SPLITS = 64;
 #endif
 
 struct ModArgs {
-    const bf16_t* q; const bf16_t* k; const bf16_t* v; bf16_t* o; float* lse;
+    const bf16_t* q; const bf16_t* k; const bf16_t* v; bf16_t* o; bf16_t* o_rest; float* lse;
     long q_bs, q_rs, q_hs, k_bs, k_rs, k_hs, v_bs, v_rs, v_hs, o_bs, o_rs, o_hs;
     int B, H, Hk, G, Nq, Nk;                  // G = H / Hk
     float scale, cap;
@@ -276,6 +276,15 @@ __device__ __forceinline__ void hide(f32x16& x, f32x16& y, int left, int mydoc, 
     }
 }
 
+// four elements of o, and for the backward pass what their rounding left out
+__device__ __forceinline__ void store_o(const ModArgs& a, long at, const float4 v) {
+    const uint2 w = make_uint2(pack_bf2(v.x, v.y), pack_bf2(v.z, v.w));
+    *reinterpret_cast<uint2*>(a.o + at) = w;
+    if (a.o_rest)
+        *reinterpret_cast<uint2*>(a.o_rest + at) = make_uint2(pack_bf2(v.x - __uint_as_float(w.x << 16), v.y - __uint_as_float(w.x & 0xffff0000u)),
+                                                             pack_bf2(v.z - __uint_as_float(w.y << 16), v.w - __uint_as_float(w.y & 0xffff0000u)));
+}
+
 // ================================================ forward ===============================================
 // NW waves of 32 queries.  NW = 1 serves up to 32 queries (a pooled or a single new token): every workgroup is one wave, and the keys are
 // split over many of them.
@@ -479,13 +488,12 @@ __global__ __launch_bounds__(64 * NW, FOCC) void attn_mod_fwd_kernel(const ModAr
         return;
     }
     const float inv = l_run == 0.f ? 0.f : 1.f / l_run;
-    bf16_t* op = a.o + (long)b * a.o_bs + (long)row * a.o_rs + (long)h * a.o_hs;
+    const long at = (long)b * a.o_bs + (long)row * a.o_rs + (long)h * a.o_hs;
 #pragma unroll
     for (int dj = 0; dj < DJ; ++dj)
 #pragma unroll
         for (int g = 0; g < 4; ++g)
-            *reinterpret_cast<uint2*>(op + dj * 32 + 8 * g + 4 * (lane >> 5)) =
-                make_uint2(pack_bf2(o[dj][4 * g] * inv, o[dj][4 * g + 1] * inv), pack_bf2(o[dj][4 * g + 2] * inv, o[dj][4 * g + 3] * inv));
+            store_o(a, at + dj * 32 + 8 * g + 4 * (lane >> 5), make_float4(o[dj][4 * g] * inv, o[dj][4 * g + 1] * inv, o[dj][4 * g + 2] * inv, o[dj][4 * g + 3] * inv));
     if (a.lse && lane < 32) a.lse[((long)b * a.H + h) * a.Nq + row] = l_run == 0.f ? -INFINITY : (m_run * unit + __log2f(l_run)) * LN2_F;
 }
 
@@ -519,7 +527,7 @@ __global__ __launch_bounds__(256) void attn_mod_join_kernel(const ModArgs a) {
     const float inv = l == 0.f ? 0.f : 1.f / l;
     const long bh = r / a.Nq;
     const int row = (int)(r - bh * a.Nq), b = (int)(bh / a.H), h = (int)(bh - (long)b * a.H);
-    *reinterpret_cast<uint2*>(a.o + (long)b * a.o_bs + (long)row * a.o_rs + (long)h * a.o_hs + c) = make_uint2(pack_bf2(acc.x * inv, acc.y * inv), pack_bf2(acc.z * inv, acc.w * inv));
+    store_o(a, (long)b * a.o_bs + (long)row * a.o_rs + (long)h * a.o_hs + c, make_float4(acc.x * inv, acc.y * inv, acc.z * inv, acc.w * inv));
     if (a.lse && c == 0) a.lse[r] = l == 0.f ? -INFINITY : (m + __log2f(l)) * LN2_F;
 }
 
@@ -568,12 +576,14 @@ __global__ __launch_bounds__(256, BOCC) void attn_mod_bwd_kernel(const ModArgs a
             fb[kk] = *reinterpret_cast<const bf16x8*>(pb + kk * 16 + 8 * (lane >> 5));
         }
         if (OWN_Q) {
-            const bf16_t* po = a.o + (long)b * a.o_bs + (long)ro * a.o_rs + (long)ho * a.o_hs;
+            const long at_o = (long)b * a.o_bs + (long)ro * a.o_rs + (long)ho * a.o_hs;
 #pragma unroll
             for (int kk = 0; kk < KS; ++kk) {
-                const bf16x8 fo = *reinterpret_cast<const bf16x8*>(po + kk * 16 + 8 * (lane >> 5));
+                const bf16x8 fo = *reinterpret_cast<const bf16x8*>(a.o + at_o + kk * 16 + 8 * (lane >> 5));
+                bf16x8 rest = {0, 0, 0, 0, 0, 0, 0, 0};
+                if (a.o_rest) rest = *reinterpret_cast<const bf16x8*>(a.o_rest + at_o + kk * 16 + 8 * (lane >> 5));
 #pragma unroll
-                for (int e = 0; e < 8; ++e) D = fmaf(bf2f((bf16_t)fo[e]), bf2f((bf16_t)fb[kk][e]), D);
+                for (int e = 0; e < 8; ++e) D = fmaf(bf2f((bf16_t)fo[e]) + bf2f((bf16_t)rest[e]), bf2f((bf16_t)fb[kk][e]), D);
             }
             const float2 dh = halves(D);
             D = dh.x + dh.y;
@@ -866,7 +876,7 @@ bool aligned8(const void* p, long a, long b, long c) { return (uintptr_t)p % 16 
 
 ModArgs mod_args(const mrg_attn_mod_desc* d, const Plan& p) {
     ModArgs a = {};
-    a.q = (const bf16_t*)d->q; a.k = (const bf16_t*)d->k; a.v = (const bf16_t*)d->v; a.o = (bf16_t*)d->o; a.lse = d->lse;
+    a.q = (const bf16_t*)d->q; a.k = (const bf16_t*)d->k; a.v = (const bf16_t*)d->v; a.o = (bf16_t*)d->o; a.o_rest = (bf16_t*)d->o_rest; a.lse = d->lse;
     a.q_bs = d->q_bs; a.q_rs = d->q_rs; a.q_hs = d->q_hs; a.k_bs = d->k_bs; a.k_rs = d->k_rs; a.k_hs = d->k_hs;
     a.v_bs = d->v_bs; a.v_rs = d->v_rs; a.v_hs = d->v_hs; a.o_bs = d->o_bs; a.o_rs = d->o_rs; a.o_hs = d->o_hs;
     a.B = d->B; a.H = d->H; a.Hk = d->Hk; a.G = d->H / d->Hk; a.Nq = d->Nq; a.Nk = d->Nk; a.scale = d->scale; a.cap = d->cap;
@@ -943,7 +953,7 @@ extern "C" int mrg_attn_mod_fwd(const mrg_attn_mod_desc* d, hipStream_t stream) 
     const Plan p = plan_for(d, false);
     MRG_REQUIRE(d->q && d->o && (d->Nk == 0 || (d->k && d->v)) && (p.bytes == 0 || d->ws), MRG_ERR_ARG, "mrg_attn_mod_fwd: null pointer");
     MRG_REQUIRE(aligned8(d->q, d->q_bs, d->q_rs, d->q_hs) && aligned8(d->k, d->k_bs, d->k_rs, d->k_hs) && aligned8(d->v, d->v_bs, d->v_rs, d->v_hs)
-                && aligned8(d->o, d->o_bs, d->o_rs, d->o_hs), MRG_ERR_ARG, "mrg_attn_mod_fwd: operands and their strides must be multiples of 16 bytes");
+                && aligned8(d->o, d->o_bs, d->o_rs, d->o_hs) && (uintptr_t)d->o_rest % 16 == 0, MRG_ERR_ARG, "mrg_attn_mod_fwd: operands and their strides must be multiples of 16 bytes");
     ModArgs a = mod_args(d, p);
     a.nblk = p.nblk; a.splits = p.splits;
     doc_tables(d, p, a, stream);
@@ -966,7 +976,7 @@ extern "C" int mrg_attn_mod_bwd(const mrg_attn_mod_desc* d, hipStream_t stream) 
     MRG_REQUIRE((d->Nq == 0 || (d->q && d->o && d->lse && d->d_o && d->dq)) && (d->Nk == 0 || (d->k && d->v && d->dk && d->dv)) && (p.bytes == 0 || d->ws), MRG_ERR_ARG,
                 "mrg_attn_mod_bwd: null pointer");
     MRG_REQUIRE(aligned8(d->q, d->q_bs, d->q_rs, d->q_hs) && aligned8(d->k, d->k_bs, d->k_rs, d->k_hs) && aligned8(d->v, d->v_bs, d->v_rs, d->v_hs)
-                && aligned8(d->o, d->o_bs, d->o_rs, d->o_hs) && aligned8(d->d_o, d->do_bs, d->do_rs, d->do_hs) && aligned8(d->dq, d->dq_bs, d->dq_rs, d->dq_hs)
+                && aligned8(d->o, d->o_bs, d->o_rs, d->o_hs) && (uintptr_t)d->o_rest % 16 == 0 && aligned8(d->d_o, d->do_bs, d->do_rs, d->do_hs) && aligned8(d->dq, d->dq_bs, d->dq_rs, d->dq_hs)
                 && aligned8(d->dk, d->dk_bs, d->dk_rs, d->dk_hs) && aligned8(d->dv, d->dv_bs, d->dv_rs, d->dv_hs), MRG_ERR_ARG,
                 "mrg_attn_mod_bwd: operands and their strides must be multiples of 16 bytes");
     ModArgs a = mod_args(d, p);

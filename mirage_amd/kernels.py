@@ -7,7 +7,7 @@ import ctypes as C
 import json
 import os
 import weakref
-from typing import Dict, Optional, Sequence
+from typing import Dict, NamedTuple, Optional, Sequence
 
 import torch
 
@@ -953,6 +953,12 @@ class ScoreMod:
         self.doc_q, self.doc_k, self.causal, self.prefix = doc_q, doc_k, bool(causal), prefix
 
 
+class AttnSaved(NamedTuple):
+    """what the backward pass of attn_mod_fwd needs besides its operands and o"""
+    lse: torch.Tensor          # fp32 [B, H, Nq]: natural logarithm of the sum of exponentials, -inf where a row saw nothing
+    o_rest: torch.Tensor       # bf16, shape and strides of o: what the rounding of o left out (sum(do o) is formed with both)
+
+
 def _attn_mod_desc(q, k, v, scale, mod: Optional[ScoreMod]):
     _need_cuda(q, "attention q")
     dev = q.device
@@ -1003,32 +1009,34 @@ def _attn_mod_ws(d, backward: int, dev):
 
 def attn_mod_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, mod: Optional[ScoreMod] = None, need_lse: bool = True):
     """softmax(modified scores) v (mrg_attn_mod_fwd): q bf16 [B, Nq, H, hd], k / v bf16 [B, Nk, Hk, hd], H a multiple of Hk, hd 32 or 64, any batch / row /
-    head strides that are multiples of 8 elements.  Returns (o bf16 [B, Nq, H, hd], lse fp32 [B, H, Nq] or None); a row that sees nothing gives
-    o = 0 and lse = -inf."""
+    head strides that are multiples of 8 elements.  Returns (o bf16 [B, Nq, H, hd], AttnSaved for the backward pass, or None without need_lse); a row that
+    sees nothing gives o = 0 and lse = -inf."""
     d, dev = _attn_mod_desc(q, k, v, scale, mod)
     o = torch.empty_like(q, memory_format=_DENSE)
     d.o = o.data_ptr()
     d.o_bs, d.o_rs, d.o_hs, _ = o.stride()
-    lse = None
+    saved = None
     if need_lse:
-        lse = torch.empty((d.B, d.H, d.Nq), dtype=F32, device=dev)
-        d.lse = lse.data_ptr()
+        saved = AttnSaved(torch.empty((d.B, d.H, d.Nq), dtype=F32, device=dev), torch.empty_like(o))
+        d.lse, d.o_rest = saved.lse.data_ptr(), saved.o_rest.data_ptr()
     ws = _attn_mod_ws(d, 0, dev)      # noqa: F841
     _launch(lib.mrg_attn_mod_fwd, d, dev, "mrg_attn_mod_fwd")
-    return o, lse
+    return o, saved
 
 
-def attn_mod_bwd(q, k, v, o, lse, d_o, scale: float, mod: Optional[ScoreMod] = None, dq=None, dk=None, dv=None):
-    """Gradients of attn_mod_fwd: (dq, dk, dv) bf16, new contiguous tensors or the destinations given (views into a fused gradient buffer, apart from
+def attn_mod_bwd(q, k, v, o, saved: AttnSaved, d_o, scale: float, mod: Optional[ScoreMod] = None, dq=None, dk=None, dv=None):
+    """Gradients of attn_mod_fwd, given its o and AttnSaved: (dq, dk, dv) bf16, new contiguous tensors or the destinations given (views into a fused gradient buffer, apart from
     every operand and from each other)."""
     d, dev = _attn_mod_desc(q, k, v, scale, mod)
     oshape, os_ = _heads(o, "attention o", d.B, d.Nq, dev, BF16)
     gshape, gs = _heads(d_o, "attention d_o", d.B, d.Nq, dev, BF16)
     if oshape != q.shape or gshape != q.shape:
         raise ValueError("mirage_amd: attention o and d_o must have the shape of q")
-    if lse is None:
-        raise ValueError("mirage_amd: attn_mod_bwd needs the forward pass's lse")
-    _want(lse, "attention lse", dev, _ONLY32, (d.B, d.H, d.Nq))
+    if not isinstance(saved, AttnSaved):
+        raise ValueError(f"mirage_amd: attn_mod_bwd needs the forward pass's AttnSaved, got {type(saved).__name__}")
+    _want(saved.lse, "attention lse", dev, _ONLY32, (d.B, d.H, d.Nq))
+    if _heads(saved.o_rest, "attention o_rest", d.B, d.Nq, dev, BF16) != (oshape, os_):
+        raise ValueError("mirage_amd: attention o_rest must have the shape and strides of o")
     outs, strides = [], []
     for g, src, what in ((dq, q, "attention dq"), (dk, k, "attention dk"), (dv, v, "attention dv")):
         if g is None:
@@ -1039,7 +1047,7 @@ def attn_mod_bwd(q, k, v, o, lse, d_o, scale: float, mod: Optional[ScoreMod] = N
             for t in (q, k, v, o, d_o, *outs):
                 _need_apart(g, t, what)
         outs.append(g)
-    d.o, d.lse, d.d_o = o.data_ptr(), lse.data_ptr(), d_o.data_ptr()
+    d.o, d.o_rest, d.lse, d.d_o = o.data_ptr(), saved.o_rest.data_ptr(), saved.lse.data_ptr(), d_o.data_ptr()
     d.o_bs, d.o_rs, d.o_hs = os_[:3]
     d.do_bs, d.do_rs, d.do_hs = gs[:3]
     d.dq, d.dk, d.dv = outs[0].data_ptr(), outs[1].data_ptr(), outs[2].data_ptr()

@@ -61,18 +61,18 @@ class _AttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, v, scale, mod):
         need = any(ctx.needs_input_grad)
-        o, lse = K.attn_mod_fwd(q, k, v, scale, mod, need_lse=need)
+        o, saved = K.attn_mod_fwd(q, k, v, scale, mod, need_lse=need)
         if need:
-            ctx.save_for_backward(q, k, v, o, lse)
+            ctx.save_for_backward(q, k, v, o, *saved)
             ctx.how = (scale, mod)
         return o
 
     @staticmethod
     def backward(ctx, d_o):
-        q, k, v, o, lse = ctx.saved_tensors
+        q, k, v, o, *saved = ctx.saved_tensors
         if d_o.stride(-1) != 1:
             d_o = d_o.contiguous()
-        return (*K.attn_mod_bwd(q, k, v, o, lse, d_o, *ctx.how), None, None)
+        return (*K.attn_mod_bwd(q, k, v, o, K.AttnSaved(*saved), d_o, *ctx.how), None, None)
 
 
 def attention(q, k, v, scale: float, mod: Optional[K.ScoreMod] = None):
@@ -148,23 +148,23 @@ class _PackedAttentionFn(torch.autograd.Function):
             freqs = att.freqs(y16.device)
             K.rotary_axes(q, k, pos, freqs, att.sections, pairing=att.pairing, out_q=q, out_k=k)
         need = any(ctx.needs_input_grad)
-        o, lse = K.attn_mod_fwd(q, k, v, att.scale, mod, need_lse=need)
+        o, saved = K.attn_mod_fwd(q, k, v, att.scale, mod, need_lse=need)
         branch, _, _ = E.lin_fwd(o.view(B, N, -1), att.proj)
         if need:
             ctx.att, ctx.mod = att, mod
-            ctx.save_for_backward(y16, qkv, o, lse, pos, freqs)
+            ctx.save_for_backward(y16, qkv, pos, freqs, o, *saved)
         return branch
 
     @staticmethod
     def backward(ctx, dbranch):
-        y16, qkv, o, lse, pos, freqs = ctx.saved_tensors
+        y16, qkv, pos, freqs, o, *saved = ctx.saved_tensors
         att = ctx.att
         B, N, _ = y16.shape
         d_o, _ = E.lin_bwd(dbranch.contiguous(), o.view(B, N, -1), att.proj)
         q, k, v = att.split(qkv.view(B, N, -1, att.head_dim))
         d_qkv = torch.empty_like(qkv)
         dq, dk, dv = att.split(d_qkv.view(B, N, -1, att.head_dim))
-        K.attn_mod_bwd(q, k, v, o, lse, d_o.view(o.shape), att.scale, ctx.mod, dq=dq, dk=dk, dv=dv)
+        K.attn_mod_bwd(q, k, v, o, K.AttnSaved(*saved), d_o.view(o.shape), att.scale, ctx.mod, dq=dq, dk=dk, dv=dv)
         if att.sections is not None:
             K.rotary_axes(dq, dk, pos, freqs, att.sections, pairing=att.pairing, inverse=True, out_q=dq, out_k=dk)
         dy, _ = E.lin_bwd(d_qkv, y16, att.qkv)

@@ -271,7 +271,7 @@ def test_launchers_refuse_on_the_gpu(P):
     t = torch.zeros(1, 8, 4, 64, dtype=BF16, device=dev())
     pos, f = torch.zeros(8, 1, dtype=torch.int32, device=dev()), torch.ones(32, dtype=F64, device=dev())
     x, w = torch.zeros(2, 3, 64, device=dev()), torch.ones(64, device=dev())
-    q, k = t[:, :, :2], t[:, :, 2:]
+    q, k, l = t[:, :, :2], t[:, :, 2:], torch.zeros(1, 4, 8, device=dev())
     bad = [
         (ValueError, lambda: K.rotary_axes(t.half(), None, pos, f, (32,))), (ValueError, lambda: K.rotary_axes(t, k.float(), pos, f, (32,))),
         (ValueError, lambda: K.rotary_axes(q, k, pos.long(), f, (32,))), (ValueError, lambda: K.rotary_axes(q, k, pos, f.float(), (32,))),
@@ -292,8 +292,9 @@ def test_launchers_refuse_on_the_gpu(P):
         (NotImplementedError, lambda: K.attn_mod_fwd(t[..., :48], t[..., :48], t[..., :48], 0.1)), (RuntimeError, lambda: K.attn_mod_fwd(t[..., 4:36], t[..., 4:36], t[..., 4:36], 0.1)),
         (RuntimeError, lambda: K.attn_mod_fwd(t, t, t, -0.1)), (ValueError, lambda: K.attn_mod_fwd(t, t, t, 0.1, K.ScoreMod(doc_q=pos[None, :, 0], doc_k=pos[None, :, 0].long()))),
         (ValueError, lambda: K.attn_mod_fwd(t, t, t, 0.1, K.ScoreMod(slopes=w[:3], pos_q=x, pos_k=x))), (ValueError, lambda: K.attn_mod_fwd(t, t, t, 0.1, K.ScoreMod(causal=True, prefix=pos[:2, 0]))),
-        (ValueError, lambda: K.attn_mod_bwd(t, t, t, t, None, t, 0.1)), (ValueError, lambda: K.attn_mod_bwd(t, t, t, t, x, t, 0.1)),
-        (ValueError, lambda: K.attn_mod_bwd(t, t, t, t, torch.zeros(1, 4, 8, device=dev()), t, 0.1, dq=t)),
+        (ValueError, lambda: K.attn_mod_bwd(t, t, t, t, None, t, 0.1)), (ValueError, lambda: K.attn_mod_bwd(t, t, t, t, l, t, 0.1)),
+        (ValueError, lambda: K.attn_mod_bwd(t, t, t, t, K.AttnSaved(x, t), t, 0.1)), (ValueError, lambda: K.attn_mod_bwd(t, t, t, t, K.AttnSaved(l, q), t, 0.1)),
+        (ValueError, lambda: K.attn_mod_bwd(t, t, t, t, K.AttnSaved(l, t), t, 0.1, dq=t)),
     ]
     for i, (kind, call) in enumerate(bad):
         with pytest.raises(kind):

@@ -286,10 +286,10 @@ def attn_ref(q, k, v, scale, cap, slopes, pos_q, pos_k, doc_q, doc_k, causal, pr
         dp = g @ vh.transpose(-1, -2)
         D = (g * o).sum(-1, keepdim=True)
         ds = p * (dp - D) * steep
-        # D is formed with the o that was stored; fp32 noise of p, dp, D; ds itself is rounded to bf16
-        eD = (g.abs() * eo).sum(-1, keepdim=True)
+        # D is formed with o to 2^-16 of its value, whose weights were rounded to bf16; fp32 noise of p, dp, D; ds enters its products to 2^-16
+        eD = (g.abs() * (eo - o.abs() * HALF16)).sum(-1, keepdim=True)
         fp = (wob + 128 * HALF32) * 4
-        eds = ds.abs() * HALF16 * 1.01 + p * eD + p * ((g.abs() @ vh.abs().transpose(-1, -2)) + (g.abs() * o.abs()).sum(-1, keepdim=True)) * fp
+        eds = ds.abs() * 2.0 ** -16 + p * eD + p * ((g.abs() @ vh.abs().transpose(-1, -2)) + (g.abs() * o.abs()).sum(-1, keepdim=True)) * fp
         fold = lambda t: t.view(B, Hk, G, Nk, hd).sum(2)
         dq = ds @ kh * scale
         dk, dv = fold(ds.transpose(-1, -2) @ qh * scale), fold(p.transpose(-1, -2) @ g)
@@ -352,18 +352,20 @@ def test_attn_mod_matches_the_formula(K, case):
     q, k, v, d_o, scale, m = attn_case(case)
     ref = attn_ref(q, k, v, scale, *m.values(), d_o=d_o)
     mod = K.ScoreMod(**m)
-    o, lse = K.attn_mod_fwd(q, k, v, scale, mod)
+    o, saved = K.attn_mod_fwd(q, k, v, scale, mod)
+    lse = saved.lse
     within(o, *ref["o"], "o")
+    assert bool((saved.o_rest.float().abs() <= HALF16 * o.float().abs()).all())
     empty = torch.isinf(ref["lse"][0])
     assert torch.equal(empty, lse == -math.inf)
     within(torch.where(empty, torch.zeros_like(lse), lse), torch.where(empty, torch.zeros_like(ref["lse"][0]), ref["lse"][0]), ref["lse"][1], "lse")
     assert bool((o.transpose(1, 2)[empty] == 0).all())
     o2, none = K.attn_mod_fwd(q, k, v, scale, mod, need_lse=False)
     assert none is None and torch.equal(o, o2)
-    dq, dk, dv = K.attn_mod_bwd(q, k, v, o, lse, d_o, scale, mod)
+    dq, dk, dv = K.attn_mod_bwd(q, k, v, o, saved, d_o, scale, mod)
     for got, n in ((dq, "dq"), (dk, "dk"), (dv, "dv")):
         within(got, *ref[n], n)
-    again = K.attn_mod_bwd(q, k, v, o, lse, d_o, scale, mod)
+    again = K.attn_mod_bwd(q, k, v, o, saved, d_o, scale, mod)
     assert all(torch.equal(a, b) for a, b in zip((dq, dk, dv), again)), "the same bits on every run"
 
 
@@ -372,7 +374,7 @@ def test_attn_mod_no_keys_no_queries(K):
         q, k, v = (torch.ones(B, n, 2, 64, dtype=BF16, device=dev()) for n in (Nq, Nk, Nk))
         for mod in (None, K.ScoreMod(doc_q=torch.zeros(B, Nq, dtype=torch.int32, device=dev()), doc_k=torch.zeros(B, Nk, dtype=torch.int32, device=dev()), causal=True)):
             o, lse = K.attn_mod_fwd(q, k, v, 0.125, mod)
-            assert bool((o == 0).all()) and bool((lse == -math.inf).all()) and o.shape == q.shape
+            assert bool((o == 0).all()) and bool((lse.lse == -math.inf).all()) and o.shape == q.shape
             for g, src in zip(K.attn_mod_bwd(q, k, v, o, lse, torch.ones_like(q), 0.125, mod), (q, k, v)):
                 assert g.shape == src.shape and bool((g == 0).all())
 
