@@ -36,6 +36,9 @@ constexpr int MAX_SPLITS = 64;
 #ifndef TABMIN
 #define TABMIN 4
 #endif
+#ifndef LEAST
+#define LEAST 4
+#endif
 #ifndef NWF
 #define NWF 4
 #endif
@@ -252,27 +255,32 @@ __device__ __forceinline__ void modify(f32x16& s, f32x16& steep, const ModArgs& 
     }
 }
 
-// scores a lane may not see take `value` (x; with BOTH, y as well): register r stands for the staged row 8 (r >> 2) + (r & 3) behind the lane's
-// first one, `left` and `doc` (null: order alone decides) count from there; visible below `left` (BELOW) or from it on.  One group of four at
-// a time: all 16 conditions at once are 32 scalar registers that the kernels do not have
-template <bool BELOW, bool BOTH>
-__device__ __forceinline__ void hide(f32x16& x, f32x16& y, int left, int mydoc, const int* doc, float value) {
-    asm volatile("" : "+v"(left));                               // the conditions are formed here, not ahead of the branch that rarely comes here
-#pragma unroll
-    for (int g = 0; g < 4; ++g) {
-        bool on[4];
-#pragma unroll
-        for (int e = 0; e < 4; ++e) on[e] = BELOW ? 8 * g + e < left : 8 * g + e >= left;
-        if (doc) {
-            const int4 d = *reinterpret_cast<const int4*>(doc + 8 * g);
-            on[0] &= d.x == mydoc; on[1] &= d.y == mydoc; on[2] &= d.z == mydoc; on[3] &= d.w == mydoc;
+// What a lane sees of a staged tile, one bit per row.  Documents: for every document among the wave's rows (one or two as a rule) one ballot over the
+// tile's rows, `theirs` = the document of the tile's row `lane`.  Order: rows below `left` (BELOW) or from it on.
+template <bool BELOW>
+__device__ __forceinline__ unsigned long long seen_rows(int left, bool bydoc, int mydoc, int theirs) {
+    const unsigned long long upto = left <= 0 ? 0ull : (left >= 64 ? ~0ull : (1ull << left) - 1);
+    unsigned long long m = BELOW ? upto : ~upto;
+    if (bydoc) {
+        unsigned long long same = 0, todo = __builtin_amdgcn_ballot_w64(mydoc >= 0);
+        while (todo) {
+            const int d = __builtin_amdgcn_readlane(mydoc, __builtin_ctzll(todo));
+            const unsigned long long rows = __builtin_amdgcn_ballot_w64(theirs == d);
+            if (mydoc == d) same = rows;
+            todo &= ~__builtin_amdgcn_ballot_w64(mydoc == d);
         }
+        m &= same;
+    }
+    return m;
+}
+// accumulator register r of a lane stands for row 8 (r >> 2) + (r & 3) of its block behind the lane's first one; rows that are not seen take `value`
+__device__ __forceinline__ void hide(f32x16& x, unsigned long long seen, int kb, int lane, float value) {
+    const int bits = (int)((unsigned)(seen >> (kb * 32)) >> (4 * (lane >> 5)));
 #pragma unroll
-        for (int e = 0; e < 4; ++e) {
-            x[4 * g + e] = on[e] ? x[4 * g + e] : value;
-            if (BOTH) y[4 * g + e] = on[e] ? y[4 * g + e] : value;
-        }
-        __builtin_amdgcn_sched_barrier(0);
+    for (int r = 0; r < 16; ++r) {
+        int t;                                                    // all ones or none; as asm, because the compiler turns the builtin into a compare and a select
+        asm("v_bfe_i32 %0, %1, %2, 1" : "=v"(t) : "v"(bits), "n"(8 * (r >> 2) + (r & 3)));
+        x[r] = __int_as_float((t & __float_as_int(x[r])) | (~t & __float_as_int(value)));
     }
 }
 
@@ -294,7 +302,6 @@ __global__ __launch_bounds__(64 * NW, FOCC) void attn_mod_fwd_kernel(const ModAr
     __shared__ __attribute__((aligned(16))) char ldsK[2][TB];
     __shared__ __attribute__((aligned(16))) char ldsV[2][TB];
     __shared__ __attribute__((aligned(16))) float ldsP[2][BIAS ? 3 * TT : 4];
-    __shared__ __attribute__((aligned(16))) int ldsD[2][TT];
     __shared__ unsigned long long noted[3];                      // of tile n: slot n % 3
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int bh, blk;
@@ -359,8 +366,8 @@ __global__ __launch_bounds__(64 * NW, FOCC) void attn_mod_fwd_kernel(const ModAr
     ColFrag<HD> fv; fv.init(lane);
     Dma<HD, NW> dk, dv;
     dk.init(a.k_rs, lane, wave); dv.init(a.v_rs, lane, wave);
-    constexpr int AXW = (3 + NW - 1) / NW;                       // the waves share the axes; the last one takes the documents
-    float pv[AXW] = {}; int dc = 0;
+    constexpr int AXW = (3 + NW - 1) / NW;                       // the waves share the axes
+    float pv[AXW] = {}; int dc = 0, dn = 0;                      // documents of the tile's rows, one per lane: of this tile and of the next
     auto fetch = [&](int t, int buf) {
         dk.fetch(kp, t * TT, a.Nk, ldsK[buf], lane, wave);
         dv.fetch(vp, t * TT, a.Nk, ldsV[buf], lane, wave);
@@ -369,14 +376,14 @@ __global__ __launch_bounds__(64 * NW, FOCC) void attn_mod_fwd_kernel(const ModAr
 #pragma unroll
             for (int x = 0; x < AXW; ++x) if (wave + NW * x < a.axes) pv[x] = posk[(long)r * a.axes + wave + NW * x];
         }
-        if (docs && wave == NW - 1) dc = docs[r];
+        if (docs) dn = docs[r];
     };
     auto land = [&](int buf, int slot, bool partial) {
         if (BIAS) {
 #pragma unroll
             for (int x = 0; x < AXW; ++x) if (wave + NW * x < a.axes) ldsP[buf][(wave + NW * x) * TT + lane] = pv[x];
         }
-        if (docs && wave == NW - 1) ldsD[buf][lane] = dc;
+        dc = dn;
         dma_landed();
         if (partial) dv.tidy(ldsV[buf], &noted[slot], lane, wave);
     };
@@ -417,6 +424,8 @@ __global__ __launch_bounds__(64 * NW, FOCC) void attn_mod_fwd_kernel(const ModAr
         const int j0 = (split + (base + i) * a.splits) * TT;
         const bool see = (wk.wsee >> i) & 1, whole = (wk.wwhole >> i) & 1;
         if (see) {
+            unsigned long long seen = ~0ull;
+            if (!whole) seen = seen_rows<true>(lim - j0, docs != nullptr, mydoc, dc);
             const uint32_t kt = lds_addr(ldsK[buf]), vt = lds_addr(ldsV[buf]);
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
@@ -425,7 +434,7 @@ __global__ __launch_bounds__(64 * NW, FOCC) void attn_mod_fwd_kernel(const ModAr
 #pragma unroll
                 for (int kk = 0; kk < KS; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fk.read(kt, kb * 32, kk), qf[kk], s, 0, 0, 0);
                 modify<CAP, BIAS, false>(s, s, a, mine, ldsP[buf], kb * 32, kslope, lane);
-                if (!whole) hide<true, false>(s, s, lim - j0 - kb * 32 - 4 * (lane >> 5), mydoc, docs ? &ldsD[buf][kb * 32 + 4 * (lane >> 5)] : nullptr, -INFINITY);
+                if (!whole) hide(s, seen, kb, lane, -INFINITY);
                 float mx = s[0];
 #pragma unroll
                 for (int r = 1; r < 16; ++r) mx = fmaxf(mx, s[r]);
@@ -458,12 +467,7 @@ __global__ __launch_bounds__(64 * NW, FOCC) void attn_mod_fwd_kernel(const ModAr
                     for (int dj = 0; dj < DJ; ++dj) o[dj] = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fv.read(vt, kb * 32 + 16 * m, dj), p, o[dj], 0, 0, 0);
                 }
             }
-            unsigned long long nt = noted[slot];
-            while (nt) {
-                const int r = __builtin_ctzll(nt);
-                nt &= nt - 1;
-                if (j0 + r < lim && (!docs || ldsD[buf][r] == mydoc)) poisoned = true;
-            }
+            if (((wk.part >> i) & 1) && (noted[slot] & seen)) poisoned = true;
         }
         if (in >= 0) land(buf ^ 1, slot_n, (wk.part >> in) & 1);
         __syncthreads();
@@ -542,7 +546,6 @@ __global__ __launch_bounds__(256, BOCC) void attn_mod_bwd_kernel(const ModArgs a
     __shared__ __attribute__((aligned(16))) char ldsX[2][TB];
     __shared__ __attribute__((aligned(16))) char ldsY[2][TB];
     __shared__ __attribute__((aligned(16))) float ldsP[2][BIAS ? 3 * TT : 4];
-    __shared__ __attribute__((aligned(16))) int ldsD[2][TT];
     __shared__ __attribute__((aligned(16))) float ldsL[2][OWN_Q ? 4 : 2 * TT];      // lse (log2 units) and sum(do o) of the staged queries
     __shared__ unsigned long long noted[3];
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
@@ -628,7 +631,7 @@ __global__ __launch_bounds__(256, BOCC) void attn_mod_bwd_kernel(const ModArgs a
     ColFrag<HD> fc; fc.init(lane);
     Dma<HD, 4> dx, dy;
     dx.init(OWN_Q ? a.k_rs : a.q_rs, lane, wave); dy.init(OWN_Q ? a.v_rs : a.do_rs, lane, wave);
-    float pv = 0.f, lv = 0.f; int dc = 0;
+    float pv = 0.f, lv = 0.f; int dc = 0, dn = 0;
     const bf16_t *X = nullptr, *Y = nullptr;
     const float* rowv = nullptr;                                 // OWN_K: wave 0 reads lse, wave 1 sum(do o)
     auto fetch = [&](int t, int buf) {
@@ -636,12 +639,12 @@ __global__ __launch_bounds__(256, BOCC) void attn_mod_bwd_kernel(const ModArgs a
         dy.fetch(Y, t * TT, NS, ldsY[buf], lane, wave);
         const int r = min(t * TT + lane, NS - 1);
         if (BIAS && wave < a.axes) pv = pos_s[(long)r * a.axes + wave];
-        if (bydoc && wave == 3) dc = doc_s[r];
+        if (bydoc) dn = doc_s[r];
         if (!OWN_Q && wave < 2) lv = rowv[r];
     };
     auto land = [&](int t, int buf, int slot, bool partial) {
         if (BIAS && wave < a.axes) ldsP[buf][wave * TT + lane] = pv;
-        if (bydoc && wave == 3) ldsD[buf][lane] = dc;
+        dc = dn;
         if (!OWN_Q && wave < 2) {
             // negated: raw scores and dp start from them in the accumulators; behind the last query and in rows that saw nothing p = 0
             const bool in = t * TT + lane < NS;
@@ -694,6 +697,8 @@ __global__ __launch_bounds__(256, BOCC) void attn_mod_bwd_kernel(const ModArgs a
         const int j0 = (split + (base + i) * a.splits) * TT;
         const bool see = (wk.wsee >> i) & 1, whole = (wk.wwhole >> i) & 1;
         if (see) {
+            unsigned long long seen = ~0ull;
+            if (!whole) seen = seen_rows<OWN_Q>(edge - j0, bydoc, mydoc, dc);
             const float kslope = !BIAS ? 0.f : (CAP ? a.slopes[h] * LOG2E_F : a.slopes[h] / a.scale);
             const uint32_t xb = lds_addr(ldsX[buf]), yb = lds_addr(ldsY[buf]);
 #pragma unroll
@@ -729,9 +734,8 @@ __global__ __launch_bounds__(256, BOCC) void attn_mod_bwd_kernel(const ModArgs a
                     }
                 }
                 if (!whole) {
-                    const int left = edge - j0 - kb * 32 - 4 * (lane >> 5);
-                    const int* doc = bydoc ? &ldsD[buf][kb * 32 + 4 * (lane >> 5)] : nullptr;
-                    hide<OWN_Q, !OWN_Q>(dp, s, left, mydoc, doc, 0.f);
+                    if (!OWN_Q) hide(s, seen, kb, lane, 0.f);
+                    hide(dp, seen, kb, lane, 0.f);
                 }
 #pragma unroll
                 for (int m = 0; m < 2; ++m) {
@@ -749,12 +753,7 @@ __global__ __launch_bounds__(256, BOCC) void attn_mod_bwd_kernel(const ModArgs a
                     }
                 }
             }
-            unsigned long long nt = noted[slot];
-            while (nt) {
-                const int r = __builtin_ctzll(nt), j = j0 + r;
-                nt &= nt - 1;
-                if ((OWN_Q ? j < edge : (j >= edge && j < NS)) && (!bydoc || ldsD[buf][r] == mydoc)) poisoned = true;
-            }
+            if (((wk.part >> i) & 1) && (noted[slot] & seen)) poisoned = true;
         }
         if (in >= 0) land(tn, buf ^ 1, slot_n, (wk.part >> in) & 1);
         __syncthreads();
@@ -835,14 +834,15 @@ Plan plan_for(const mrg_attn_mod_desc* d, bool backward) {
         // up to 32 queries: workgroups of one wave, four resident per CU, and the keys cut until every CU has its four
         p.nw = d->Nq <= 32 ? 1 : NWF;
         p.nblk = (d->Nq + 32 * p.nw - 1) / (32 * p.nw);
-        p.splits = splits_for((long)d->B * d->H * p.nblk, p.nw == 1 ? WANT1 : WANTF, p.ntk, 4);
+        p.splits = splits_for((long)d->B * d->H * p.nblk, p.nw == 1 ? WANT1 : WANTF, p.ntk, p.nw == 1 ? 4 : LEAST);
         p.tables = d->doc_k && (p.nw == 1 ? p.ntk > 2 : p.ntk > TABMIN);
         if (p.splits > 1) { p.part = take(4l * p.splits * rows_q * d->head_dim); p.part_ml = take(8l * p.splits * rows_q); }
     } else {
         p.dsum = take(4l * rows_q);
         p.tables = d->doc_k && (p.ntk > TABMIN || p.ntq > TABMIN);
-        p.dq_splits = splits_for((long)d->B * d->H * ((d->Nq + 127) / 128), WANTQ, p.ntk, 4);
-        p.dkv_splits = splits_for((long)d->B * d->Hk * ((d->Nk + 127) / 128), d->causal ? WANTKC : WANTK, p.ntq, 4);
+        p.dq_splits = splits_for((long)d->B * d->H * ((d->Nq + 127) / 128), WANTQ, p.ntk, LEAST);
+        p.dkv_splits = splits_for((long)d->B * d->Hk * ((d->Nk + 127) / 128), d->causal ? WANTKC : WANTK, p.ntq * (d->H / d->Hk), LEAST);
+        if (p.dkv_splits > p.ntq) p.dkv_splits = p.ntq ? p.ntq : 1;
         long part = 0;
         if (p.dq_splits > 1) part = 4l * p.dq_splits * rows_q * d->head_dim;
         if (p.dkv_splits > 1 && 8l * p.dkv_splits * rows_k * d->head_dim > part) part = 8l * p.dkv_splits * rows_k * d->head_dim;
