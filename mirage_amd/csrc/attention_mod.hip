@@ -31,7 +31,7 @@ constexpr float LOG2E_F = 1.4426950408889634f, LN2_F = 0.6931471805599453f;
 constexpr int TT = 64;                        // tokens of a staged tile
 constexpr int MAX_SPLITS = 64;
 #ifndef FOCC
-#define FOCC 3
+#define FOCC (BIAS ? 2 : 3)
 #endif
 #ifndef TABMIN
 #define TABMIN 4
@@ -226,16 +226,16 @@ struct Walk { unsigned long long see, part, wsee, wwhole; };
 __device__ __forceinline__ int take_tile(unsigned long long& see) { const int i = __builtin_ctzll(see); see &= see - 1; return i; }
 
 // scores in registers: CAP -> log2 units, otherwise q.k stays as it is (the exponential takes the factor) and the bias comes in q.k's units.
-// kslope: slope / scale, or with CAP slope log2(e).  steep: 1 - tanh^2
+// kslope: slope / scale, or with CAP slope log2(e).  steep: (1 - tanh^2) / 4
 template <bool CAP, bool BIAS, bool STEEP>
 __device__ __forceinline__ void modify(f32x16& s, f32x16& steep, const ModArgs& a, const float (&mine)[3], const float* pos, int row0, float kslope, int lane) {
     if (CAP) {
         const float up = 2.f * a.scale * LOG2E_F / a.cap, capl = a.cap * LOG2E_F;
 #pragma unroll
         for (int r = 0; r < 16; ++r) {
-            const float th = fmaf(-2.f, __builtin_amdgcn_rcpf(fast_exp2(s[r] * up) + 1.f), 1.f);       // tanh(x) = 1 - 2 / (e^2x + 1)
-            s[r] = capl * th;
-            if (STEEP) steep[r] = fmaf(-th, th, 1.f);
+            const float u = __builtin_amdgcn_rcpf(fast_exp2(s[r] * up) + 1.f);                         // tanh(x) = 1 - 2 u, u = 1 / (e^2x + 1)
+            s[r] = fmaf(u, -2.f * capl, capl);
+            if (STEEP) steep[r] = fmaf(-u, u, u);                                                      // 1 - tanh^2 = 4 (u - u^2)
         }
     }
     if (BIAS) {
@@ -764,7 +764,7 @@ __global__ __launch_bounds__(256, BOCC) void attn_mod_bwd_kernel(const ModArgs a
     }
     }
     if (row >= NO) return;
-    const float fa_out = poisoned ? NAN : a.scale, fb_out = poisoned ? NAN : 1.f;
+    const float fa_out = poisoned ? NAN : (CAP ? 4.f * a.scale : a.scale), fb_out = poisoned ? NAN : 1.f;
     if (a.splits > 1) {
         const long rows = (long)a.B * OH * NO;
         float* base = a.part + (((long)split * rows + ((long)b * OH + ho) * NO + row) * (OWN_Q ? 1 : 2)) * HD;
