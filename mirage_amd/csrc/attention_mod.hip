@@ -68,6 +68,7 @@ struct ModArgs {
     float* dsum;                              // [B, H, Nq] sum(do o)
     float* part; float* part_ml; int splits;  // split rows: [split][rows][HD] unnormalised, [split][rows][2] {max, sum}
     int nblk;                                 // row blocks of the owner
+    const int* order;                         // [B][nblk]: the row blocks, longest first (null: causal order tells, or they are alike)
 };
 
 // byte offset of 16-byte chunk c of row r in a [TT][HD] bf16 tile; the XOR spreads the rows that one instruction reads over the banks
@@ -124,8 +125,20 @@ __device__ __forceinline__ float2 halves(float v) {
     const auto r = __builtin_amdgcn_permlane32_swap(__float_as_uint(v), __float_as_uint(v), false, false);
     return make_float2(__uint_as_float(r[0]), __uint_as_float(r[1]));
 }
-__device__ __forceinline__ int wave_min_i(int v) { for (int o = 32; o > 0; o >>= 1) v = min(v, __shfl_xor(v, o, 64)); return v; }
-__device__ __forceinline__ int wave_max_i(int v) { for (int o = 32; o > 0; o >>= 1) v = max(v, __shfl_xor(v, o, 64)); return v; }
+// minimum / maximum over the wave, in registers: four DPP steps within 16 lanes, then the swaps of rows and of halves
+template <bool MAX> __device__ __forceinline__ int pick(int a, int b) { return MAX ? max(a, b) : min(a, b); }
+template <bool MAX> __device__ __forceinline__ int wave_pick(int v) {
+    v = pick<MAX>(v, __builtin_amdgcn_update_dpp(v, v, 0xB1, 0xF, 0xF, true));      // quad_perm [1,0,3,2]
+    v = pick<MAX>(v, __builtin_amdgcn_update_dpp(v, v, 0x4E, 0xF, 0xF, true));      // quad_perm [2,3,0,1]
+    v = pick<MAX>(v, __builtin_amdgcn_update_dpp(v, v, 0x141, 0xF, 0xF, true));     // row_half_mirror
+    v = pick<MAX>(v, __builtin_amdgcn_update_dpp(v, v, 0x140, 0xF, 0xF, true));     // row_mirror
+    const auto r = __builtin_amdgcn_permlane16_swap(v, v, false, false);
+    v = pick<MAX>(r[0], r[1]);
+    const auto h = __builtin_amdgcn_permlane32_swap(v, v, false, false);
+    return pick<MAX>(h[0], h[1]);
+}
+__device__ __forceinline__ int wave_min_i(int v) { return wave_pick<false>(v); }
+__device__ __forceinline__ int wave_max_i(int v) { return wave_pick<true>(v); }
 
 // does any of the 8 bf16 values have an all-ones exponent
 __device__ __forceinline__ bool not_finite(const uint4 w) {
@@ -192,8 +205,11 @@ struct Dma {
 };
 __device__ __forceinline__ void dma_landed() { asm volatile("s_waitcnt vmcnt(0)" ::: "memory"); }
 
-// smallest / largest document and number of valid tokens of every 64-token tile of a batch row: the queries' tiles, then the keys' (0 tiles of
-// queries where both sides are the same tokens)
+// smallest / largest document and number of valid tokens of a tile whose tokens the wave's lanes hold
+__device__ __forceinline__ int4 doc_range(int d) {
+    return make_int4(wave_min_i(d < 0 ? 0x7fffffff : d), wave_max_i(d), __popcll(__builtin_amdgcn_ballot_w64(d >= 0)), 0);
+}
+// ... of every tile of every batch row: the queries' tiles, then the keys' (no tiles of queries where both sides are the same tokens)
 __global__ __launch_bounds__(256) void doc_tiles_kernel(const int* __restrict__ doc_q, const int* __restrict__ doc_k, int4* __restrict__ tab_q, int4* __restrict__ tab_k,
                                                         int B, int Nq, int Nk, int ntq, int ntk) {
     int t = blockIdx.x * 4 + (threadIdx.x >> 6);
@@ -203,10 +219,8 @@ __global__ __launch_bounds__(256) void doc_tiles_kernel(const int* __restrict__ 
     const int nt = ofk ? ntk : ntq, N = ofk ? Nk : Nq;
     if (t >= B * nt) return;
     const int b = t / nt, j = (t - b * nt) * TT + lane;
-    const int d = j < N ? (ofk ? doc_k : doc_q)[(long)b * N + j] : -1;
-    const int lo = wave_min_i(d < 0 ? 0x7fffffff : d), hi = wave_max_i(d);
-    const int n = __popcll(__builtin_amdgcn_ballot_w64(d >= 0));
-    if (lane == 0) (ofk ? tab_k : tab_q)[t] = make_int4(lo, hi, n, 0);
+    const int4 e = doc_range(j < N ? (ofk ? doc_k : doc_q)[(long)b * N + j] : -1);
+    if (lane == 0) (ofk ? tab_k : tab_q)[t] = e;
 }
 
 // Work of a launch: `heads` (batch, head) pairs of `per` row blocks each.  Workgroups are dispatched round-robin over the 8 dies; a die gets whole
@@ -218,6 +232,72 @@ __device__ __forceinline__ void place(int id, int heads, int per, bool by_length
     const int die = id % dies, idx = id / dies;
     if (by_length) { head = die * mine + idx % mine; blk = idx / mine; }
     else { head = die * mine + idx / per; blk = idx % per; }
+}
+
+// Tables and order of the row blocks in one launch, one workgroup per batch row: the tiles' ranges, the number of tiles that each block of `rows` rows
+// will walk, and the blocks by that number, the longest first (equal ones in their place).  order_q: blocks of queries, order_k (may be null):
+// of keys.  At 8192 tokens in 12 documents and 16 heads the blocks walk 5 to 18 tiles; dispatched as they come the last round ran half empty.
+constexpr int ORDER_TILES = 512, ORDER_THREADS = 1024, ORDER_PARTS = 8;
+struct OrderArgs { const int* doc_q; const int* doc_k; int4* tab_q; int4* tab_k; int* order_q; int* order_k; int Nq, Nk, ntq, ntk, rows, causal; const int* prefix; };
+__device__ __forceinline__ void order_tiles(const int* __restrict__ doc, int N, int nt, int4* table, int4* __restrict__ out) {
+    const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
+    constexpr int W = ORDER_THREADS / 64;
+    for (int t0 = wave; t0 < nt; t0 += 8 * W) {
+        int d[8];                                                 // eight tiles of this wave requested at once
+#pragma unroll
+        for (int i = 0; i < 8; ++i) { const int j = (t0 + W * i) * TT + lane; d[i] = j < N ? doc[j] : -1; }
+#pragma unroll
+        for (int i = 0; i < 8; ++i) {
+            const int t = t0 + W * i;
+            const int4 e = doc_range(d[i]);
+            if (t < nt && lane == 0) { table[t] = e; out[t] = e; }
+        }
+    }
+}
+__device__ __forceinline__ int part_sum(int v) { for (int o = 1; o < ORDER_PARTS; o <<= 1) v += __shfl_xor(v, o, 64); return v; }
+__global__ __launch_bounds__(ORDER_THREADS) void doc_order_kernel(const OrderArgs a) {
+    __shared__ int4 tq[ORDER_TILES], tk[ORDER_TILES];
+    __shared__ int count[ORDER_TILES];
+    const int b = blockIdx.x;
+    const bool same = a.doc_q == a.doc_k && a.Nq == a.Nk;
+    order_tiles(a.doc_k + (long)b * a.Nk, a.Nk, a.ntk, tk, a.tab_k + (long)b * a.ntk);
+    if (!same) order_tiles(a.doc_q + (long)b * a.Nq, a.Nq, a.ntq, tq, a.tab_q + (long)b * a.ntq);
+    const int off = a.Nk - a.Nq, pre = a.causal ? (a.prefix ? min(max(a.prefix[b], 0), a.Nk) : 0) : a.Nk;
+    const bool alike = same && !a.causal;                         // keys are seen by as many tiles as queries see
+    const int part = threadIdx.x % ORDER_PARTS;
+    for (int side = 0; side < (a.order_k && !alike ? 2 : 1); ++side) {
+        const int N = side ? a.Nk : a.Nq, nblk = (N + a.rows - 1) / a.rows, nts = side ? a.ntq : a.ntk;
+        const int4* own = side || same ? tk : tq;
+        const int4* other = !side || same ? tk : tq;
+        __syncthreads();
+        for (int i0 = 0; i0 < nblk; i0 += ORDER_THREADS / ORDER_PARTS) {
+            const int i = i0 + threadIdx.x / ORDER_PARTS;
+            int n = 0;
+            if (i < nblk) {
+                const int r0 = i * a.rows, r1 = min(r0 + a.rows, N) - 1;
+                int lo = 0x7fffffff, hi = -1;
+                for (int t = r0 / TT; t <= r1 / TT; ++t) { lo = min(lo, own[t].x); hi = max(hi, own[t].y); }
+                const int edge = side ? (r0 < pre ? 0 : r0 - off) : max(pre, min(r1 + off + 1, a.Nk));
+                for (int t = part; t < nts; t += ORDER_PARTS) n += other[t].x <= hi && other[t].y >= lo && (side ? t * TT + TT > edge : t * TT < edge);
+            }
+            n = part_sum(n);
+            if (i < nblk && part == 0) count[i] = n;
+        }
+        __syncthreads();
+        for (int i0 = 0; i0 < nblk; i0 += ORDER_THREADS / ORDER_PARTS) {
+            const int i = i0 + threadIdx.x / ORDER_PARTS;
+            int rank = 0;
+            if (i < nblk) {
+                const int n = count[i];
+                for (int j = part; j < nblk; j += ORDER_PARTS) rank += count[j] > n || (count[j] == n && j < i);
+            }
+            rank = part_sum(rank);
+            if (i < nblk && part == 0) {
+                (side ? a.order_k : a.order_q)[(long)b * nblk + rank] = i;
+                if (alike && a.order_k) a.order_k[(long)b * nblk + rank] = i;
+            }
+        }
+    }
 }
 
 // ---- the tiles a row block walks, 64 at a time, one per lane: seen by some row of the workgroup; of those, not by every row in whole; seen by
@@ -305,10 +385,11 @@ __global__ __launch_bounds__(64 * NW, FOCC) void attn_mod_fwd_kernel(const ModAr
     __shared__ unsigned long long noted[3];                      // of tile n: slot n % 3
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int bh, blk;
-    place(blockIdx.x, a.B * a.H, a.nblk * a.splits, a.causal, bh, blk);
+    place(blockIdx.x, a.B * a.H, a.nblk * a.splits, a.causal || a.order, bh, blk);
     const int split = blk % a.splits, b = bh / a.H, h = bh - b * a.H, hk = h / a.G;
     blk /= a.splits;
-    if (a.causal) blk = a.nblk - 1 - blk;                       // the last queries see the most
+    if (a.order) blk = a.order[(long)b * a.nblk + blk];
+    else if (a.causal) blk = a.nblk - 1 - blk;                  // the last queries see the most
     const bf16_t* kp = a.k + (long)b * a.k_bs + (long)hk * a.k_hs;
     const bf16_t* vp = a.v + (long)b * a.v_bs + (long)hk * a.v_hs;
     const int* docs = a.doc_k ? a.doc_k + (long)b * a.Nk : nullptr;
@@ -551,10 +632,11 @@ __global__ __launch_bounds__(256, BOCC) void attn_mod_bwd_kernel(const ModArgs a
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int OH = OWN_Q ? a.H : a.Hk;                                               // the owner's head: a query head or a key head
     int bo, blk;
-    place(blockIdx.x, a.B * OH, a.nblk * a.splits, a.causal, bo, blk);
+    place(blockIdx.x, a.B * OH, a.nblk * a.splits, a.causal || a.order, bo, blk);
     const int split = blk % a.splits, b = bo / OH, ho = bo - b * OH;
     blk /= a.splits;
-    if (OWN_Q && a.causal) blk = a.nblk - 1 - blk;                                   // the last queries see the most, the first keys are seen the most
+    if (a.order) blk = a.order[(long)b * a.nblk + blk];
+    else if (OWN_Q && a.causal) blk = a.nblk - 1 - blk;                                   // the last queries see the most, the first keys are seen the most
     const int NO = OWN_Q ? a.Nq : a.Nk, NS = OWN_Q ? a.Nk : a.Nq;                    // rows of the owner's side and of the staged side
     const int off = a.Nk - a.Nq;
     const int pre = a.causal ? (a.prefix ? min(max(a.prefix[b], 0), a.Nk) : 0) : a.Nk;
@@ -812,8 +894,8 @@ __global__ __launch_bounds__(256) void attn_mod_sum_kernel(const float* __restri
 // ================================================ host ==================================================
 struct Plan {
     int ntq, ntk, nw, nblk, splits, dq_splits, dkv_splits;
-    bool tables;
-    long tab_q, tab_k, dsum, part, part_ml, bytes;             // byte offsets into the workspace
+    bool tables, ordered;
+    long tab_q, tab_k, order_q, order_k, dsum, part, part_ml, bytes;             // byte offsets into the workspace
 };
 
 int splits_for(long blocks, long want, int tiles, int least) {  // enough workgroups for the chip, but `least` tiles for each
@@ -848,7 +930,14 @@ Plan plan_for(const mrg_attn_mod_desc* d, bool backward) {
         if (p.dkv_splits > 1 && 8l * p.dkv_splits * rows_k * d->head_dim > part) part = 8l * p.dkv_splits * rows_k * d->head_dim;
         p.part = take(part);                                    // used by dq first, by dk / dv behind it
     }
-    if (p.tables) { p.tab_q = take(16l * d->B * p.ntq); p.tab_k = take(16l * d->B * p.ntk); }
+    if (p.tables) {
+        p.tab_q = take(16l * d->B * p.ntq); p.tab_k = take(16l * d->B * p.ntk);
+        // more workgroups than run at once (three or two per CU), and tables that one workgroup per batch row makes in a few microseconds
+        const int rows = backward ? 128 : 32 * p.nw;
+        const long blocks = (long)d->B * (backward ? (d->Hk < d->H ? d->Hk : d->H) : d->H) * ((d->Nq + rows - 1) / rows);
+        p.ordered = blocks > (backward ? 512 : 768) && p.ntq <= ORDER_TILES && p.ntk <= ORDER_TILES && p.ntq > 0 && p.ntk > 0 && p.nw != 1;
+        if (p.ordered) { p.order_q = take(4l * d->B * ((d->Nq + rows - 1) / rows)); p.order_k = take(backward ? 4l * d->B * ((d->Nk + rows - 1) / rows) : 0); }
+    }
     p.bytes = at;
     return p;
 }
@@ -894,10 +983,17 @@ ModArgs mod_args(const mrg_attn_mod_desc* d, const Plan& p) {
     return a;
 }
 
-void doc_tables(const mrg_attn_mod_desc* d, const Plan& p, ModArgs& a, hipStream_t st) {
+void doc_tables(const mrg_attn_mod_desc* d, const Plan& p, ModArgs& a, bool backward, hipStream_t st) {
     if (!p.tables) return;
     const bool same = d->doc_q == d->doc_k && d->Nq == d->Nk;
     if (same) a.tab_q = a.tab_k;
+    if (p.ordered) {
+        char* ws = (char*)d->ws;
+        const OrderArgs o = {d->doc_q, d->doc_k, (int4*)a.tab_q, (int4*)a.tab_k, (int*)(ws + p.order_q), backward ? (int*)(ws + p.order_k) : nullptr,
+                             d->Nq, d->Nk, p.ntq, p.ntk, backward ? 128 : 32 * p.nw, d->causal != 0, d->prefix};
+        hipLaunchKernelGGL(doc_order_kernel, dim3(d->B), dim3(ORDER_THREADS), 0, st, o);
+        return;
+    }
     const int ntq = same || !d->doc_q ? 0 : p.ntq, tiles = d->B * (ntq + p.ntk);
     if (tiles) hipLaunchKernelGGL(doc_tiles_kernel, dim3((tiles + 3) / 4), dim3(256), 0, st, d->doc_q, d->doc_k, (int4*)a.tab_q, (int4*)a.tab_k, d->B, d->Nq, d->Nk, ntq, p.ntk);
 }
@@ -956,7 +1052,8 @@ extern "C" int mrg_attn_mod_fwd(const mrg_attn_mod_desc* d, hipStream_t stream) 
                 && aligned8(d->o, d->o_bs, d->o_rs, d->o_hs) && (uintptr_t)d->o_rest % 16 == 0, MRG_ERR_ARG, "mrg_attn_mod_fwd: operands and their strides must be multiples of 16 bytes");
     ModArgs a = mod_args(d, p);
     a.nblk = p.nblk; a.splits = p.splits;
-    doc_tables(d, p, a, stream);
+    if (p.ordered) a.order = (const int*)((char*)d->ws + p.order_q);
+    doc_tables(d, p, a, false, stream);
     const dim3 grid((unsigned)((long)a.B * a.H * a.nblk * a.splits));
     if (d->head_dim == 64) { if (p.nw == 1) fwd_go<64, 1>(a, grid, stream); else fwd_go<64, NWF>(a, grid, stream); }
     else { if (p.nw == 1) fwd_go<32, 1>(a, grid, stream); else fwd_go<32, NWF>(a, grid, stream); }
@@ -980,8 +1077,10 @@ extern "C" int mrg_attn_mod_bwd(const mrg_attn_mod_desc* d, hipStream_t stream) 
                 && aligned8(d->dk, d->dk_bs, d->dk_rs, d->dk_hs) && aligned8(d->dv, d->dv_bs, d->dv_rs, d->dv_hs), MRG_ERR_ARG,
                 "mrg_attn_mod_bwd: operands and their strides must be multiples of 16 bytes");
     ModArgs a = mod_args(d, p);
-    doc_tables(d, p, a, stream);
+    doc_tables(d, p, a, true, stream);
+    if (p.ordered) a.order = (const int*)((char*)d->ws + p.order_q);
     bwd_side<true>(a, p.dq_splits, d->head_dim, stream);
+    if (p.ordered) a.order = (const int*)((char*)d->ws + p.order_k);
     bwd_side<false>(a, p.dkv_splits, d->head_dim, stream);
     return mrg_check_launch("mrg_attn_mod_bwd");
 }
