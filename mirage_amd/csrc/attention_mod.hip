@@ -30,29 +30,6 @@ namespace {
 constexpr float LOG2E_F = 1.4426950408889634f, LN2_F = 0.6931471805599453f;
 constexpr int TT = 64;                        // tokens of a staged tile
 constexpr int MAX_SPLITS = 64;
-#ifndef FOCC
-#define FOCC (BIAS ? 2 : 3)
-#endif
-#ifndef TABMIN
-#define TABMIN 4
-#endif
-#ifndef LEAST
-#define LEAST 4
-#endif
-#ifndef NWF
-#define NWF 4
-#endif
-#ifndef WANT1
-#define WANT1 2048
-#define WANTF 512
-#define WANTQ 512
-#define WANTK 512
-#define WANTKC 1024
-#endif
-#ifndef BOCC
-#define BOCC (OWN_Q && !BIAS ? 3 : 2)
-#endif
-
 struct ModArgs {
     const bf16_t* q; const bf16_t* k; const bf16_t* v; bf16_t* o; bf16_t* o_rest; float* lse;
     long q_bs, q_rs, q_hs, k_bs, k_rs, k_hs, v_bs, v_rs, v_hs, o_bs, o_rs, o_hs;
@@ -157,10 +134,9 @@ struct Dma {
     static constexpr int CPR = HD / 8, RPB = 64 / CPR, NB = TT / RPB, PER = NB / NW;      // rows per block, blocks per tile and per wave
     static constexpr int PAR = (HD == 64 && NW == 1) ? 2 : 1;
     uint32_t off[PAR];
-    int rs2, r0, c16;
+    int rs2;
     __device__ __forceinline__ int block(int j, int wave) const {                          // j-th block of this wave
         if (NW == 1) return j;
-        if (NW == 2) return wave + 2 * j;
         return HD == 64 ? (wave & 1) + 4 * (wave >> 1) + 2 * j : wave;
     }
     __device__ __forceinline__ void init(long rs, int lane, int wave) {
@@ -377,7 +353,7 @@ __device__ __forceinline__ void store_o(const ModArgs& a, long at, const float4 
 // NW waves of 32 queries.  NW = 1 serves up to 32 queries (a pooled or a single new token): every workgroup is one wave, and the keys are
 // split over many of them.
 template <int HD, int NW, bool CAP, bool BIAS>
-__global__ __launch_bounds__(64 * NW, FOCC) void attn_mod_fwd_kernel(const ModArgs a) {
+__global__ __launch_bounds__(64 * NW, BIAS ? 2 : 3) void attn_mod_fwd_kernel(const ModArgs a) {
     constexpr int KS = HD / 16, DJ = HD / 32, NT = 64 * NW, TB = TT * HD * 2;
     __shared__ __attribute__((aligned(16))) char ldsK[2][TB];
     __shared__ __attribute__((aligned(16))) char ldsV[2][TB];
@@ -622,7 +598,7 @@ __global__ __launch_bounds__(256) void attn_mod_join_kernel(const ModArgs a) {
 //   OWN_K: lane = key, tiles of queries: S = Q K^T,  dP = dO V^T,  dV^T += dO^T P, dK^T += Q^T dS
 // X, Y: the staged matrices (K, V or Q, dO); own fragments: (Q, dO) or (K, V).  OWN_Q also forms sum(do o), which OWN_K reads.
 template <int HD, bool OWN_Q, bool CAP, bool BIAS>
-__global__ __launch_bounds__(256, BOCC) void attn_mod_bwd_kernel(const ModArgs a) {
+__global__ __launch_bounds__(256, OWN_Q && !BIAS ? 3 : 2) void attn_mod_bwd_kernel(const ModArgs a) {
     constexpr int KS = HD / 16, DJ = HD / 32, TB = TT * HD * 2;
     __shared__ __attribute__((aligned(16))) char ldsX[2][TB];
     __shared__ __attribute__((aligned(16))) char ldsY[2][TB];
@@ -898,12 +874,20 @@ struct Plan {
     long tab_q, tab_k, order_q, order_k, dsum, part, part_ml, bytes;             // byte offsets into the workspace
 };
 
-int splits_for(long blocks, long want, int tiles, int least) {  // enough workgroups for the chip, but `least` tiles for each
-    if (blocks <= 0 || blocks >= want || tiles < 2 * least) return 1;
-    long s = (want + blocks - 1) / blocks;
+// Splits of a row's tiles, so that `want` workgroups run.  Partial results are written and read in fp32, so a split keeps the more tiles the better
+// the blocks fill the chip by themselves: 4, from 128 blocks on 8, from 256 on 16.  Measured at 8 x 12 heads of 512 tokens (384 blocks of 8
+// tiles): 24 us whole, 41 in two splits; 3 x 12 heads of 538 (180 of 9): 22 and 28; causal, 8 heads of 4096 (256 of 64): 83 and 61.  Blocks of
+// one wave cost less to join and fill less: half of that, at half as many (one query, us with 2 / 4 / 8 tiles: 32 blocks of 11 tiles 12.0 /
+// 16.1 / 21.3, 96 of 24 18.3 / 15.8 / 20.5, 384 of 16 28.1 / 26.1 / 23.2); more than 32 splits only with 8 tiles each (256 tiles, 24 blocks:
+// 23.6 us in 32 splits, 27.4 in 64).
+int splits_for(long blocks, int waves, long want, int tiles) {
+    if (blocks <= 0 || blocks >= want) return 1;
+    const int half = waves == 1 ? 2 : 1, least = (blocks * half < 128 ? 4 : (blocks * half < 256 ? 8 : 16)) / half;
+    int s = (int)((want + blocks - 1) / blocks);
     if (s > tiles / least) s = tiles / least;
+    if (s > 32 && s > tiles / 8) s = tiles / 8 > 32 ? tiles / 8 : 32;
     if (s > MAX_SPLITS) s = MAX_SPLITS;
-    return (int)s;
+    return s < 1 ? 1 : s;
 }
 
 Plan plan_for(const mrg_attn_mod_desc* d, bool backward) {
@@ -914,16 +898,16 @@ Plan plan_for(const mrg_attn_mod_desc* d, bool backward) {
     const long rows_q = (long)d->B * d->H * d->Nq, rows_k = (long)d->B * d->Hk * d->Nk;
     if (!backward) {
         // up to 32 queries: workgroups of one wave, four resident per CU, and the keys cut until every CU has its four
-        p.nw = d->Nq <= 32 ? 1 : NWF;
+        p.nw = d->Nq <= 32 ? 1 : 4;
         p.nblk = (d->Nq + 32 * p.nw - 1) / (32 * p.nw);
-        p.splits = splits_for((long)d->B * d->H * p.nblk, p.nw == 1 ? WANT1 : WANTF, p.ntk, p.nw == 1 ? 4 : LEAST);
-        p.tables = d->doc_k && (p.nw == 1 ? p.ntk > 2 : p.ntk > TABMIN);
+        p.splits = splits_for((long)d->B * d->H * p.nblk, p.nw, p.nw == 1 ? 2048 : 512, p.ntk);
+        p.tables = d->doc_k && (p.nw == 1 ? p.ntk > 2 : p.ntk > 4);
         if (p.splits > 1) { p.part = take(4l * p.splits * rows_q * d->head_dim); p.part_ml = take(8l * p.splits * rows_q); }
     } else {
         p.dsum = take(4l * rows_q);
-        p.tables = d->doc_k && (p.ntk > TABMIN || p.ntq > TABMIN);
-        p.dq_splits = splits_for((long)d->B * d->H * ((d->Nq + 127) / 128), WANTQ, p.ntk, LEAST);
-        p.dkv_splits = splits_for((long)d->B * d->Hk * ((d->Nk + 127) / 128), d->causal ? WANTKC : WANTK, p.ntq * (d->H / d->Hk), LEAST);
+        p.tables = d->doc_k && (p.ntk > 4 || p.ntq > 4);
+        p.dq_splits = splits_for((long)d->B * d->H * ((d->Nq + 127) / 128), 4, 512, p.ntk);
+        p.dkv_splits = splits_for((long)d->B * d->Hk * ((d->Nk + 127) / 128), 4, d->causal ? 1024 : 512, p.ntq * (d->H / d->Hk));
         if (p.dkv_splits > p.ntq) p.dkv_splits = p.ntq ? p.ntq : 1;
         long part = 0;
         if (p.dq_splits > 1) part = 4l * p.dq_splits * rows_q * d->head_dim;
@@ -1055,8 +1039,8 @@ extern "C" int mrg_attn_mod_fwd(const mrg_attn_mod_desc* d, hipStream_t stream) 
     if (p.ordered) a.order = (const int*)((char*)d->ws + p.order_q);
     doc_tables(d, p, a, false, stream);
     const dim3 grid((unsigned)((long)a.B * a.H * a.nblk * a.splits));
-    if (d->head_dim == 64) { if (p.nw == 1) fwd_go<64, 1>(a, grid, stream); else fwd_go<64, NWF>(a, grid, stream); }
-    else { if (p.nw == 1) fwd_go<32, 1>(a, grid, stream); else fwd_go<32, NWF>(a, grid, stream); }
+    if (d->head_dim == 64) { if (p.nw == 1) fwd_go<64, 1>(a, grid, stream); else fwd_go<64, 4>(a, grid, stream); }
+    else { if (p.nw == 1) fwd_go<32, 1>(a, grid, stream); else fwd_go<32, 4>(a, grid, stream); }
     if (a.splits > 1) {
         const dim3 rows((unsigned)(((long)a.B * a.H * a.Nq + 3) / 4));
         if (d->head_dim == 64) hipLaunchKernelGGL(attn_mod_join_kernel<64>, rows, dim3(256), 0, stream, a);

@@ -324,7 +324,9 @@ ATTN = [  # B, H, Hk, Nq, Nk, hd, cap, axes, docs, causal, prefix
     (1, 1, 1, 1, 9000, 64, 0.0, 0, "packed", False, None), (1, 2, 1, 700, 700, 64, 0.0, 2, "packed", False, None), (1, 1, 1, 65, 5000, 32, 0.0, 0, "packed", True, "some"),
     (1, 2, 1, 5000, 65, 32, 8.0, 0, "packed", False, None), (2, 2, 2, 31, 64, 32, 0.0, 0, "mixed", False, None), (5, 3, 3, 257, 257, 64, 0.0, 2, None, False, None),
     # more workgroups than run at once: the row blocks are put in order
-    (8, 12, 12, 1100, 1100, 32, 0.0, 0, "packed", False, None), (9, 10, 10, 1200, 1150, 64, 0.0, 0, "mixed", True, "some"), (3, 24, 8, 1500, 1500, 32, 9.0, 0, "packed", True, None)]
+    (8, 12, 12, 1100, 1100, 32, 0.0, 0, "packed", False, None), (9, 10, 10, 1200, 1150, 64, 0.0, 0, "mixed", True, "some"), (3, 24, 8, 1500, 1500, 32, 9.0, 0, "packed", True, None),
+    # rows split although the blocks cover the chip; as many splits as there may be
+    (2, 8, 2, 2083, 2083, 32, 0.0, 1, "packed", True, "some"), (1, 1, 1, 2, 33000, 32, 0.0, 0, "packed", False, None)]
 
 
 def attn_case(case, seed=0):
