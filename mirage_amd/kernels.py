@@ -918,6 +918,8 @@ def resid_norm_bwd(dx_new: torch.Tensor, dy: Optional[torch.Tensor], x_new: torc
             g = torch.empty_like(src)
         else:
             _want(g, f"resid_norm gradient {name}", dev, _ONLY32, src.shape)
+            if any(g.data_ptr() == m.data_ptr() for m in made.values()):
+                raise ValueError(f"mirage_amd: resid_norm gradient {name} has the destination of another one")
         made[name] = g
         setattr(d, field, g.data_ptr())
     if todo:
@@ -978,6 +980,8 @@ def _attn_mod_desc(q, k, v, scale, mod: Optional[ScoreMod]):
     if mod is not None:
         d.cap, d.causal = mod.cap, mod.causal
         if mod.slopes is not None:
+            if not isinstance(mod.pos_q, torch.Tensor):
+                _refuse(mod.pos_q, "ScoreMod pos_q", dev, _ONLY32)
             axes = mod.pos_q.shape[-1] if mod.pos_q.dim() else 0
             if not 1 <= axes <= L.MRG_MAX_AXES:
                 raise ValueError(f"mirage_amd: ScoreMod positions have {axes} axes (1 to {L.MRG_MAX_AXES})")
@@ -1044,7 +1048,7 @@ def attn_mod_bwd(q, k, v, o, saved: AttnSaved, d_o, scale: float, mod: Optional[
             strides += g.stride()[:3]
         else:
             strides += _out_heads(g, what, src.shape, dev, BF16)[:3]
-            for t in (q, k, v, o, d_o, *outs):
+            for t in (q, k, v, o, saved.o_rest, d_o, *outs):
                 _need_apart(g, t, what)
         outs.append(g)
     d.o, d.o_rest, d.lse, d.d_o = o.data_ptr(), saved.o_rest.data_ptr(), saved.lse.data_ptr(), d_o.data_ptr()

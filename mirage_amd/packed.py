@@ -14,6 +14,7 @@ from typing import Optional, Sequence
 
 import torch
 import torch.nn as nn
+from torch.autograd.function import once_differentiable
 
 from . import engine as E
 from . import kernels as K
@@ -38,6 +39,40 @@ def rotary_frequencies(sections: Sequence[int], theta: float = 100.0, device=Non
 
 
 # ------------------------------------------------------------------------------------------------- differentiable operators
+def _anchor(params, device):
+    """A leaf that ties a module's Function to the graph in its parameters' place (their gradients do not travel through autograd), or None where
+    nothing is to be learnt.  Of its own for every call: a backward pass may be captured into a graph while another graph of the same
+    parameters lives, whose accumulation nodes belong to the stream of their first use."""
+    if torch.is_grad_enabled() and any(p.requires_grad for p in params):
+        return torch.empty((), device=device, requires_grad=True)
+    return None
+
+
+def _learns(*tensors) -> bool:
+    return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
+
+
+def _dense_heads(g):
+    """a gradient as the kernels read it: heads in one piece, rows and heads on 16 bytes (autograd also hands over broadcast and sliced ones)"""
+    if g is None or (g.stride(-1) == 1 and not any(s % 8 for s in g.stride()[:-1]) and g.data_ptr() % 16 == 0):
+        return g
+    return g.contiguous()
+
+
+_MOD_TENSORS = ("slopes", "pos_q", "pos_k", "doc_q", "doc_k", "prefix")
+
+
+def _mod_parts(mod: Optional[K.ScoreMod]):
+    """a ScoreMod as plain values and as tensors: these are saved like operands, so that a change between the two passes is an error"""
+    if mod is None:
+        return None, ()
+    return (mod.cap, mod.causal), tuple(getattr(mod, n) for n in _MOD_TENSORS)
+
+
+def _mod_whole(plain, tensors) -> Optional[K.ScoreMod]:
+    return None if plain is None else K.ScoreMod(plain[0], causal=plain[1], **dict(zip(_MOD_TENSORS, tensors)))
+
+
 class _RotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, pos, freqs, sections, pairing):
@@ -46,8 +81,10 @@ class _RotaryFn(torch.autograd.Function):
         return K.rotary_axes(q, k, pos, freqs, sections, pairing=pairing)
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dq, dk):
         pos, freqs = ctx.saved_tensors
+        dq, dk = _dense_heads(dq), _dense_heads(dk)
         dq, dk = K.rotary_axes(dq, dk, pos, freqs, ctx.how[0], pairing=ctx.how[1], inverse=True)
         return dq, dk, None, None, None, None
 
@@ -59,32 +96,33 @@ def rotary(q, k, pos, freqs, sections, pairing: str = "axial"):
 
 class _AttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, q, k, v, scale, mod):
-        need = any(ctx.needs_input_grad)
-        o, saved = K.attn_mod_fwd(q, k, v, scale, mod, need_lse=need)
-        if need:
-            ctx.save_for_backward(q, k, v, o, *saved)
-            ctx.how = (scale, mod)
+    def forward(ctx, q, k, v, scale, mod, learns):
+        o, saved = K.attn_mod_fwd(q, k, v, scale, mod, need_lse=learns)
+        if learns:
+            plain, tensors = _mod_parts(mod)
+            ctx.save_for_backward(q, k, v, o, *saved, *tensors)
+            ctx.how = (scale, plain)
         return o
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, d_o):
-        q, k, v, o, *saved = ctx.saved_tensors
-        if d_o.stride(-1) != 1:
-            d_o = d_o.contiguous()
-        return (*K.attn_mod_bwd(q, k, v, o, K.AttnSaved(*saved), d_o, *ctx.how), None, None)
+        q, k, v, o, lse, o_rest, *tensors = ctx.saved_tensors
+        scale, plain = ctx.how
+        grads = K.attn_mod_bwd(q, k, v, o, K.AttnSaved(lse, o_rest), _dense_heads(d_o), scale, _mod_whole(plain, tensors))
+        return (*grads, None, None, None)
 
 
 def attention(q, k, v, scale: float, mod: Optional[K.ScoreMod] = None):
     """kernels.attn_mod_fwd with its gradient: [B, Nq, H, hd] from bf16 q [B, Nq, H, hd] and k, v [B, Nk, Hk, hd]."""
-    return _AttentionFn.apply(q, k, v, scale, mod)
+    return _AttentionFn.apply(q, k, v, scale, mod, _learns(q, k, v))
 
 
 class _SeamFn(torch.autograd.Function):
     """kernels.resid_norm_fwd; the gradients of a per-sample gate are returned, those of the parameters written into their buffers."""
 
     @staticmethod
-    def forward(ctx, x, branch, gates, seam, pre, *params):
+    def forward(ctx, x, branch, gates, seam, pre, anchor):
         how = dict(gate=gates if gates is not None else seam.gate, alpha=seam.alpha, post=_wb(seam.post), pre=_wb(pre), kind=seam.kind, eps=seam.eps)
         x_new, y, stats = K.resid_norm_fwd(x, branch, **how)
         ctx.seam, ctx.pre = seam, pre
@@ -92,6 +130,7 @@ class _SeamFn(torch.autograd.Function):
         return x_new, y
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dx_new, dy):
         x_new, branch, gates, stats = ctx.saved_tensors
         seam, pre = ctx.seam, ctx.pre
@@ -101,7 +140,9 @@ class _SeamFn(torch.autograd.Function):
         dx, dbranch, grads = K.resid_norm_bwd(dx_new.contiguous(), None if pre is None else dy.contiguous(), x_new, branch, stats,
                                               gate=gates if gates is not None else seam.gate, alpha=seam.alpha, post=_wb(seam.post), pre=_wb(pre), kind=seam.kind,
                                               eps=seam.eps, grads={n: g for n, g in into.items() if g is not None})
-        return (dx, dbranch, grads["gate"] if gates is not None else None) + (None,) * (len(ctx.needs_input_grad) - 3)
+        if gates is not None and seam.gate is not None and seam.gate.grad is not None:
+            seam.gate.grad.zero_()                                # it took no part: what an earlier pass left is not this pass' gradient
+        return dx, dbranch, grads["gate"] if gates is not None else None, None, None, None
 
 
 def _wb(norm):
@@ -133,12 +174,12 @@ class Seam(nn.Module):
     def forward(self, x, branch, pre: Optional[Norm] = None, gates: Optional[torch.Tensor] = None):
         """(x', y); y is None without `pre`"""
         params = [p for m in (self, pre) if m is not None for p in m.parameters()]
-        return _SeamFn.apply(x, branch, gates, self, pre, *params)
+        return _SeamFn.apply(x, branch, gates, self, pre, _anchor(params, x.device))
 
 
 class _PackedAttentionFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y16, att, pos, mod, *params):
+    def forward(ctx, y16, att, pos, mod, need, anchor):
         B, N, _ = y16.shape
         qkv, _, _ = E.lin_fwd(y16, att.qkv)
         heads = qkv.view(B, N, att.num_heads + 2 * att.num_kv_heads, att.head_dim)
@@ -147,29 +188,30 @@ class _PackedAttentionFn(torch.autograd.Function):
         if att.sections is not None:                              # q and k are turned where the projection left them
             freqs = att.freqs(y16.device)
             K.rotary_axes(q, k, pos, freqs, att.sections, pairing=att.pairing, out_q=q, out_k=k)
-        need = any(ctx.needs_input_grad)
         o, saved = K.attn_mod_fwd(q, k, v, att.scale, mod, need_lse=need)
         branch, _, _ = E.lin_fwd(o.view(B, N, -1), att.proj)
         if need:
-            ctx.att, ctx.mod = att, mod
-            ctx.save_for_backward(y16, qkv, pos, freqs, o, *saved)
+            ctx.att = att
+            ctx.plain, tensors = _mod_parts(mod)
+            ctx.save_for_backward(y16, qkv, pos, freqs, o, *saved, *tensors)
         return branch
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dbranch):
-        y16, qkv, pos, freqs, o, *saved = ctx.saved_tensors
+        y16, qkv, pos, freqs, o, lse, o_rest, *tensors = ctx.saved_tensors
         att = ctx.att
         B, N, _ = y16.shape
         d_o, _ = E.lin_bwd(dbranch.contiguous(), o.view(B, N, -1), att.proj)
         q, k, v = att.split(qkv.view(B, N, -1, att.head_dim))
         d_qkv = torch.empty_like(qkv)
         dq, dk, dv = att.split(d_qkv.view(B, N, -1, att.head_dim))
-        K.attn_mod_bwd(q, k, v, o, K.AttnSaved(*saved), d_o.view(o.shape), att.scale, ctx.mod, dq=dq, dk=dk, dv=dv)
+        K.attn_mod_bwd(q, k, v, o, K.AttnSaved(lse, o_rest), d_o.view(o.shape), att.scale, _mod_whole(ctx.plain, tensors), dq=dq, dk=dk, dv=dv)
         if att.sections is not None:
             K.rotary_axes(dq, dk, pos, freqs, att.sections, pairing=att.pairing, inverse=True, out_q=dq, out_k=dk)
         dy, _ = E.lin_bwd(d_qkv, y16, att.qkv)
         E.join_side_stream()
-        return (dy,) + (None,) * (len(ctx.needs_input_grad) - 1)
+        return dy, None, None, None, None, None
 
 
 class PackedAttention(nn.Module):
@@ -193,6 +235,8 @@ class PackedAttention(nn.Module):
     def freqs(self, device) -> torch.Tensor:
         """the rotary table on `device` (float64 whatever type the module's parameters are cast to)"""
         if device not in self._freqs:
+            if torch.cuda.is_current_stream_capturing():
+                raise RuntimeError("mirage_amd.PackedAttention: run the module once before capturing it (its rotary table is made on the first call)")
             self._freqs[device] = rotary_frequencies(self.sections, self.theta, device)
         return self._freqs[device]
 
@@ -205,13 +249,15 @@ class PackedAttention(nn.Module):
             raise ValueError(f"mirage_amd.PackedAttention: needs contiguous bf16 [B, N, dim] (a norm's output), got {y16.dtype} {tuple(y16.shape)}")
         if (pos is None) != (self.sections is None):
             raise ValueError("mirage_amd.PackedAttention: positions go with rotary sections")
-        return _PackedAttentionFn.apply(y16, self, pos, mod, *self.parameters())
+        if y16.is_cuda and y16.device.index != torch.cuda.current_device():
+            raise ValueError(f"mirage_amd.PackedAttention: input on {y16.device}, the projections run on the current device cuda:{torch.cuda.current_device()}")
+        anchor = _anchor(self.parameters(), y16.device)
+        return _PackedAttentionFn.apply(y16, self, pos, mod, anchor is not None or _learns(y16), anchor)
 
 
 class _PackedMlpFn(torch.autograd.Function):
     @staticmethod
-    def forward(ctx, y16, mlp, *params):
-        need = any(ctx.needs_input_grad)
+    def forward(ctx, y16, mlp, need, anchor):
         act, _, pre = E.lin_fwd(y16, mlp.fc1, gelu=True, save_pre=need)
         branch, _, _ = E.lin_fwd(act, mlp.fc2)
         if need:
@@ -220,12 +266,13 @@ class _PackedMlpFn(torch.autograd.Function):
         return branch
 
     @staticmethod
+    @once_differentiable
     def backward(ctx, dbranch):
         y16, pre, act = ctx.saved_tensors
         d_pre, _ = E.lin_bwd(dbranch.contiguous(), act, ctx.mlp.fc2, gelu_pre=pre)
         dy, _ = E.lin_bwd(d_pre, y16, ctx.mlp.fc1)
         E.join_side_stream()
-        return (dy,) + (None,) * (len(ctx.needs_input_grad) - 1)
+        return dy, None, None, None
 
 
 class PackedBlock(nn.Module):
@@ -246,7 +293,8 @@ class PackedBlock(nn.Module):
         """one block from (x, norm1(x)): (x, following(x) or None).  gates: (attention's, mlp's) rows per sample, [samples, dim] each"""
         g1, g2 = gates if gates is not None else (None, None)
         x, y16 = self.seam1(x, self.attn(y16, pos, mod), self.norm2, g1)
-        return self.seam2(x, _PackedMlpFn.apply(y16, self.mlp, *self.mlp.parameters()), following, g2)
+        anchor = _anchor(self.mlp.parameters(), y16.device)
+        return self.seam2(x, _PackedMlpFn.apply(y16, self.mlp, anchor is not None or _learns(y16), anchor), following, g2)
 
 
 class PackedEncoder(nn.Module):

@@ -301,3 +301,96 @@ def test_launchers_refuse_on_the_gpu(P):
             call()
             pytest.fail(f"call {i} was not refused")
     torch.cuda.synchronize()
+
+
+def test_functions_take_any_gradient(P):
+    """autograd hands over broadcast gradients (a sum's) and slices on odd strides: the same result as their dense copies'"""
+    s = pass_state(P)
+    def grads(join):
+        q, k, v = (s["qkv"][:, :, a:b].clone().requires_grad_(True) for a, b in ((0, 4), (4, 6), (6, 8)))
+        qr, kr = P.rotary(q, k, s["pos"], s["freqs"], (8, 12, 12))
+        o = P.attention(qr, kr, v, 0.125, s["mod"])
+        join(qr, kr, o)
+        return q.grad, k.grad, v.grad
+
+    whole = [torch.ones(*s["qkv"].shape[:2], h, 64, dtype=BF16, device=dev()) for h in (4, 2, 4)]
+    dense = grads(lambda *t: torch.autograd.backward(t, whole))
+    for join in (lambda *t: sum(x.sum() for x in t).backward(), lambda *t: torch.autograd.backward(t, [torch.ones((), dtype=BF16, device=dev()).expand(x.shape) for x in t]),
+                 lambda *t: torch.autograd.backward(t, [torch.ones(*x.shape[:3], 67, dtype=BF16, device=dev())[..., 1:65] for x in t])):
+        assert all(torch.equal(a, b) for a, b in zip(grads(join), dense))
+    q = s["qkv"][:, :, :4].clone().requires_grad_(True)            # one of the two outputs goes unused, or there is only one
+    P.rotary(q, s["qkv"][:, :, 4:6], s["pos"], s["freqs"], (8, 12, 12))[0].sum().backward()
+    alone = s["qkv"][:, :, :4].clone().requires_grad_(True)
+    P.rotary(alone, None, s["pos"], s["freqs"], (8, 12, 12))[0].sum().backward()
+    assert torch.equal(q.grad, alone.grad)
+
+
+def test_what_the_backward_pass_needs_is_watched(P):
+    """masks changed between the passes, and a gradient of the gradient, are errors"""
+    s = pass_state(P)
+    q = s["qkv"][:, :, :4].clone().requires_grad_(True)
+    o = P.attention(q, s["qkv"][:, :, 4:6], s["qkv"][:, :, 6:], 0.125, s["mod"])
+    s["mod"].doc_q[0, 0] = 5
+    with pytest.raises(RuntimeError, match="modified by an inplace operation"):
+        o.sum().backward()
+    qr, _ = P.rotary(q, None, s["pos"], s["freqs"], (8, 12, 12))
+    (g,) = torch.autograd.grad(qr, q, torch.ones_like(qr).requires_grad_(True), create_graph=True)
+    with pytest.raises(RuntimeError, match="once_differentiable"):
+        g.sum().backward()
+
+
+def test_learnt_gate_gets_no_stale_gradient(P):
+    """a pass with gates per sample does not use the learnt one: its gradient is zero, not the one of the pass before"""
+    enc = fill(P.PackedEncoder(128, 1, 2).to(dev()))
+    x, gates = rnd(2, 20, 128, seed=1), [tuple(0.5 * rnd(2, 128, seed=i) for i in (2, 3))]
+    enc(x)[0].sum().backward()
+    assert float(enc.blocks[0].seam1.gate.grad.abs().max()) > 0 and float(enc.blocks[0].seam2.gate.grad.abs().max()) > 0
+    enc(x, gates=gates)[0].sum().backward()
+    assert float(enc.blocks[0].seam1.gate.grad.abs().max()) == 0 and float(enc.blocks[0].seam2.gate.grad.abs().max()) == 0
+
+
+def test_captured_training_pass_beside_a_living_graph(P):
+    """forward and backward of the modules captured while an eager pass of the same parameters waits for its backward: replays equal the eager passes"""
+    from mirage_amd import kernels as K
+    enc = fill(P.PackedEncoder(128, 2, 2, sections=(8, 12, 12), norm="rms").to(dev()))
+    pos, doc, _, _ = volume(P)
+    mod = K.ScoreMod(cap=20.0, doc_q=doc, doc_k=doc)
+    x, dx, dy = rnd(2, doc.shape[1], 128, seed=1), rnd(2, doc.shape[1], 128, seed=2), rnd(2, doc.shape[1], 128, dtype=BF16, seed=3)
+
+    def go():
+        h, y = enc(x, pos, mod)
+        torch.autograd.backward([h, y], [dx, dy])
+        return [h.detach(), y.detach()] + [p.grad for p in enc.parameters()]
+
+    go()
+    waiting = enc(x, pos, mod)
+    torch.cuda.synchronize()
+    g = torch.cuda.CUDAGraph()
+    with torch.cuda.graph(g):
+        out = go()
+    for turn in range(3):
+        x.copy_(rnd(*x.shape, seed=10 + turn))
+        want = [t.clone() for t in go()]
+        torch.cuda.synchronize()
+        for p in enc.parameters():
+            p.grad.fill_(float("nan"))
+        g.replay()
+        torch.cuda.synchronize()
+        assert all(torch.equal(a, b) for a, b in zip(out, want))
+    assert len(waiting) == 2
+
+
+def test_modules_refuse_another_device(P, monkeypatch):
+    att = P.PackedAttention(128, 2).to(dev())
+    y = torch.zeros(1, 4, 128, dtype=BF16, device=dev())
+    monkeypatch.setattr(torch.cuda, "current_device", lambda: 1)
+    with pytest.raises(ValueError, match="current device"):
+        att(y)
+
+
+def test_resid_norm_refuses_one_destination_for_two(P):
+    from mirage_amd import kernels as K
+    x, w, g = torch.zeros(2, 3, 64, device=dev()), torch.ones(64, device=dev()), torch.zeros(64, device=dev())
+    x_new, y, stats = K.resid_norm_fwd(x, x, post=(w, None), pre=(w, None))
+    with pytest.raises(ValueError, match="destination"):
+        K.resid_norm_bwd(x, y, x_new, x, stats, post=(w, None), pre=(w, None), grads={"post_weight": g, "pre_weight": g})
