@@ -10,7 +10,9 @@
 //     dgate = w_post A + b_post T      dw_post = sum over gates of g A      db_post = sum over gates of g T
 // so a workgroup carries four sums per column instead of five, whatever the gate's shape.
 //
-// Bound: HBM.  Forward reads 4 + 2 and writes 4 + 2 bytes an element (fp32 residual, bf16 branch and y), backward reads 12 and writes 6.
+// Bound: HBM.  Forward reads 4 + 2 and writes 4 + 2 bytes an element (fp32 residual, bf16 branch and y), backward reads 12 and writes 6: 65792
+// rows of 1024 with a gate per sample take 182 us (4.4 TB/s) and 258 us (4.7 TB/s, the adding of the partial sums with it), where a plain copy of
+// 2 GiB ran at 4.9.
 // A row is read once into registers (forward: a wave per row up to 1024 columns, four waves beyond; backward, which carries the column sums
 // and a requested row as well: one wave per 256 columns), all statistics in fp32: the mean first, then the
 // squares of the differences, from registers.  Column sums stay in registers over a workgroup's rows, meet in LDS, and leave as one
@@ -263,15 +265,22 @@ __global__ __launch_bounds__(256) void resid_norm_sum_kernel(const SumArgs a, in
     if (rl == 0 && c * 4 < a.D) reinterpret_cast<float4*>(job.dst)[c] = box[0][cl];
 }
 
-// units of the backward launch: the rows that share a gate, cut into `parts` so that about two workgroups per CU have work, but no part
-// below 16 rows (four per wave) where a gate has that many
-constexpr int RN_GRID = 1024;
-int rn_parts(int samples, int L) {
-    int parts = (RN_GRID + samples - 1) / samples;
-    const int most = (L + 15) / 16;
+// waves of a backward row, and of a workgroup (four rows side by side where one wave holds a row)
+int rn_waves(int D) { return D <= 256 ? 1 : (D <= 512 ? 2 : (D <= 768 ? 3 : (D <= 1024 ? 4 : (D <= 2048 ? 8 : 16)))); }
+// The backward launch: 12 of the 16 waves per CU that its registers allow, but a workgroup for every CU.  More of them leave more partial sums (65792 x
+// 1024, forward and backward: 455 us with 16 waves, 440 with 12; 8200 x 4096, backward: 203 us with four workgroups per CU, 147 with one), fewer
+// keep too little in flight (16448 x 512: 34 us with 12, 39 with 8, 44 with 4).
+// Units: the rows that share a gate, cut into parts until every workgroup has one, but no part below 16 rows (four per wave) where a gate has that
+// many; more units than workgroups fit at once are dealt evenly.
+int rn_groups(int D, int waves_per_cu) { const int w = rn_waves(D), n = waves_per_cu / (w == 1 ? 4 : w); return 256 * (n < 1 ? 1 : n); }
+int rn_parts(int samples, int L, int D) {
+    const int parts = (rn_groups(D, 12) + samples - 1) / samples, most = (L + 15) / 16;
     return parts < 1 ? 1 : (parts > most ? (most < 1 ? 1 : most) : parts);
 }
-int rn_grid(long units) { return (int)(units < RN_GRID ? units : RN_GRID); }
+int rn_grid(long units, int D) {
+    const long fit = rn_groups(D, 16), each = (units + fit - 1) / fit;
+    return (int)((units + each - 1) / each);
+}
 
 template <int WPR, bool B32, bool PRE, bool DY32>
 void rn_bwd(const ResidArgs& a, bool sample, int grid, hipStream_t st) {
@@ -319,7 +328,7 @@ void rn_scope(const mrg_resid_norm_desc* d, int& scopes, int& rows, int& parts) 
     const bool sample = d->gate_rows > 1;
     scopes = sample ? d->samples : 1;
     rows = sample ? d->rows_per_sample : d->samples * d->rows_per_sample;
-    parts = rn_parts(scopes, rows);
+    parts = rn_parts(scopes, rows, d->D);
 }
 
 }  // namespace
@@ -346,7 +355,7 @@ extern "C" long mrg_resid_norm_ws_floats(const mrg_resid_norm_desc* d) {
     int scopes, rows, parts;
     rn_scope(d, scopes, rows, parts);
     const long units = (long)scopes * parts;
-    return ((long)rn_grid(units) * 4 + units) * d->D;
+    return units ? ((long)rn_grid(units, d->D) * 4 + units) * d->D : 0;
 }
 
 extern "C" int mrg_resid_norm_bwd(const mrg_resid_norm_desc* d, hipStream_t stream) {
@@ -363,16 +372,18 @@ extern "C" int mrg_resid_norm_bwd(const mrg_resid_norm_desc* d, hipStream_t stre
     int scopes, rows, parts;
     rn_scope(d, scopes, rows, parts);
     a.L = rows; a.parts = parts; a.units = a.M ? scopes * parts : 0;
-    const int grid = a.M ? rn_grid(a.units) : 0;
+    const int grid = a.M ? rn_grid(a.units, d->D) : 0;
     const bool gated = d->gate_rows > 0;
     a.part = d->ws; a.gpart = gated ? d->ws + (long)grid * 4 * d->D : nullptr;
     if (a.M) {
-        if (d->D <= 256) rn_bwd<1>(a, sample, grid, stream);
-        else if (d->D <= 512) rn_bwd<2>(a, sample, grid, stream);
-        else if (d->D <= 768) rn_bwd<3>(a, sample, grid, stream);
-        else if (d->D <= 1024) rn_bwd<4>(a, sample, grid, stream);
-        else if (d->D <= 2048) rn_bwd<8>(a, sample, grid, stream);
-        else rn_bwd<16>(a, sample, grid, stream);
+        switch (rn_waves(d->D)) {
+            case 1: rn_bwd<1>(a, sample, grid, stream); break;
+            case 2: rn_bwd<2>(a, sample, grid, stream); break;
+            case 3: rn_bwd<3>(a, sample, grid, stream); break;
+            case 4: rn_bwd<4>(a, sample, grid, stream); break;
+            case 8: rn_bwd<8>(a, sample, grid, stream); break;
+            default: rn_bwd<16>(a, sample, grid, stream);
+        }
     }
     // the partial rows' sums (no rows at all: every gradient is zero)
     SumArgs s = {};

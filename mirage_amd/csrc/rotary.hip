@@ -7,15 +7,16 @@
 // a (row, pair) are computed once per workgroup into LDS and shared by all its heads: at 12 - 16 heads the 64-bit arithmetic fits into the
 // issue slots that the copy of the row leaves free.
 //
-// Bound: HBM, one read and one write of q and k.  A workgroup owns `rows` whole rows of q or of k (blockIdx.y), walks their (head, 8 pairs)
-// units with 16-byte loads of both members of the pairs (bf16; 4 pairs in fp32) and keeps ROT_UNITS units in flight per lane before it
-// stores the first.
+// Bound: HBM, one read and one write of q and k: 8 x 4097 rows of 16 + 16 heads of 64 in bf16 take 50 us a turn, 5.3 TB/s (a plain copy of 2 GiB ran at
+// 4.9); a single image (257 rows of 12 + 12 heads) 3.1 us, which is a launch.  A workgroup owns `rows` whole rows of q or of k (blockIdx.y), walks
+// their (head, 8 pairs) units with 16-byte loads of both members of the pairs (bf16; 4 pairs in fp32) and keeps ROT_UNITS units in flight per
+// lane before it stores the first.
 #include "common.h"
 #include "mirage_hip.h"
 
 namespace {
 
-constexpr int ROT_UNITS = 4;       // units in flight per lane
+constexpr int ROT_UNITS = 2;       // units in flight per lane (4 the same on long rows, 5 % slower on small ones: their registers cost waves)
 constexpr int ROT_MAX_HD = 256;
 
 struct RotSide { const char* in; char* out; long bs, rs, hs, obs, ors, ohs; int H; };
@@ -174,10 +175,12 @@ extern "C" int mrg_rotary_axes(const mrg_rotary_desc* d, hipStream_t stream) {
     bool copy = false;                                        // elements behind the pairs are copied unless both sides work in place
     for (int i = 0; i < sides; ++i) copy |= a.s[i].in != a.s[i].out;
     a.tail = copy ? (d->head_dim - 2 * P) / vec : 0;
-    // rows of a workgroup: enough workgroups for every CU first (one row each: a single image is a latency matter), then as many rows as
-    // keep ROT_UNITS units per lane busy.  At 32776 rows x 32 heads of 64 (bf16): 8 rows; one row each costs the whole prologue per row
+    // rows of a workgroup: enough workgroups for every CU first (one row each: a single image is a latency matter), then rows until every lane has a
+    // unit.  Forward and back at 32776 rows x 32 heads of 64 (64 units a row): 161 us with one row, 101 with 4, 105 with 8, 108 with 16;
+    // 16512 rows x 12 heads (24 units): 15 us with 4 rows, 12 with 8 and with 16
     int rows = 1;
-    while (rows < 8 && a.rows_total / rows > 2048) rows <<= 1;
+    const int row_units = (a.s[0].H > a.s[sides - 1].H ? a.s[0].H : a.s[sides - 1].H) * (a.units + a.tail);
+    while (rows < 16 && rows * row_units < 256 && a.rows_total / rows > 2048) rows <<= 1;
     a.rows = rows;
     const dim3 grid((a.rows_total + rows - 1) / rows, sides);
     const size_t lds = sizeof(float2) * rows * P;
