@@ -11,12 +11,24 @@
 // order.  Scores never leave the registers.  Tiles of 64 keys go global -> LDS by DMA one tile ahead of the products, double-buffered, one
 // barrier per tile.
 //
-// Masks by tiles.  A first small launch leaves the smallest and largest document and the count of valid tokens of every 64-token tile; a
+// Masks by tiles.  With documents, a small launch leaves the smallest and largest document and the count of valid tokens of every 64-token tile; a
 // workgroup tests 64 tiles at a time (one per lane, one ballot) and walks only tiles that some row of it may see.  Per wave a tile is skipped,
-// whole (no test per score) or partial.  Sums, maxima, lse and all products accumulate in fp32.  p is rounded to bf16 as an operand of the
-// second product (at most 2^-8 of each weight, averaging over the row; its sum is taken before the rounding).  ds goes into its product as
-// two bf16 parts, and sum(do o) takes o with what its rounding left out: with either rounded once, dq and dk were 0.0028 from the 64-bit
-// gradient, where 0.0017 is the rounding of the result itself.
+// whole (no test per score) or partial; in a partial one a lane holds what it sees as one bit per row of the tile.  Rows of up to 256 tokens are
+// walked without tables (forward, 32 x 8 heads, one document a row: 128 tokens 9.9 us without and 12.4 with, 256 15.8 and 17.7, 512 43.9 and
+// 43.7, there with several documents 69 and 55).  The row blocks of packed rows differ in length; where there are more of them than run at once,
+// the launch also puts them in order, the longest first (backward of 8 x 12 heads of 1024 in five documents 140 -> 110 us, one row of 8192 in
+// twelve documents, 16 heads 240 -> 200).
+//
+// Sums, maxima, lse and all products accumulate in fp32.  p is rounded to bf16 as an operand of the second product (at most 2^-8 of each weight,
+// averaging over the row; its sum is taken before the rounding).  ds goes into its product as two bf16 parts, and sum(do o) takes o with what its
+// rounding left out: dq and dk are then 0.0017 to 0.0024 from the 64-bit gradient, where 0.0017 is the rounding of the result itself.  In one part
+// they were 0.0024 to 0.0031 away (the terms of a sum that nearly cancel are rounded apart) for 8 to 18 % less time of the backward pass.
+//
+// What bounds it: the arithmetic between the products.  At 16 heads of 4095 tokens behind a prefix a score costs 7 vector operations forward, 10 for
+// dq, 11 for dk and dv; the vector pipe is busy 66 % and the matrix pipe 32 % of the forward pass (98 us, 700 TFLOP/s), 61 / 44 % for dq and
+// 44 / 38 % for dk and dv (370 us together with their joining, 830 TFLOP/s counting the products that are made).  A distance of two axes takes
+// the forward pass to 16 operations, padded rows counted (64 x 12 heads of 257 tokens, 60 us: 57 / 13 %).  One query of many keys is bound by
+// HBM: 16 x 12 heads of 4097 keys in 45.6 us, 4.4 TB/s.
 //
 // Values that are not finite behind a mask: 0 * inf would reach the products, so in partial tiles the rows of the second product's left
 // operand that hold such values are replaced by zeros in LDS and noted; a row that SEES one of them is NaN in full.
@@ -351,7 +363,9 @@ __device__ __forceinline__ void store_o(const ModArgs& a, long at, const float4 
 
 // ================================================ forward ===============================================
 // NW waves of 32 queries.  NW = 1 serves up to 32 queries (a pooled or a single new token): every workgroup is one wave, and the keys are
-// split over many of them.
+// split over many of them.  NW = 4 otherwise: two waves would stage every tile for half as many queries (83 -> 102 us on 16 heads of 8192 packed
+// tokens).  Three waves per SIMD (98 us in three, 99 in two, 105 in four for 16 heads
+// of 4095 tokens behind a prefix); with a distance bias the registers are those of two (64 x 12 heads of 257 tokens 61 us, 63 when held to three).
 template <int HD, int NW, bool CAP, bool BIAS>
 __global__ __launch_bounds__(64 * NW, BIAS ? 2 : 3) void attn_mod_fwd_kernel(const ModArgs a) {
     constexpr int KS = HD / 16, DJ = HD / 32, NT = 64 * NW, TB = TT * HD * 2;
@@ -594,8 +608,12 @@ __global__ __launch_bounds__(256) void attn_mod_join_kernel(const ModArgs a) {
 
 // ================================================ backward ==============================================
 // The two owner kernels share the walk, the staging and the arithmetic of a 32 x 32 block:
-//   OWN_Q: lane = query, tiles of keys:  S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T          (7 of the 10 hd flop a pair twice: 14 hd in all)
-//   OWN_K: lane = key, tiles of queries: S = Q K^T,  dP = dO V^T,  dV^T += dO^T P, dK^T += Q^T dS
+//   OWN_Q: lane = query, tiles of keys:  S^T = K Q^T, dP^T = V dO^T, dQ^T += K^T dS^T          (8 hd flop a pair, ds in two parts)
+//   OWN_K: lane = key, tiles of queries: S = Q K^T,  dP = dO V^T,  dV^T += dO^T P, dK^T += Q^T dS         (10 hd)
+// Scores and dP are formed twice (4 hd of the 18), which costs less than the atomics or the traffic of dq partials that one kernel would need: a
+// tile of 64 keys would add 64 KiB of fp32 to HBM for every 128 queries.  Four waves of 32 rows; dq runs at three waves per SIMD
+// (375 us the pass above in two), dk / dv and a distance bias at two: in three they spill (370 -> 512 us; 16 heads of 8192 packed tokens with a
+// distance 200 -> 299).
 // X, Y: the staged matrices (K, V or Q, dO); own fragments: (Q, dO) or (K, V).  OWN_Q also forms sum(do o), which OWN_K reads.
 template <int HD, bool OWN_Q, bool CAP, bool BIAS>
 __global__ __launch_bounds__(256, OWN_Q && !BIAS ? 3 : 2) void attn_mod_bwd_kernel(const ModArgs a) {
