@@ -71,7 +71,8 @@ def rotary_bound(ref, size, dtype):
 
 ROTARY = [  # B, N, H, Hk, hd, sections
     (1, 1, 1, 1, 32, (16,)), (2, 257, 12, 12, 64, (16, 16)), (3, 65, 4, 2, 64, (8, 12, 12)), (2, 33, 3, 1, 48, (5, 7, 3)), (1, 300, 2, 2, 64, (4, 6, 6)),
-    (2, 19, 2, 1, 6, (1, 1)), (1, 2100, 2, 1, 128, (16, 24, 24)), (1, 5, 1, 1, 2, (1,)), (2, 40, 4, 4, 32, (4, 6, 6)), (1, 7, 2, 3, 256, (64, 64))]
+    (2, 19, 2, 1, 6, (1, 1)), (1, 2100, 2, 1, 128, (16, 24, 24)), (1, 5, 1, 1, 2, (1,)), (2, 40, 4, 4, 32, (4, 6, 6)), (1, 7, 2, 3, 256, (64, 64)),
+    (3, 13337, 2, 1, 16, (3, 2))]                                  # 16 rows a workgroup, the last one short
 
 
 @pytest.mark.parametrize("pairing", ["half", "interleaved", "axial"])
@@ -173,7 +174,10 @@ NORM = [  # shape, kind, gate, post bias, pre bias (None: no norm), alpha, branc
     ((1, 70, 1028), "layer", "channel", True, False, 1.0, BF16), ((3, 9, 2052), "rms", "sample", True, True, 1.0, F32),
     ((2, 11, 4096), "layer", "sample", True, True, 0.3, BF16), ((700, 1, 128), "layer", "sample", True, True, 1.0, BF16),
     ((2, 3, 40, 192), "rms", "channel", True, True, 1.0, BF16), ((6, 516), "layer", "sample", False, False, 1.0, F32),
-    ((1, 2500, 132), "layer", "none", True, True, 1.0, BF16)]
+    ((1, 2500, 132), "layer", "none", True, True, 1.0, BF16),
+    # more gates than workgroups run at once; parts of a gate's rows that do not divide
+    ((2500, 3, 64), "layer", "sample", True, True, 1.0, BF16), ((700, 2, 2052), "rms", "sample", False, False, 1.0, BF16), ((300, 1, 4096), "layer", "sample", True, True, 0.9, F32),
+    ((33, 517, 768), "layer", "sample", True, True, 1.0, BF16)]
 
 
 @pytest.mark.parametrize("shape,kind,gate,post,pre,alpha,branch", NORM)
