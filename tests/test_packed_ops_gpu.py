@@ -330,7 +330,9 @@ ATTN = [  # B, H, Hk, Nq, Nk, hd, cap, axes, docs, causal, prefix
     # more workgroups than run at once: the row blocks are put in order
     (8, 12, 12, 1100, 1100, 32, 0.0, 0, "packed", False, None), (9, 10, 10, 1200, 1150, 64, 0.0, 0, "mixed", True, "some"), (3, 24, 8, 1500, 1500, 32, 9.0, 0, "packed", True, None),
     # rows split although the blocks cover the chip; as many splits as there may be
-    (2, 8, 2, 2083, 2083, 32, 0.0, 1, "packed", True, "some"), (1, 1, 1, 2, 33000, 32, 0.0, 0, "packed", False, None)]
+    (2, 8, 2, 2083, 2083, 32, 0.0, 1, "packed", True, "some"), (1, 1, 1, 2, 33000, 32, 0.0, 0, "packed", False, None),
+    # key blocks in order and split as well
+    (4, 16, 8, 2083, 2083, 32, 0.0, 0, "packed", True, "some")]
 
 
 def attn_case(case, seed=0):
@@ -451,3 +453,27 @@ def test_attn_mod_gradient_by_differences(K):
         want = (ends[0] - ends[1]) / (2 * h)
         bound = float((ref[("dq", "dk", "dv")[n]][1] * step.abs()).sum()) + 1e-5
         assert abs(float((got.double() * step).sum()) - want) <= bound
+
+
+def test_rows_beyond_32_bits(K):
+    """q, k and v as columns of rows that lie 2^22 elements apart (the last one behind 2^32): the same bits as from dense copies, gradients in place too"""
+    N, rs = 1100, 1 << 22
+    far = torch.empty((N - 1) * rs + 512, dtype=BF16, device=dev())
+    rows = torch.as_strided(far, (1, N, 8, 64), (N * rs, rs, 64, 1))
+    rows.copy_(rnd(1, N, 8, 64, dtype=BF16, seed=1))
+    doc = documents(1, N, "packed", 3)
+    mod = K.ScoreMod(cap=20.0, doc_q=doc, doc_k=doc)
+    pos, freqs = torch.arange(N, device=dev(), dtype=torch.int32)[:, None].contiguous(), torch.linspace(1, 0.01, 32, dtype=torch.float64, device=dev())
+    d_o = rnd(1, N, 4, 64, dtype=BF16, seed=2)
+
+    def go(t, grads):
+        q, k, v = t[:, :, :4], t[:, :, 4:6], t[:, :, 6:]
+        K.rotary_axes(q, k, pos, freqs, (32,), out_q=q, out_k=k)
+        o, saved = K.attn_mod_fwd(q, k, v, 0.125, mod)
+        one, _ = K.attn_mod_fwd(q[:, -1:], k, v, 0.125, K.ScoreMod(causal=True), need_lse=False)
+        outs = [None] * 3 if grads is None else [grads[:, :, :4], grads[:, :, 4:6], grads[:, :, 6:]]
+        return [o, one, saved.lse, *K.attn_mod_bwd(q, k, v, o, saved, d_o, 0.125, mod, *outs)]
+
+    dense = go(rows.contiguous(), None)
+    into = torch.as_strided(torch.empty_like(far), (1, N, 8, 64), (N * rs, rs, 64, 1))
+    assert all(torch.equal(a, b) for a, b in zip(go(rows, into), dense))
