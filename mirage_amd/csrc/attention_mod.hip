@@ -212,9 +212,10 @@ __global__ __launch_bounds__(256) void doc_tiles_kernel(const int* __restrict__ 
 }
 
 // Work of a launch: `heads` (batch, head) pairs of `per` row blocks each.  Workgroups are dispatched round-robin over the 8 dies; a die gets whole
-// heads (where they divide by 8), so that a head's keys stay in its own L2.  Under an order the blocks differ in length, `longest` first: then
-// all heads' longest blocks start first and the short ones fill the end (one head after the other left a quarter of the chip idle behind the
-// last head's long blocks); otherwise a head's blocks follow each other.
+// heads (where they divide by 8), so that a head's keys stay in its own L2.  Where blocks differ in length -- under an order, the longest first, and
+// with documents -- all heads' first blocks start first and the short ones fill the end, and a CU's workgroups are not all of one length (one
+// head after the other left a quarter of the chip idle behind the last head's long blocks; 4 x 12 heads of 1024 tokens in five documents 32 ->
+// 28 us); otherwise, and where rows are split, a head's blocks follow each other.
 __device__ __forceinline__ void place(int id, int heads, int per, bool by_length, int& head, int& blk) {
     const int dies = heads % 8 == 0 ? 8 : 1, mine = heads / dies;
     const int die = id % dies, idx = id / dies;
@@ -341,6 +342,8 @@ __device__ __forceinline__ unsigned long long seen_rows(int left, bool bydoc, in
     }
     return m;
 }
+// does no lane of the wave see any of the 32 rows of half kb (a document that ends in the other half, keys behind the last visible one)
+__device__ __forceinline__ bool none_seen(unsigned long long seen, int kb) { return __builtin_amdgcn_ballot_w64((unsigned)(seen >> (kb * 32)) != 0) == 0; }
 // accumulator register r of a lane stands for row 8 (r >> 2) + (r & 3) of its block behind the lane's first one; rows that are not seen take `value`
 __device__ __forceinline__ void hide(f32x16& x, unsigned long long seen, int kb, int lane, float value) {
     const int bits = (int)((unsigned)(seen >> (kb * 32)) >> (4 * (lane >> 5)));
@@ -375,7 +378,7 @@ __global__ __launch_bounds__(64 * NW, BIAS ? 2 : 3) void attn_mod_fwd_kernel(con
     __shared__ unsigned long long noted[3];                      // of tile n: slot n % 3
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int bh, blk;
-    place(blockIdx.x, a.B * a.H, a.nblk * a.splits, a.causal || a.order, bh, blk);
+    place(blockIdx.x, a.B * a.H, a.nblk * a.splits, a.causal || (a.tab_k && a.splits == 1), bh, blk);
     const int split = blk % a.splits, b = bh / a.H, h = bh - b * a.H, hk = h / a.G;
     blk /= a.splits;
     if (a.order) blk = a.order[(long)b * a.nblk + blk];
@@ -500,7 +503,7 @@ __global__ __launch_bounds__(64 * NW, BIAS ? 2 : 3) void attn_mod_fwd_kernel(con
             const uint32_t kt = lds_addr(ldsK[buf]), vt = lds_addr(ldsV[buf]);
 #pragma unroll
             for (int kb = 0; kb < 2; ++kb) {
-                if (j0 + kb * 32 >= wlim_hi) break;
+                if (!whole && none_seen(seen, kb)) continue;
                 f32x16 s = zero16();
 #pragma unroll
                 for (int kk = 0; kk < KS; ++kk) s = __builtin_amdgcn_mfma_f32_32x32x16_bf16(fk.read(kt, kb * 32, kk), qf[kk], s, 0, 0, 0);
@@ -626,7 +629,7 @@ __global__ __launch_bounds__(256, OWN_Q && !BIAS ? 3 : 2) void attn_mod_bwd_kern
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int OH = OWN_Q ? a.H : a.Hk;                                               // the owner's head: a query head or a key head
     int bo, blk;
-    place(blockIdx.x, a.B * OH, a.nblk * a.splits, a.causal || a.order, bo, blk);
+    place(blockIdx.x, a.B * OH, a.nblk * a.splits, a.causal || (a.tab_k && a.splits == 1), bo, blk);
     const int split = blk % a.splits, b = bo / OH, ho = bo - b * OH;
     blk /= a.splits;
     if (a.order) blk = a.order[(long)b * a.nblk + blk];
@@ -934,10 +937,11 @@ Plan plan_for(const mrg_attn_mod_desc* d, bool backward) {
     }
     if (p.tables) {
         p.tab_q = take(16l * d->B * p.ntq); p.tab_k = take(16l * d->B * p.ntk);
-        // more workgroups than run at once (three or two per CU), and tables that one workgroup per batch row makes in a few microseconds
+        // more than two workgroups per CU, and tables that one workgroup per batch row makes in a few microseconds (2 - 3 us more than the tables
+        // alone: 8 x 12 heads of 1024 tokens, 768 blocks, 49 -> 42 us forward; 6 x 12 heads of 538, 360 blocks, 27 -> 29)
         const int rows = backward ? 128 : 32 * p.nw;
         const long blocks = (long)d->B * (backward ? (d->Hk < d->H ? d->Hk : d->H) : d->H) * ((d->Nq + rows - 1) / rows);
-        p.ordered = blocks > (backward ? 512 : 768) && p.ntq <= ORDER_TILES && p.ntk <= ORDER_TILES && p.ntq > 0 && p.ntk > 0 && p.nw != 1;
+        p.ordered = blocks > 512 && p.ntq <= ORDER_TILES && p.ntk <= ORDER_TILES && p.ntq > 0 && p.ntk > 0 && p.nw != 1;
         if (p.ordered) { p.order_q = take(4l * d->B * ((d->Nq + rows - 1) / rows)); p.order_k = take(backward ? 4l * d->B * ((d->Nk + rows - 1) / rows) : 0); }
     }
     p.bytes = at;
