@@ -56,7 +56,7 @@ struct ModArgs {
     long dq_bs, dq_rs, dq_hs, dk_bs, dk_rs, dk_hs, dv_bs, dv_rs, dv_hs;
     float* dsum;                              // [B, H, Nq] sum(do o)
     float* part; float* part_ml; int splits;  // split rows: [split][rows][HD] unnormalised, [split][rows][2] {max, sum}
-    int nblk;                                 // row blocks of the owner
+    int nblk, abreast;                        // row blocks of the owner; do the heads' blocks start side by side
     const int* order;                         // [B][nblk]: the row blocks, longest first (null: causal order tells, or they are alike)
 };
 
@@ -212,14 +212,12 @@ __global__ __launch_bounds__(256) void doc_tiles_kernel(const int* __restrict__ 
 }
 
 // Work of a launch: `heads` (batch, head) pairs of `per` row blocks each.  Workgroups are dispatched round-robin over the 8 dies; a die gets whole
-// heads (where they divide by 8), so that a head's keys stay in its own L2.  Where blocks differ in length -- under an order, the longest first, and
-// with documents -- all heads' first blocks start first and the short ones fill the end, and a CU's workgroups are not all of one length (one
-// head after the other left a quarter of the chip idle behind the last head's long blocks; 4 x 12 heads of 1024 tokens in five documents 32 ->
-// 28 us); otherwise, and where rows are split, a head's blocks follow each other.
-__device__ __forceinline__ void place(int id, int heads, int per, bool by_length, int& head, int& blk) {
+// heads (where they divide by 8), so that a head's keys stay in its own L2.  abreast: all heads' first blocks start first; otherwise a head's blocks
+// follow each other.
+__device__ __forceinline__ void place(int id, int heads, int per, int abreast, int& head, int& blk) {
     const int dies = heads % 8 == 0 ? 8 : 1, mine = heads / dies;
     const int die = id % dies, idx = id / dies;
-    if (by_length) { head = die * mine + idx % mine; blk = idx / mine; }
+    if (abreast) { head = die * mine + idx % mine; blk = idx / mine; }
     else { head = die * mine + idx / per; blk = idx % per; }
 }
 
@@ -378,7 +376,7 @@ __global__ __launch_bounds__(64 * NW, BIAS ? 2 : 3) void attn_mod_fwd_kernel(con
     __shared__ unsigned long long noted[3];                      // of tile n: slot n % 3
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     int bh, blk;
-    place(blockIdx.x, a.B * a.H, a.nblk * a.splits, a.causal || (a.tab_k && a.splits == 1), bh, blk);
+    place(blockIdx.x, a.B * a.H, a.nblk * a.splits, a.abreast, bh, blk);
     const int split = blk % a.splits, b = bh / a.H, h = bh - b * a.H, hk = h / a.G;
     blk /= a.splits;
     if (a.order) blk = a.order[(long)b * a.nblk + blk];
@@ -629,7 +627,7 @@ __global__ __launch_bounds__(256, OWN_Q && !BIAS ? 3 : 2) void attn_mod_bwd_kern
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int OH = OWN_Q ? a.H : a.Hk;                                               // the owner's head: a query head or a key head
     int bo, blk;
-    place(blockIdx.x, a.B * OH, a.nblk * a.splits, a.causal || (a.tab_k && a.splits == 1), bo, blk);
+    place(blockIdx.x, a.B * OH, a.nblk * a.splits, a.abreast, bo, blk);
     const int split = blk % a.splits, b = bo / OH, ho = bo - b * OH;
     blk /= a.splits;
     if (a.order) blk = a.order[(long)b * a.nblk + blk];
@@ -1004,6 +1002,18 @@ void doc_tables(const mrg_attn_mod_desc* d, const Plan& p, ModArgs& a, bool back
     if (tiles) hipLaunchKernelGGL(doc_tiles_kernel, dim3((tiles + 3) / 4), dim3(256), 0, st, d->doc_q, d->doc_k, (int4*)a.tab_q, (int4*)a.tab_k, d->B, d->Nq, d->Nk, ntq, p.ntk);
 }
 
+// Do the heads' blocks start side by side?  Where blocks differ in length the short ones then fill the end, and a CU's workgroups are not all of one
+// length: under an order of the keys or of the blocks and with documents (one head after the other left a quarter of the chip idle behind the last
+// head's long blocks; 4 x 12 heads of 1024 tokens in five documents 32 -> 28 us, 32 x 12 of them 113 -> 105), and where the last block holds one
+// wave's rows or fewer, while what a die's heads read stays in its 4 MB of L2 (64 x 12 heads of 129 tokens 29 -> 26 us; 16 x 12 of 1025, 6 MB
+// for a die, 93 -> 96).  Split rows stay together.
+bool start_abreast(const ModArgs& a, int rows, int heads, long head_bytes) {
+    if (a.causal) return true;
+    if (a.splits > 1) return false;
+    const int tail = rows % 128;
+    return a.tab_k != nullptr || (tail > 0 && tail <= 32 && (heads + 7) / 8 * head_bytes <= (4l << 20));
+}
+
 template <int HD, int NW>
 void fwd_go(const ModArgs& a, dim3 grid, hipStream_t st) {
     const bool bias = a.slopes != nullptr;
@@ -1032,6 +1042,7 @@ void bwd_side(ModArgs a, int splits, int HD, hipStream_t st) {
     if (NO == 0) return;
     a.splits = splits;
     a.nblk = (NO + 127) / 128;
+    a.abreast = start_abreast(a, NO, a.B * a.Hk, 4l * HD * (OWN_Q ? a.Nk : a.Nq * (long)a.G));
     const dim3 grid((unsigned)((long)a.B * OH * a.nblk * splits));
     if (HD == 64) bwd_go<64, OWN_Q>(a, grid, st); else bwd_go<32, OWN_Q>(a, grid, st);
     if (splits > 1) {
@@ -1059,6 +1070,7 @@ extern "C" int mrg_attn_mod_fwd(const mrg_attn_mod_desc* d, hipStream_t stream) 
     ModArgs a = mod_args(d, p);
     a.nblk = p.nblk; a.splits = p.splits;
     if (p.ordered) a.order = (const int*)((char*)d->ws + p.order_q);
+    a.abreast = start_abreast(a, a.Nq, a.B * a.Hk, 4l * d->head_dim * a.Nk);
     doc_tables(d, p, a, false, stream);
     const dim3 grid((unsigned)((long)a.B * a.H * a.nblk * a.splits));
     if (d->head_dim == 64) { if (p.nw == 1) fwd_go<64, 1>(a, grid, stream); else fwd_go<64, 4>(a, grid, stream); }
