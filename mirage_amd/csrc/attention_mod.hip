@@ -15,9 +15,9 @@
 // workgroup tests 64 tiles at a time (one per lane, one ballot) and walks only tiles that some row of it may see.  Per wave a tile is skipped,
 // whole (no test per score) or partial; in a partial one a lane holds what it sees as one bit per row of the tile.  Rows of up to 256 tokens are
 // walked without tables (forward, 32 x 8 heads, one document a row: 128 tokens 9.9 us without and 12.4 with, 256 15.8 and 17.7, 512 43.9 and
-// 43.7, there with several documents 69 and 55).  The row blocks of packed rows differ in length; where there are more of them than run at once,
-// the launch also puts them in order, the longest first (backward of 8 x 12 heads of 1024 in five documents 140 -> 110 us, one row of 8192 in
-// twelve documents, 16 heads 240 -> 200).
+// 43.7, there with several documents 69 and 55).  The row blocks of packed rows differ in length; where there are more than two of them for a
+// CU, the launch also puts them in order, the longest first (8 x 12 heads of 1024 in five documents: forward 49 -> 41 us, backward 140 -> 110; one
+// row of 8192 in twelve documents, 16 heads: backward 240 -> 200).
 //
 // Sums, maxima, lse and all products accumulate in fp32.  p is rounded to bf16 as an operand of the second product (at most 2^-8 of each weight,
 // averaging over the row; its sum is taken before the rounding).  ds goes into its product as two bf16 parts, and sum(do o) takes o with what its
