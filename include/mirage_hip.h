@@ -237,7 +237,8 @@ int mrg_resid_norm_bwd(const mrg_resid_norm_desc* d, hipStream_t stream);
  *   visible (i, j):  doc_q[b, i] == doc_k[b, j] >= 0 (documents given)  and  j < max(prefix[b], i + Nk - Nq + 1) (causal)
  * A row that sees nothing gives o = 0, lse = -inf and no gradient.  bf16, head_dim 32 or 64; H query heads share Hk key / value heads (H a
  * multiple of Hk: head h reads h / (H / Hk)).  *_bs / *_rs / *_hs: batch, row and head strides in elements.  Rows whose document is negative
- * see nothing and take part in no sum; values behind a mask do not reach the result even when they are not finite.
+ * see nothing and take part in no sum; values behind a mask do not reach the result even when they are not finite; a row
+ * that sees a value that is not finite may be NaN in full.
  *   fwd: o, lse fp32 [B, H, Nq] (may be NULL), o_rest (may be NULL): what the rounding of o to bf16 left out, bf16 with o's strides;
  *        ws: mrg_attn_mod_ws_bytes(d, 0) bytes.
  *   bwd: reads o, lse, d_o and, where given, o_rest (sum(do o) then takes o to 2^-16);  writes dq, dk, dv;  ws: mrg_attn_mod_ws_bytes(d, 1) bytes. */

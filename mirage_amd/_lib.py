@@ -6,6 +6,7 @@ There is no fallback: if the shared library is missing or fails to load, importi
 """
 import ctypes as C
 import os
+import struct
 
 import torch  # noqa: F401  (must precede CDLL: one HIP runtime per process)
 
@@ -96,6 +97,18 @@ class RotaryDesc(C.Structure):
                 ("dtype", ci), ("B", ci), ("N", ci), ("Hq", ci), ("Hk", ci), ("head_dim", ci),
                 ("pos_dtype", ci), ("pos", vp), ("pos_bs", cl), ("pos_rs", cl), ("freqs", vp),
                 ("axes", ci), ("sections", ci * MRG_MAX_AXES), ("pairing", ci), ("inverse", ci)]
+
+
+def packer(desc):
+    """A function that makes `desc` from the values of its fields in order (arrays item by item, null pointers as 0) with one struct.pack: 1.5 us for
+    the 33 values of a RotaryDesc, whose constructor takes 4.0.  A value that does not fit its field is an error, not cut off."""
+    codes = {vp: "P", cl: "l", ci: "i", cf: "f"}
+    fmt = "".join(codes[t] if t in codes else f"{t._length_}{codes[t._type_]}" for _, t in desc._fields_)
+    pack, make = struct.Struct(f"@{fmt}0q").pack, desc.from_buffer_copy
+    return lambda *values: make(pack(*values))
+
+
+rotary_desc = packer(RotaryDesc)
 
 
 class ResidNormDesc(C.Structure):

@@ -760,7 +760,7 @@ def _in_place(out: torch.Tensor, src: torch.Tensor) -> bool:
 
 
 _F64, _FLOATS, _POS, _I32, _ONLY32 = (torch.float64,), (BF16, F32), (torch.int32, F32), (torch.int32,), (F32,)
-_NO_STRIDE = (0, 0, 0)
+_NO_STRIDE = _NO_SECTIONS = (0, 0, 0)
 _DENSE = torch.contiguous_format                      # (empty_like with it costs half of torch.empty)
 _PAIRING = {"half": L.MRG_PAIR_HALF, "interleaved": L.MRG_PAIR_INTERLEAVED, "axial": L.MRG_PAIR_AXIAL}
 
@@ -803,7 +803,7 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], pos: torch.Tensor, f
             _need_apart(out_q, q, "rotary out_q")
         if k is not None:
             _need_apart(out_q, k, "rotary out_q")
-    k_ptr = ko_ptr = None
+    k_ptr = ko_ptr = 0
     Hk, ks, kos = 0, _NO_STRIDE, _NO_STRIDE
     if k is not None:
         kshape, ks = _heads(k, "rotary k", B, N, dev, dt)
@@ -824,9 +824,9 @@ def rotary_axes(q: torch.Tensor, k: Optional[torch.Tensor], pos: torch.Tensor, f
         k_ptr, ko_ptr = k.data_ptr(), out_k.data_ptr()
     elif out_k is not None:
         raise ValueError("mirage_amd: rotary out_k without k")
-    d = L.RotaryDesc(q.data_ptr(), k_ptr, out_q.data_ptr(), ko_ptr, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], qos[0], qos[1], qos[2], kos[0], kos[1], kos[2],
-                     L.MRG_DT_BF16 if dt is BF16 else L.MRG_DT_F32, B, N, Hq, Hk, hd, L.MRG_POS_F32 if pos.dtype is F32 else L.MRG_POS_I32, pos.data_ptr(),
-                     0 if shared else ps[0], ps[-2], freqs.data_ptr(), axes, tuple(sections), kind, 1 if inverse else 0)
+    d = L.rotary_desc(q.data_ptr(), k_ptr, out_q.data_ptr(), ko_ptr, qs[0], qs[1], qs[2], ks[0], ks[1], ks[2], qos[0], qos[1], qos[2], kos[0], kos[1], kos[2],
+                      L.MRG_DT_BF16 if dt is BF16 else L.MRG_DT_F32, B, N, Hq, Hk, hd, L.MRG_POS_F32 if pos.dtype is F32 else L.MRG_POS_I32, pos.data_ptr(),
+                      0 if shared else ps[0], ps[-2], freqs.data_ptr(), axes, *sections, *_NO_SECTIONS[axes:], kind, 1 if inverse else 0)
     _launch(lib.mrg_rotary_axes, d, dev, "mrg_rotary_axes")
     return out_q, out_k
 
@@ -1014,7 +1014,7 @@ def _attn_mod_ws(d, backward: int, dev):
 def attn_mod_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, mod: Optional[ScoreMod] = None, need_lse: bool = True):
     """softmax(modified scores) v (mrg_attn_mod_fwd): q bf16 [B, Nq, H, hd], k / v bf16 [B, Nk, Hk, hd], H a multiple of Hk, hd 32 or 64, any batch / row /
     head strides that are multiples of 8 elements.  Returns (o bf16 [B, Nq, H, hd], AttnSaved for the backward pass, or None without need_lse); a row that
-    sees nothing gives o = 0 and lse = -inf."""
+    sees nothing gives o = 0 and lse = -inf; what a mask hides may hold anything, and a row that sees a value that is not finite may be NaN in full."""
     d, dev = _attn_mod_desc(q, k, v, scale, mod)
     o = torch.empty_like(q, memory_format=_DENSE)
     d.o = o.data_ptr()

@@ -186,3 +186,13 @@ def test_modules_refuse():
     assert "blocks.0.attn.qkv.weight" in names and "blocks.1.seam2.gate" in names and "norm.weight" in names and not any("_first" in n or "norm1.bias" in n for n in names)
     with pytest.raises(RuntimeError, match="GPU"):
         enc(torch.zeros(1, 4, 128), torch.zeros(4, 3, dtype=torch.int32))
+
+
+def test_packed_descriptor_equals_the_constructors():
+    sizes = [n * 7919 + 1 for n in range(len(L.RotaryDesc._fields_))]
+    one = L.RotaryDesc(*sizes[:28], (3, 4, 5), *sizes[29:])
+    two = L.rotary_desc(*sizes[:28], 3, 4, 5, *sizes[29:])
+    assert bytes(one) == bytes(two) and isinstance(two, L.RotaryDesc)
+    assert L.RotaryDesc._fields_[28][0] == "sections"
+    with pytest.raises(Exception, match="argument out of range|format requires"):       # the constructor would cut it off
+        L.rotary_desc(*sizes[:17], 1 << 31, *sizes[18:28], 3, 4, 5, *sizes[29:])
