@@ -294,15 +294,35 @@ __device__ __forceinline__ int take_tile(unsigned long long& see) { const int i 
 
 // scores in registers: CAP -> log2 units, otherwise q.k stays as it is (the exponential takes the factor) and the bias comes in q.k's units.
 // kslope: slope / scale, or with CAP slope log2(e).  steep: (1 - tanh^2) / 4
-template <bool CAP, bool BIAS, bool STEEP>
+// cap tanh(s / cap) as cap - 2 cap u is off by up to cap 2^-21 whatever the score (u, near 1/2, is known to 2^-23): for caps up to CAP_NEAR at most
+// 2^-13, a 32nd of what the rounding of p to bf16 may be.  Above it scores below 0.35 cap come from tanh's series and all are within 2^-20 of
+// their value.  One kernel with both forms would hold the registers of the larger one and more (dq at head width 64 spills 124 bytes a lane
+// instead of 44, at 32 it runs three waves per SIMD instead of four), so each is compiled by itself.  The series costs (caps of 250 and 260, us forward
+// and backward): 8 x 12 heads of 1024 tokens in five documents 41 and 45, 110 and 131; 16 over 4 heads of 2048 without masks 79 and 100, 231 and 301.
+enum { NEAR = 1, FAR = 2 };                   // the forms of a cap; 0: none
+constexpr float CAP_NEAR = 256.f;
+template <int CAP, bool BIAS, bool STEEP>
 __device__ __forceinline__ void modify(f32x16& s, f32x16& steep, const ModArgs& a, const float (&mine)[3], const float* pos, int row0, float kslope, int lane) {
     if (CAP) {
         const float up = 2.f * a.scale * LOG2E_F / a.cap, capl = a.cap * LOG2E_F;
+        if (CAP == NEAR) {
 #pragma unroll
-        for (int r = 0; r < 16; ++r) {
-            const float u = __builtin_amdgcn_rcpf(fast_exp2(s[r] * up) + 1.f);                         // tanh(x) = 1 - 2 u, u = 1 / (e^2x + 1)
-            s[r] = fmaf(u, -2.f * capl, capl);
-            if (STEEP) steep[r] = fmaf(-u, u, u);                                                      // 1 - tanh^2 = 4 (u - u^2)
+            for (int r = 0; r < 16; ++r) {
+                const float u = __builtin_amdgcn_rcpf(fast_exp2(s[r] * up) + 1.f);                     // tanh(x) = 1 - 2 u, u = 1 / (e^2x + 1)
+                s[r] = fmaf(u, -2.f * capl, capl);
+                if (STEEP) steep[r] = fmaf(-u, u, u);                                                  // 1 - tanh^2 = 4 (u - u^2)
+            }
+        } else {
+            const float raw = a.scale * LOG2E_F;
+#pragma unroll
+            for (int r = 0; r < 16; ++r) {
+                const float y = s[r] * up, x = y * (0.5f * LN2_F), z = x * x;
+                // tanh(x) / x up to x^8; 1382 / 155925 x^10 is left out
+                const float t = fmaf(fmaf(fmaf(fmaf(z, 62.f / 2835.f, -17.f / 315.f), z, 2.f / 15.f), z, -1.f / 3.f), z, 1.f);
+                const float u = __builtin_amdgcn_rcpf(fast_exp2(y) + 1.f);
+                s[r] = fabsf(x) < 0.35f ? s[r] * raw * t : fmaf(u, -2.f * capl, capl);
+                if (STEEP) steep[r] = fmaf(-u, u, u);
+            }
         }
     }
     if (BIAS) {
@@ -367,7 +387,7 @@ __device__ __forceinline__ void store_o(const ModArgs& a, long at, const float4 
 // split over many of them.  NW = 4 otherwise: two waves would stage every tile for half as many queries (83 -> 102 us on 16 heads of 8192 packed
 // tokens).  Three waves per SIMD (98 us in three, 99 in two, 105 in four for 16 heads
 // of 4095 tokens behind a prefix); with a distance bias the registers are those of two (64 x 12 heads of 257 tokens 61 us, 63 when held to three).
-template <int HD, int NW, bool CAP, bool BIAS>
+template <int HD, int NW, int CAP, bool BIAS>
 __global__ __launch_bounds__(64 * NW, BIAS ? 2 : 3) void attn_mod_fwd_kernel(const ModArgs a) {
     constexpr int KS = HD / 16, DJ = HD / 32, NT = 64 * NW, TB = TT * HD * 2;
     __shared__ __attribute__((aligned(16))) char ldsK[2][TB];
@@ -616,7 +636,7 @@ __global__ __launch_bounds__(256) void attn_mod_join_kernel(const ModArgs a) {
 // (375 us the pass above in two), dk / dv and a distance bias at two: in three they spill (370 -> 512 us; 16 heads of 8192 packed tokens with a
 // distance 200 -> 299).
 // X, Y: the staged matrices (K, V or Q, dO); own fragments: (Q, dO) or (K, V).  OWN_Q also forms sum(do o), which OWN_K reads.
-template <int HD, bool OWN_Q, bool CAP, bool BIAS>
+template <int HD, bool OWN_Q, int CAP, bool BIAS>
 __global__ __launch_bounds__(256, OWN_Q && !BIAS ? 3 : 2) void attn_mod_bwd_kernel(const ModArgs a) {
     constexpr int KS = HD / 16, DJ = HD / 32, TB = TT * HD * 2;
     __shared__ __attribute__((aligned(16))) char ldsX[2][TB];
@@ -1014,27 +1034,27 @@ bool start_abreast(const ModArgs& a, int rows, int heads, long head_bytes) {
     return a.tab_k != nullptr || (tail > 0 && tail <= 32 && (heads + 7) / 8 * head_bytes <= (4l << 20));
 }
 
+template <int HD, int NW, int CAP>
+void fwd_go(const ModArgs& a, dim3 grid, hipStream_t st) {
+    if (a.slopes) hipLaunchKernelGGL((attn_mod_fwd_kernel<HD, NW, CAP, true>), grid, dim3(64 * NW), 0, st, a);
+    else hipLaunchKernelGGL((attn_mod_fwd_kernel<HD, NW, CAP, false>), grid, dim3(64 * NW), 0, st, a);
+}
 template <int HD, int NW>
 void fwd_go(const ModArgs& a, dim3 grid, hipStream_t st) {
-    const bool bias = a.slopes != nullptr;
-    if (a.cap > 0.f) {
-        if (bias) hipLaunchKernelGGL((attn_mod_fwd_kernel<HD, NW, true, true>), grid, dim3(64 * NW), 0, st, a);
-        else hipLaunchKernelGGL((attn_mod_fwd_kernel<HD, NW, true, false>), grid, dim3(64 * NW), 0, st, a);
-    } else {
-        if (bias) hipLaunchKernelGGL((attn_mod_fwd_kernel<HD, NW, false, true>), grid, dim3(64 * NW), 0, st, a);
-        else hipLaunchKernelGGL((attn_mod_fwd_kernel<HD, NW, false, false>), grid, dim3(64 * NW), 0, st, a);
-    }
+    if (a.cap > CAP_NEAR) fwd_go<HD, NW, FAR>(a, grid, st);
+    else if (a.cap > 0.f) fwd_go<HD, NW, NEAR>(a, grid, st);
+    else fwd_go<HD, NW, 0>(a, grid, st);
+}
+template <int HD, bool OWN_Q, int CAP>
+void bwd_go(const ModArgs& a, dim3 grid, hipStream_t st) {
+    if (a.slopes) hipLaunchKernelGGL((attn_mod_bwd_kernel<HD, OWN_Q, CAP, true>), grid, dim3(256), 0, st, a);
+    else hipLaunchKernelGGL((attn_mod_bwd_kernel<HD, OWN_Q, CAP, false>), grid, dim3(256), 0, st, a);
 }
 template <int HD, bool OWN_Q>
 void bwd_go(const ModArgs& a, dim3 grid, hipStream_t st) {
-    const bool bias = a.slopes != nullptr;
-    if (a.cap > 0.f) {
-        if (bias) hipLaunchKernelGGL((attn_mod_bwd_kernel<HD, OWN_Q, true, true>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((attn_mod_bwd_kernel<HD, OWN_Q, true, false>), grid, dim3(256), 0, st, a);
-    } else {
-        if (bias) hipLaunchKernelGGL((attn_mod_bwd_kernel<HD, OWN_Q, false, true>), grid, dim3(256), 0, st, a);
-        else hipLaunchKernelGGL((attn_mod_bwd_kernel<HD, OWN_Q, false, false>), grid, dim3(256), 0, st, a);
-    }
+    if (a.cap > CAP_NEAR) bwd_go<HD, OWN_Q, FAR>(a, grid, st);
+    else if (a.cap > 0.f) bwd_go<HD, OWN_Q, NEAR>(a, grid, st);
+    else bwd_go<HD, OWN_Q, 0>(a, grid, st);
 }
 template <bool OWN_Q>
 void bwd_side(ModArgs a, int splits, int HD, hipStream_t st) {

@@ -1,0 +1,75 @@
+"""Packed-volume operators at the edges of what they accept, against their formulas in 64 bits: large caps, sizes, gradients and paddings as a caller
+may hand them over."""
+import math
+
+import pytest
+import torch
+
+pytestmark = pytest.mark.gpu
+
+BF16, F32, F64 = torch.bfloat16, torch.float32, torch.float64
+HALF16, HALF32 = torch.finfo(BF16).eps / 2, torch.finfo(F32).eps / 2
+
+
+@pytest.fixture(scope="module")
+def K():
+    assert torch.cuda.is_available(), "GPU tests need a GPU"
+    from mirage_amd import kernels
+    return kernels
+
+
+def dev():
+    return torch.device("cuda:0")
+
+
+def rnd(*shape, dtype=F32, scale=1.0, seed=0):
+    return (torch.randn(*shape, generator=torch.Generator().manual_seed(seed)) * scale).to(dtype).to(dev())
+
+
+def within(got, ref, bound, what):
+    bad = ~((got.double() - ref).abs() <= bound)
+    assert not bad.any(), f"{what}: {int(bad.sum())} of {bad.numel()} out of bounds, worst {float(((got.double() - ref).abs() / bound)[bad].max()):.3g} x"
+
+
+def capped_attention(q, k, v, d_o, scale, cap):
+    """o, lse, dq, dk, dv with elementwise bounds.  Noise of a score: fp32 accumulation of q.k; the cap's own error, cap 2^-21 for caps up to 256 and
+    2^-20 of the score above; factor, running maximum and exponential.  Then the roundings to bf16: p in its products, o, the gradients; ds
+    enters its products to 2^-16, o its sum with d_o as well."""
+    q, k, v, g = (t.double().transpose(1, 2) for t in (q, k, v, d_o))
+    raw = q @ k.transpose(-1, -2) * scale
+    th = torch.tanh(raw / cap)
+    s, steep = cap * th, 1 - th * th
+    noise = (q.abs() @ k.abs().transpose(-1, -2)) * scale * (q.shape[-1] * HALF32) + (s.abs() + 16) * 8 * HALF32
+    noise = noise + (cap * 2.0 ** -21 if cap <= 256 else s.abs() * 2.0 ** -20)
+    p = torch.softmax(s, -1)
+    wob = noise.amax(-1, keepdim=True) * 2                                      # relative error of p in fp32
+    o = p @ v
+    eo = (p @ v.abs()) * (HALF16 + wob + 64 * HALF32)
+    dp = g @ v.transpose(-1, -2)
+    ds = p * (dp - (g * o).sum(-1, keepdim=True)) * steep
+    eD, fp = (g.abs() * eo).sum(-1, keepdim=True), (wob + 128 * HALF32) * 4
+    eds = ds.abs() * 2.0 ** -16 + p * eD + p * ((g.abs() @ v.abs().transpose(-1, -2)) + (g.abs() * o.abs()).sum(-1, keepdim=True)) * fp
+    dq, dk, dv = ds @ k * scale, ds.transpose(-1, -2) @ q * scale, p.transpose(-1, -2) @ g
+    half = lambda t: t.abs() * HALF16 * 1.01 + 1e-30
+    out = {"o": (o, eo + half(o)), "dq": (dq, eds @ k.abs() * scale + half(dq)), "dk": (dk, eds.transpose(-1, -2) @ q.abs() * scale + half(dk)),
+           "dv": (dv, (p * (HALF16 + fp)).transpose(-1, -2) @ g.abs() + half(dv))}
+    lse = torch.logsumexp(s, -1)
+    return {n: (a.transpose(1, 2), e.transpose(1, 2)) for n, (a, e) in out.items()} | {"lse": (lse, wob[..., 0] + 4e-6 * (1 + lse.abs()))}
+
+
+@pytest.mark.parametrize("Nq,hd,bias", [(150, 64, False), (1, 64, False), (70, 32, False), (150, 64, True)])
+@pytest.mark.parametrize("cap,size", [(200.0, 1.5), (256.0, 1.5), (257.0, 1.5), (300.0, 12.0), (1e3, 1.5), (1e3, 20.0), (1e5, 1.5), (1e6, 1.5), (1e8, 1.5), (9e29, 1.5)])
+def test_caps_of_any_size(K, cap, size, Nq, hd, bias):
+    """a cap far above the scores leaves them as they are; near them (size 12 and 20: scores to some hundreds) it bends them"""
+    B, H, Nk = 2, 2, 333
+    q, k = rnd(B, Nq, H, hd, dtype=BF16, scale=size, seed=1), rnd(B, Nk, H, hd, dtype=BF16, scale=size, seed=2)
+    v, d_o, scale = rnd(B, Nk, H, hd, dtype=BF16, seed=3), rnd(B, Nq, H, hd, dtype=BF16, seed=4), hd ** -0.5
+    # a distance of zero everywhere: the kernels with a bias, the same values
+    at = dict(slopes=torch.ones(H, device=dev()), pos_q=torch.ones(B, Nq, 1, device=dev()), pos_k=torch.ones(B, Nk, 1, device=dev())) if bias else {}
+    mod = K.ScoreMod(cap=cap, **at)
+    ref = capped_attention(q, k, v, d_o, scale, cap)
+    o, saved = K.attn_mod_fwd(q, k, v, scale, mod)
+    within(o, *ref["o"], "o")
+    within(saved.lse, *ref["lse"], "lse")
+    for got, n in zip(K.attn_mod_bwd(q, k, v, o, saved, d_o, scale, mod), ("dq", "dk", "dv")):
+        within(got, *ref[n], n)
