@@ -975,8 +975,10 @@ int mod_check(const mrg_attn_mod_desc* d, const char* who) {
                 MRG_ERR_SHAPE, "%s: too many rows for one launch", who);
     // a tile's rows are addressed by 32-bit offsets from its first one
     MRG_REQUIRE((d->Nq <= 1 || (d->q_rs <= (1 << 23) && d->do_rs <= (1 << 23))) && (d->Nk <= 1 || (d->k_rs <= (1 << 23) && d->v_rs <= (1 << 23))), MRG_ERR_SHAPE, "%s: row strides above 2^23 elements", who);
-    MRG_REQUIRE(d->scale > 0.f && d->scale < 1e30f, MRG_ERR_ARG, "%s: scale %g must be positive and finite", who, d->scale);
-    MRG_REQUIRE(d->cap >= 0.f && d->cap < 1e30f, MRG_ERR_ARG, "%s: cap %g must be 0 (none) or positive", who, d->cap);
+    // (the kernels form scale / cap, slope / scale and lse / scale in fp32)
+    MRG_REQUIRE(d->scale >= 1e-30f && d->scale < 1e30f, MRG_ERR_ARG, "%s: scale %g must be positive and finite (1e-30 to 1e30)", who, d->scale);
+    MRG_REQUIRE(d->cap == 0.f || (d->cap >= 1e-30f && d->cap < 1e30f), MRG_ERR_ARG, "%s: cap %g must be 0 (none) or positive and finite (1e-30 to 1e30)", who, d->cap);
+    MRG_REQUIRE(d->cap == 0.f || d->scale <= 1e30f * d->cap, MRG_ERR_ARG, "%s: cap %g is too small for a scale of %g", who, d->cap, d->scale);
     const bool some = d->B > 0 && d->Nq > 0 && d->Nk > 0;        // (tensors without elements may have no address)
     MRG_REQUIRE(!some || ((d->slopes != nullptr) == (d->pos_q != nullptr) && (d->slopes != nullptr) == (d->pos_k != nullptr)), MRG_ERR_ARG, "%s: a distance bias needs slopes, pos_q and pos_k", who);
     MRG_REQUIRE(!d->slopes || (d->axes >= 1 && d->axes <= MRG_MAX_AXES), MRG_ERR_SHAPE, "%s: %d axes (1 to %d)", who, d->axes, MRG_MAX_AXES);

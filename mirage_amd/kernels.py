@@ -935,7 +935,7 @@ def resid_norm_bwd(dx_new: torch.Tensor, dy: Optional[torch.Tensor], x_new: torc
 
 class ScoreMod:
     """What attn_mod_fwd / attn_mod_bwd do to the scores besides the scale (include/mirage_hip.h mrg_attn_mod_desc):
-    cap            s = cap tanh(s / cap); 0: none
+    cap            s = cap tanh(s / cap), 1e-30 <= cap < 1e30; 0: none
     slopes         fp32 [heads], with pos_q [B, Nq, axes] and pos_k [B, Nk, axes] (fp32, 1 to 3 axes): s -= slopes[h] sum_a |pos_q - pos_k|
     doc_q, doc_k   int32 [B, Nq], [B, Nk]: a query sees the keys of its own document; negative: padding, sees and is seen by nothing
     causal         query i sees keys j <= i + Nk - Nq (the last query sees all); prefix int32 [B]: and keys j < prefix in any case
@@ -943,8 +943,8 @@ class ScoreMod:
     __slots__ = ("cap", "slopes", "pos_q", "pos_k", "doc_q", "doc_k", "causal", "prefix")
 
     def __init__(self, cap: float = 0.0, slopes=None, pos_q=None, pos_k=None, doc_q=None, doc_k=None, causal: bool = False, prefix=None):
-        if not 0.0 <= float(cap) < 1e30:
-            raise ValueError(f"mirage_amd: ScoreMod cap {cap} must be 0 (none) or positive and finite")
+        if float(cap) != 0.0 and not 1e-30 <= float(cap) < 1e30:
+            raise ValueError(f"mirage_amd: ScoreMod cap {cap} must be 0 (none) or positive and finite (1e-30 to 1e30)")
         if not ((slopes is None) == (pos_q is None) == (pos_k is None)):
             raise ValueError("mirage_amd: ScoreMod distance bias needs slopes, pos_q and pos_k together")
         if (doc_q is None) != (doc_k is None):

@@ -1,0 +1,43 @@
+"""Refusals and host helpers of the packed-volume operators at the edges of what they accept: no GPU needed, nothing is launched."""
+import ctypes as C
+
+import pytest
+import torch
+
+from mirage_amd import _lib as L
+from mirage_amd import kernels as K
+
+BF16 = torch.bfloat16
+
+
+def error():
+    return L.lib.mrg_last_error_string().decode()
+
+
+def attn_desc(**kw):
+    d = L.AttnModDesc()
+    for f in ("q", "k", "v", "o", "lse", "d_o", "dq", "dk", "dv", "ws"):
+        setattr(d, f, 4096)
+    for f, _ in L.AttnModDesc._fields_:
+        if f[-3:] in ("_bs", "_rs", "_hs"):
+            setattr(d, f, 64)
+    d.B, d.H, d.Hk, d.Nq, d.Nk, d.head_dim, d.scale = 1, 4, 2, 5, 5, 64, 0.125
+    for k, v in kw.items():
+        setattr(d, k, v)
+    return d
+
+
+@pytest.mark.parametrize("kw,text", [(dict(scale=1e-38), "scale"), (dict(cap=1e-40), "cap"), (dict(cap=1e-31), "cap"), (dict(cap=1e30), "cap"), (dict(scale=1e10, cap=1e-25), "too small")])
+def test_attention_refuses_factors_whose_quotients_leave_fp32(kw, text):
+    d = attn_desc(**kw)
+    for f in (L.lib.mrg_attn_mod_fwd, L.lib.mrg_attn_mod_bwd):
+        assert f(C.byref(d), None) < 0 and text in error()
+    assert L.lib.mrg_attn_mod_ws_bytes(C.byref(d), 0) == -1
+
+
+def test_score_mod_refuses_a_cap_that_fp32_cannot_hold():
+    for cap in (1e-46, 1e-40, -0.5, 1e30):                       # the first would arrive as 0: no cap at all
+        with pytest.raises(ValueError, match="cap"):
+            K.ScoreMod(cap=cap)
+    assert K.ScoreMod(cap=1e-30).cap == 1e-30 and K.ScoreMod(cap=-0.0).cap == 0.0
+    assert L.lib.mrg_attn_mod_ws_bytes(C.byref(attn_desc(cap=1e-30)), 0) == 0        # the smallest one arrives and is accepted

@@ -73,3 +73,17 @@ def test_caps_of_any_size(K, cap, size, Nq, hd, bias):
     within(saved.lse, *ref["lse"], "lse")
     for got, n in zip(K.attn_mod_bwd(q, k, v, o, saved, d_o, scale, mod), ("dq", "dk", "dv")):
         within(got, *ref[n], n)
+
+
+@pytest.mark.parametrize("cap", [1e-30, 1e-3, 0.25])
+def test_smallest_caps(K, cap):
+    """every score at the cap, one of them with nothing to bend (a query of zeros)"""
+    q, k, v, d_o = (rnd(1, 100, 2, 64, dtype=BF16, seed=i) for i in range(4))
+    q[0, 3] = 0
+    ref = capped_attention(q, k, v, d_o, 0.125, cap)
+    mod = K.ScoreMod(cap=cap)
+    o, saved = K.attn_mod_fwd(q, k, v, 0.125, mod)
+    within(o, *ref["o"], "o")
+    within(saved.lse, *ref["lse"], "lse")
+    for got, n in zip(K.attn_mod_bwd(q, k, v, o, saved, d_o, 0.125, mod), ("dq", "dk", "dv")):
+        within(got, *ref[n], n)
