@@ -973,7 +973,10 @@ int mod_check(const mrg_attn_mod_desc* d, const char* who) {
                 d->B, d->H, d->Hk, d->Nq, d->Nk);
     MRG_REQUIRE(d->Nq <= (1 << 26) && d->Nk <= (1 << 26) && (long)d->B * d->H * (((long)(d->Nq > d->Nk ? d->Nq : d->Nk) + 31) / 32) * MAX_SPLITS <= 0x7fffffffl,
                 MRG_ERR_SHAPE, "%s: too many rows for one launch", who);
-    // a tile's rows are addressed by 32-bit offsets from its first one
+    const long steps[] = {d->q_bs, d->q_rs, d->q_hs, d->k_bs, d->k_rs, d->k_hs, d->v_bs, d->v_rs, d->v_hs, d->o_bs, d->o_rs, d->o_hs, d->do_bs, d->do_rs, d->do_hs,
+                          d->dq_bs, d->dq_rs, d->dq_hs, d->dk_bs, d->dk_rs, d->dk_hs, d->dv_bs, d->dv_rs, d->dv_hs};
+    for (const long s : steps) MRG_REQUIRE(s >= 0, MRG_ERR_SHAPE, "%s: negative stride %ld", who, s);
+    // a tile's rows are addressed by 32-bit unsigned offsets from its first one
     MRG_REQUIRE((d->Nq <= 1 || (d->q_rs <= (1 << 23) && d->do_rs <= (1 << 23))) && (d->Nk <= 1 || (d->k_rs <= (1 << 23) && d->v_rs <= (1 << 23))), MRG_ERR_SHAPE, "%s: row strides above 2^23 elements", who);
     // (the kernels form scale / cap, slope / scale and lse / scale in fp32)
     MRG_REQUIRE(d->scale >= 1e-30f && d->scale < 1e30f, MRG_ERR_ARG, "%s: scale %g must be positive and finite (1e-30 to 1e30)", who, d->scale);

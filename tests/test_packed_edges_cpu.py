@@ -41,3 +41,11 @@ def test_score_mod_refuses_a_cap_that_fp32_cannot_hold():
             K.ScoreMod(cap=cap)
     assert K.ScoreMod(cap=1e-30).cap == 1e-30 and K.ScoreMod(cap=-0.0).cap == 0.0
     assert L.lib.mrg_attn_mod_ws_bytes(C.byref(attn_desc(cap=1e-30)), 0) == 0        # the smallest one arrives and is accepted
+
+
+@pytest.mark.parametrize("name", ["q_rs", "k_rs", "v_rs", "do_rs", "k_bs", "o_hs", "dv_rs"])
+def test_attention_refuses_negative_strides(name):
+    """rows of a tile lie at unsigned offsets from its first one: a negative stride would be read some GiB behind it"""
+    d = attn_desc(Nq=100, Nk=100, **{name: -64})
+    for f in (L.lib.mrg_attn_mod_fwd, L.lib.mrg_attn_mod_bwd):
+        assert f(C.byref(d), None) < 0 and "negative stride" in error()
