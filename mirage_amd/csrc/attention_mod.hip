@@ -647,7 +647,9 @@ __global__ __launch_bounds__(256, OWN_Q && !BIAS ? 3 : 2) void attn_mod_bwd_kern
     const int tid = threadIdx.x, lane = tid & 63, wave = tid >> 6;
     const int OH = OWN_Q ? a.H : a.Hk;                                               // the owner's head: a query head or a key head
     int bo, blk;
-    place(blockIdx.x, a.B * OH, a.nblk * a.splits, a.abreast, bo, blk);
+    const unsigned id = blockIdx.y * gridDim.x + blockIdx.x;                         // (a second dimension from 2^24 workgroups on)
+    if (id >= (unsigned)(a.B * OH) * a.nblk * a.splits) return;
+    place((int)id, a.B * OH, a.nblk * a.splits, a.abreast, bo, blk);
     const int split = blk % a.splits, b = bo / OH, ho = bo - b * OH;
     blk /= a.splits;
     if (a.order) blk = a.order[(long)b * a.nblk + blk];
@@ -1068,7 +1070,9 @@ void bwd_side(ModArgs a, int splits, int HD, hipStream_t st) {
     a.splits = splits;
     a.nblk = (NO + 127) / 128;
     a.abreast = start_abreast(a, NO, a.B * a.Hk, 4l * HD * (OWN_Q ? a.Nk : a.Nq * (long)a.G));
-    const dim3 grid((unsigned)((long)a.B * OH * a.nblk * splits));
+    // a launch has less than 2^32 threads along a dimension; a forward pass of up to 32 tokens a head fits more heads into them than these workgroups do
+    const long blocks = (long)a.B * OH * a.nblk * splits, across = blocks < (1l << 24) ? blocks : 1l << 23;
+    const dim3 grid((unsigned)across, (unsigned)((blocks + across - 1) / across));
     if (HD == 64) bwd_go<64, OWN_Q>(a, grid, st); else bwd_go<32, OWN_Q>(a, grid, st);
     if (splits > 1) {
         const long rows = (long)a.B * OH * NO, threads = rows * (OWN_Q ? 1 : 2) * HD / 4;

@@ -87,3 +87,16 @@ def test_smallest_caps(K, cap):
     within(saved.lse, *ref["lse"], "lse")
     for got, n in zip(K.attn_mod_bwd(q, k, v, o, saved, d_o, 0.125, mod), ("dq", "dk", "dv")):
         within(got, *ref[n], n)
+
+
+def test_attn_mod_of_more_heads_than_workgroups_fit_one_dimension(K):
+    """2^24 and some (batch, head) pairs of one token, whose backward pass needs a second dimension of workgroups: o = v, dv = d_o, nothing for q and k"""
+    B = (1 << 24) + 5
+    g = torch.Generator(device=dev()).manual_seed(1)
+    q, k, v, d_o = (torch.randn(B, 1, 1, 32, generator=g, device=dev(), dtype=BF16) for _ in range(4))
+    o, saved = K.attn_mod_fwd(q, k, v, 0.125)
+    assert torch.equal(o, v)
+    dq, dk, dv = K.attn_mod_bwd(q, k, v, o, saved, d_o, 0.125)
+    assert torch.equal(dv, d_o)
+    # dp - sum(do o) is the difference of two fp32 sums of the same 32 products (sizes below 64 x 8): 64 2^-24 of their sizes, times q or k and the scale
+    assert float(dq.abs().amax()) < 1e-2 and float(dk.abs().amax()) < 1e-2
