@@ -102,8 +102,10 @@ template <int NV, int WPR, bool BR32>
 __global__ __launch_bounds__(256) void resid_norm_fwd_kernel(const ResidArgs a) {
     __shared__ float box[2][2][WPR];
     const int lane = threadIdx.x & 63, wave = threadIdx.x >> 6;
-    const int row = WPR == 1 ? blockIdx.x * 4 + wave : blockIdx.x;
-    if (WPR == 1 && row >= a.M) return;
+    const unsigned blk = blockIdx.y * gridDim.x + blockIdx.x;     // (a second dimension from 2^24 workgroups on)
+    const unsigned at = WPR == 1 ? blk * 4 + wave : blk;
+    if (at >= (unsigned)a.M) return;
+    const int row = (int)at;
     RowSum<WPR> sum{box, 0, wave};
     const int D = a.D, nv = D >> 2, c0 = WPR == 1 ? lane : threadIdx.x, step = 64 * WPR;
     const float invD = 1.f / (float)D;
@@ -341,7 +343,9 @@ extern "C" int mrg_resid_norm_fwd(const mrg_resid_norm_desc* d, hipStream_t stre
     MRG_REQUIRE(d->x && d->branch && d->x_new && (!d->pre_w || d->y) && ((!d->pre_w && !d->post_w) || d->stats), MRG_ERR_ARG, "mrg_resid_norm_fwd: null pointer");
     const bool wide = d->D > 1024, f = d->branch_dtype == MRG_DT_F32;
     const int nv = wide ? (d->D + 1023) / 1024 : (d->D + 255) / 256;
-    const dim3 grid(wide ? a.M : (a.M + 3) / 4);
+    // a launch has less than 2^32 threads along a dimension
+    const long blocks = wide ? a.M : ((long)a.M + 3) / 4, across = blocks < (1l << 24) ? blocks : 1l << 23;
+    const dim3 grid((unsigned)across, (unsigned)((blocks + across - 1) / across));
 #define RN_F(NV, WPR) do { if (f) hipLaunchKernelGGL((resid_norm_fwd_kernel<NV, WPR, true>), grid, dim3(256), 0, stream, a); \
                            else hipLaunchKernelGGL((resid_norm_fwd_kernel<NV, WPR, false>), grid, dim3(256), 0, stream, a); } while (0)
     if (wide) { if (nv == 2) RN_F(2, 4); else if (nv == 3) RN_F(3, 4); else RN_F(4, 4); }

@@ -100,3 +100,23 @@ def test_attn_mod_of_more_heads_than_workgroups_fit_one_dimension(K):
     assert torch.equal(dv, d_o)
     # dp - sum(do o) is the difference of two fp32 sums of the same 32 products (sizes below 64 x 8): 64 2^-24 of their sizes, times q or k and the scale
     assert float(dq.abs().amax()) < 1e-2 and float(dk.abs().amax()) < 1e-2
+
+
+def test_resid_norm_of_more_rows_than_one_dimension_of_workgroups(K):
+    """every row as in calls of a part of them, the last ones as well"""
+    M, D = (1 << 26) + 5, 4
+    x = torch.empty(1, M, D, device=dev())
+    b = torch.empty(1, M, D, device=dev(), dtype=BF16)
+    tile = 1 << 16
+    for at in range(0, M, tile):                                   # rows repeat, but for the first element that counts the tiles
+        n = min(tile, M - at)
+        if at == 0:
+            x[:, :n], b[:, :n] = rnd(1, n, D, seed=1), rnd(1, n, D, dtype=BF16, seed=2)
+        else:
+            x[:, at:at + n], b[:, at:at + n] = x[:, :n], b[:, :n]
+        x[:, at:at + n, 0] = at / tile * 2.0 ** -6
+    how = dict(gate=rnd(D, seed=3), alpha=0.5, post=(rnd(D, seed=4), rnd(D, seed=5)), pre=(rnd(D, seed=6), rnd(D, seed=7)))
+    x_new, y, stats = K.resid_norm_fwd(x, b, **how)
+    for lo, hi in ((0, 1000), (M // 2 - 500, M // 2 + 500), (M - 1000, M)):
+        part, py, ps = K.resid_norm_fwd(x[:, lo:hi].clone(), b[:, lo:hi].clone(), **how)   # (clones: rows of 8 bytes)
+        assert torch.equal(part, x_new[:, lo:hi]) and torch.equal(py, y[:, lo:hi]) and torch.equal(ps, stats[:, lo:hi])
