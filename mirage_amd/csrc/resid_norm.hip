@@ -239,32 +239,34 @@ __global__ __launch_bounds__(WPR == 1 ? 256 : 64 * WPR, 4) void resid_norm_bwd_k
     if (POST) { flush(GA, out + 2 * D); if (a.post_b) flush(GT, out + 3 * D); }
 }
 
-// column sums of the partial rows: job j (blockIdx.x) adds `n` rows that lie `stride` floats apart.  32 columns and 32 rows at a time; the
-// order of the additions is fixed by the sizes alone
+// column sums of the partial rows: a job adds `n` rows that lie `stride` floats apart.  32 columns and 32 rows at a time; the order of the
+// additions is fixed by the sizes alone.  More gates than a launch has workgroups for (2^24) are walked
 struct SumJob { const float* src; float* dst; int n; long stride; };
-struct SumArgs { SumJob job[4]; const float* gsrc; float* gdst; int parts, D; };
-__global__ __launch_bounds__(256) void resid_norm_sum_kernel(const SumArgs a, int njobs) {
+struct SumArgs { SumJob job[4]; const float* gsrc; float* gdst; int parts, D, njobs, jobs; };
+__global__ __launch_bounds__(256) void resid_norm_sum_kernel(const SumArgs a) {
     __shared__ __attribute__((aligned(16))) float4 box[32][8];
     const int cl = threadIdx.x & 7, rl = threadIdx.x >> 3;
     const int c = blockIdx.y * 8 + cl;
-    SumJob job;
-    if ((int)blockIdx.x < njobs) job = a.job[blockIdx.x];
-    else {
-        const long s = (long)blockIdx.x - njobs;                  // one sample's gate: its parts are consecutive rows
-        job = SumJob{a.gsrc + s * a.parts * a.D, a.gdst + s * a.D, a.parts, (long)a.D};
-    }
-    float4 s = zero4();
-    if (c * 4 < a.D) {
+    for (long j = blockIdx.x; j < a.jobs; j += gridDim.x) {
+        SumJob job;
+        if (j < a.njobs) job = a.job[j];
+        else {
+            const long s = j - a.njobs;                     // one sample's gate: its parts are consecutive rows
+            job = SumJob{a.gsrc + s * a.parts * a.D, a.gdst + s * a.D, a.parts, (long)a.D};
+        }
+        float4 s = zero4();
+        if (c * 4 < a.D) {
 #pragma unroll 4
-        for (int r = rl; r < job.n; r += 32) s = s + reinterpret_cast<const float4*>(job.src + (long)r * job.stride)[c];
-    }
-    box[rl][cl] = s;
-    __syncthreads();
-    for (int w = 16; w > 0; w >>= 1) {
-        if (rl < w) box[rl][cl] = box[rl][cl] + box[rl + w][cl];
+            for (int r = rl; r < job.n; r += 32) s = s + reinterpret_cast<const float4*>(job.src + (long)r * job.stride)[c];
+        }
+        box[rl][cl] = s;
         __syncthreads();
+        for (int w = 16; w > 0; w >>= 1) {
+            if (rl < w) box[rl][cl] = box[rl][cl] + box[rl + w][cl];
+            __syncthreads();
+        }
+        if (rl == 0 && c * 4 < a.D) reinterpret_cast<float4*>(job.dst)[c] = box[0][cl];      // (written again by this thread itself)
     }
-    if (rl == 0 && c * 4 < a.D) reinterpret_cast<float4*>(job.dst)[c] = box[0][cl];
 }
 
 // waves of a backward row, and of a workgroup (four rows side by side where one wave holds a row)
@@ -398,6 +400,8 @@ extern "C" int mrg_resid_norm_bwd(const mrg_resid_norm_desc* d, hipStream_t stre
     s.gsrc = a.gpart; s.gdst = d->d_gate; s.D = d->D;
     s.parts = a.M == 0 ? 0 : (sample ? parts : grid);
     const int gates = gated ? (sample ? d->samples : 1) : 0;
-    if (njobs + gates) hipLaunchKernelGGL(resid_norm_sum_kernel, dim3(njobs + gates, (d->D / 4 + 7) / 8), dim3(256), 0, stream, s, njobs);
+    s.njobs = njobs; s.jobs = njobs + gates;
+    const int across = s.jobs < (1 << 23) ? s.jobs : 1 << 23;
+    if (s.jobs) hipLaunchKernelGGL(resid_norm_sum_kernel, dim3(across, (d->D / 4 + 7) / 8), dim3(256), 0, stream, s);
     return mrg_check_launch("mrg_resid_norm_bwd");
 }

@@ -120,3 +120,16 @@ def test_resid_norm_of_more_rows_than_one_dimension_of_workgroups(K):
     for lo, hi in ((0, 1000), (M // 2 - 500, M // 2 + 500), (M - 1000, M)):
         part, py, ps = K.resid_norm_fwd(x[:, lo:hi].clone(), b[:, lo:hi].clone(), **how)   # (clones: rows of 8 bytes)
         assert torch.equal(part, x_new[:, lo:hi]) and torch.equal(py, y[:, lo:hi]) and torch.equal(ps, stats[:, lo:hi])
+
+
+def test_resid_norm_of_more_gates_than_workgroups(K):
+    """2^24 and some samples of one row and a gate each: the gates' gradients are dx' times the branch, element by element"""
+    S, D = (1 << 24) + 3, 4
+    g = torch.Generator(device=dev()).manual_seed(1)
+    x, b, gate, dx_new = (torch.randn(S, 1, D, generator=g, device=dev()) for _ in range(4))
+    gate = gate.view(S, D)
+    x_new, _, _ = K.resid_norm_fwd(x, b, gate=gate)
+    x_, n_ = x.view(S, D), gate * b.view(S, D)
+    assert bool(((x_new.view(S, D) - (x_ + n_)).abs() <= 2 * HALF32 * (x_.abs() + 2 * n_.abs())).all())      # a product and a sum, each rounded on either side
+    dx, db, grads = K.resid_norm_bwd(dx_new, None, x_new, b, None, gate=gate)
+    assert torch.equal(dx, dx_new) and torch.equal(db.view(S, D), dx_new.view(S, D) * gate) and torch.equal(grads["gate"], dx_new.view(S, D) * b.view(S, D))
