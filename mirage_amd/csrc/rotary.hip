@@ -45,7 +45,9 @@ __device__ __forceinline__ void rot_put(bf16_t& d, float x) { d = f2bf(x); }
 template <typename T, int VEC, bool INTER>
 __global__ __launch_bounds__(256) void rotary_kernel(const RotArgs a) {
     extern __shared__ __attribute__((aligned(16))) float2 cs[];        // [rows][P] (cos, sin)
-    const int r0 = blockIdx.x * a.rows, nrow = min(a.rows, a.rows_total - r0);
+    const unsigned start = (blockIdx.z * gridDim.x + blockIdx.x) * a.rows;     // (a further dimension from 2^24 workgroups on)
+    if (start >= (unsigned)a.rows_total) return;
+    const int r0 = (int)start, nrow = min(a.rows, a.rows_total - r0);
     const int P = a.P;
     for (int i = threadIdx.x; i < nrow * P; i += 256) {
         const int rr = i / P, p = i - rr * P;
@@ -182,7 +184,9 @@ extern "C" int mrg_rotary_axes(const mrg_rotary_desc* d, hipStream_t stream) {
     const int row_units = (a.s[0].H > a.s[sides - 1].H ? a.s[0].H : a.s[sides - 1].H) * (a.units + a.tail);
     while (rows < 16 && rows * row_units < 256 && a.rows_total / rows > 2048) rows <<= 1;
     a.rows = rows;
-    const dim3 grid((a.rows_total + rows - 1) / rows, sides);
+    // a launch has less than 2^32 threads along a dimension
+    const int blocks = (a.rows_total + rows - 1) / rows, across = blocks < (1 << 24) ? blocks : 1 << 23;
+    const dim3 grid(across, sides, (blocks - 1) / across + 1);
     const size_t lds = sizeof(float2) * rows * P;
     if (d->dtype == MRG_DT_BF16) {
         if (vec == 8) rot_launch<bf16_t, 8>(a, inter, grid, lds, stream);

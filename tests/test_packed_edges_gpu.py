@@ -133,3 +133,16 @@ def test_resid_norm_of_more_gates_than_workgroups(K):
     assert bool(((x_new.view(S, D) - (x_ + n_)).abs() <= 2 * HALF32 * (x_.abs() + 2 * n_.abs())).all())      # a product and a sum, each rounded on either side
     dx, db, grads = K.resid_norm_bwd(dx_new, None, x_new, b, None, gate=gate)
     assert torch.equal(dx, dx_new) and torch.equal(db.view(S, D), dx_new.view(S, D) * gate) and torch.equal(grads["gate"], dx_new.view(S, D) * b.view(S, D))
+
+
+def test_rotary_of_more_rows_than_one_dimension_of_workgroups(K):
+    """2^28 and some rows of two elements (16 rows a workgroup): the last ones as in calls of a part of them"""
+    N = (1 << 28) + 37
+    q = torch.empty(1, N, 1, 2, device=dev(), dtype=BF16)
+    q.view(torch.int16).copy_(torch.arange(2 * N, device=dev(), dtype=torch.int32).view(q.shape) % 16001)      # bits of small numbers, different from row to row
+    pos = torch.arange(N, device=dev(), dtype=torch.int32)[:, None]
+    freqs = torch.ones(1, dtype=F64, device=dev())
+    out, _ = K.rotary_axes(q, None, pos, freqs, (1,))
+    for lo, hi in ((0, 1000), (N // 2, N // 2 + 1000), (N - 1000, N)):
+        part, _ = K.rotary_axes(q[:, lo:hi].clone(), None, pos[lo:hi].clone(), freqs, (1,))
+        assert torch.equal(part, out[:, lo:hi])
