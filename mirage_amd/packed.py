@@ -235,9 +235,10 @@ class PackedAttention(nn.Module):
     def freqs(self, device) -> torch.Tensor:
         """the rotary table on `device` (float64 whatever type the module's parameters are cast to)"""
         if device not in self._freqs:
-            if torch.cuda.is_current_stream_capturing():
+            if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("mirage_amd.PackedAttention: run the module once before capturing it (its rotary table is made on the first call)")
-            self._freqs[device] = rotary_frequencies(self.sections, self.theta, device)
+            with torch.inference_mode(False):                     # kept for later calls, training ones among them, whose backward pass saves it
+                self._freqs[device] = rotary_frequencies(self.sections, self.theta, device)
         return self._freqs[device]
 
     def split(self, heads):

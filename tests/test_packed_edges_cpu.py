@@ -6,6 +6,7 @@ import torch
 
 from mirage_amd import _lib as L
 from mirage_amd import kernels as K
+from mirage_amd import packed
 
 BF16 = torch.bfloat16
 
@@ -49,3 +50,12 @@ def test_attention_refuses_negative_strides(name):
     d = attn_desc(Nq=100, Nk=100, **{name: -64})
     for f in (L.lib.mrg_attn_mod_fwd, L.lib.mrg_attn_mod_bwd):
         assert f(C.byref(d), None) < 0 and "negative stride" in error()
+
+
+def test_rotary_table_made_under_inference_serves_training():
+    """the table of a module's first call is kept: made as an inference tensor, no later backward pass could save it"""
+    att = packed.PackedAttention(128, 2, sections=(8, 12, 12))
+    with torch.inference_mode():
+        table = att.freqs(torch.device("cpu"))
+        assert att.freqs(torch.device("cpu")) is table
+    assert not table.is_inference() and att.freqs(torch.device("cpu")) is table

@@ -146,3 +146,42 @@ def test_rotary_of_more_rows_than_one_dimension_of_workgroups(K):
     for lo, hi in ((0, 1000), (N // 2, N // 2 + 1000), (N - 1000, N)):
         part, _ = K.rotary_axes(q[:, lo:hi].clone(), None, pos[lo:hi].clone(), freqs, (1,))
         assert torch.equal(part, out[:, lo:hi])
+
+
+# ------------------------------------------------------------------------------------------------------------------ modules
+@pytest.fixture(scope="module")
+def P():
+    from mirage_amd import packed
+    return packed
+
+
+def encoder(P, dim=128, depth=2, heads=2, seed=0, **kw):
+    enc = P.PackedEncoder(dim, depth, heads, sections=(8, 12, 12), **kw)
+    g = torch.Generator().manual_seed(seed)
+    with torch.no_grad():
+        for p in enc.parameters():
+            p.copy_(torch.randn(p.shape, generator=g) * (p.shape[1] ** -0.5 if p.dim() == 2 else 0.3) + (0.0 if p.dim() == 2 else 0.5))
+    return enc.to(dev())
+
+
+def rows(P, K, B=2, pad=9, seed=1, dim=128):
+    """two samples in each row and padding behind them"""
+    at = torch.cat([P.grid_positions((2, 4, 5), 1), P.grid_positions((3, 3, 7), 1), torch.zeros(pad, 3, dtype=torch.int32)]).to(dev())
+    doc = torch.cat([torch.zeros(41), torch.ones(64), torch.full((pad,), -1)]).int().repeat(B, 1).to(dev())
+    return rnd(B, len(at), dim, seed=seed), at[None].repeat(B, 1, 1).contiguous(), K.ScoreMod(cap=20.0, doc_q=doc, doc_k=doc)
+
+
+def step(enc, x, pos, mod, dx, dy, gates=None):
+    h, y = enc(x, pos, mod, gates)
+    torch.autograd.backward([h, y], [dx, dy])
+    return [h.detach(), y.detach()] + [p.grad.clone() for p in enc.parameters()]
+
+
+def test_encoder_learns_after_a_first_call_under_inference(K, P):
+    x, pos, mod = rows(P, K)
+    dx, dy = rnd(*x.shape, seed=2), rnd(*x.shape, dtype=BF16, seed=3)
+    want = step(encoder(P), x, pos, mod, dx, dy)
+    enc = encoder(P)
+    with torch.inference_mode():
+        enc(x, pos, mod)
+    assert all(torch.equal(a, b) for a, b in zip(step(enc, x, pos, mod, dx, dy), want))
