@@ -233,13 +233,14 @@ class PackedAttention(nn.Module):
         self._freqs = {}
 
     def freqs(self, device) -> torch.Tensor:
-        """the rotary table on `device` (float64 whatever type the module's parameters are cast to)"""
-        if device not in self._freqs:
+        """the rotary table on `device` (float64 whatever type the module's parameters are cast to), for the sections and theta that the module has now"""
+        made_for = (device, tuple(self.sections), self.theta)
+        if made_for not in self._freqs:
             if device.type == "cuda" and torch.cuda.is_current_stream_capturing():
                 raise RuntimeError("mirage_amd.PackedAttention: run the module once before capturing it (its rotary table is made on the first call)")
             with torch.inference_mode(False):                     # kept for later calls, training ones among them, whose backward pass saves it
-                self._freqs[device] = rotary_frequencies(self.sections, self.theta, device)
-        return self._freqs[device]
+                self._freqs[made_for] = rotary_frequencies(self.sections, self.theta, device)
+        return self._freqs[made_for]
 
     def split(self, heads):
         h, k = self.num_heads, self.num_kv_heads

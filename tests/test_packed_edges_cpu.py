@@ -59,3 +59,15 @@ def test_rotary_table_made_under_inference_serves_training():
         table = att.freqs(torch.device("cpu"))
         assert att.freqs(torch.device("cpu")) is table
     assert not table.is_inference() and att.freqs(torch.device("cpu")) is table
+
+
+def test_rotary_table_follows_the_module():
+    """theta or sections changed behind the first call: a table of the new ones"""
+    att, cpu = packed.PackedAttention(128, 2, sections=(8, 12, 12)), torch.device("cpu")
+    first = att.freqs(cpu)
+    att.theta = 10_000.0
+    assert torch.equal(att.freqs(cpu), packed.rotary_frequencies((8, 12, 12), 10_000.0))
+    att.sections = (16, 16)
+    assert torch.equal(att.freqs(cpu), packed.rotary_frequencies((16, 16), 10_000.0))
+    att.sections, att.theta = (8, 12, 12), 100.0
+    assert att.freqs(cpu) is first
