@@ -149,3 +149,14 @@ def grad_buffer(p: torch.nn.Parameter) -> Optional[torch.Tensor]:
     if p.grad is None or p.grad.dtype != torch.float32 or not p.grad.is_contiguous():
         p.grad = torch.zeros_like(p, dtype=torch.float32, memory_format=torch.contiguous_format)
     return p.grad
+
+
+def follow(p: torch.nn.Parameter) -> None:
+    """The arena's bf16 copy of a parameter that was changed through torch since the last call (load_state_dict, an in-place operation).  For modules
+    that run by themselves: MIRAGEModel's forward pass refreshes its whole arena, and the optimizer's update writes the copy itself."""
+    h = getattr(p, "_mrg", None)
+    if h is None or h.arena is None or h.ptr != p.data_ptr() or h.version == p._version:
+        return
+    K.cast_bf16(p.detach(), h.bf16)
+    if not torch.cuda.is_current_stream_capturing():              # (a captured cast has not run yet)
+        h.version = p._version

@@ -18,7 +18,7 @@ from torch.autograd.function import once_differentiable
 
 from . import engine as E
 from . import kernels as K
-from .arena import grad_buffer
+from .arena import follow, grad_buffer
 from .utils import Linear, Mlp
 
 BF16, F32 = torch.bfloat16, torch.float32
@@ -181,6 +181,8 @@ class _PackedAttentionFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y16, att, pos, mod, need, anchor):
         B, N, _ = y16.shape
+        for lin in (att.qkv, att.proj):
+            follow(lin.weight)
         qkv, _, _ = E.lin_fwd(y16, att.qkv)
         heads = qkv.view(B, N, att.num_heads + 2 * att.num_kv_heads, att.head_dim)
         q, k, v = att.split(heads)
@@ -260,6 +262,8 @@ class PackedAttention(nn.Module):
 class _PackedMlpFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, y16, mlp, need, anchor):
+        for lin in (mlp.fc1, mlp.fc2):
+            follow(lin.weight)
         act, _, pre = E.lin_fwd(y16, mlp.fc1, gelu=True, save_pre=need)
         branch, _, _ = E.lin_fwd(act, mlp.fc2)
         if need:

@@ -185,3 +185,24 @@ def test_encoder_learns_after_a_first_call_under_inference(K, P):
     with torch.inference_mode():
         enc(x, pos, mod)
     assert all(torch.equal(a, b) for a, b in zip(step(enc, x, pos, mod, dx, dy), want))
+
+
+def test_encoder_sees_weights_that_change_behind_the_optimizers_arena(K, P):
+    """load_state_dict, or any change through torch, of parameters in an optimizer's arena reaches the next pass, of the encoder and of its parts"""
+    from mirage_amd import optim
+    x, pos, mod = rows(P, K)
+    dx, dy = rnd(*x.shape, seed=2), rnd(*x.shape, dtype=BF16, seed=3)
+    enc, other = encoder(P), encoder(P, seed=7)
+    opt = optim.FusedAdamW(enc, [1e-3] * 3, [0.0] * 3)
+    step(enc, x, pos, mod, dx, dy)
+    opt.step()
+    enc.load_state_dict(other.state_dict())
+    assert all(torch.equal(a, b) for a, b in zip(step(enc, x, pos, mod, dx, dy), step(other, x, pos, mod, dx, dy)))
+    opt.step()                                                     # the optimizer's own change too
+    other.load_state_dict(enc.state_dict())
+    assert all(torch.equal(a, b) for a, b in zip(step(enc, x, pos, mod, dx, dy), step(other, x, pos, mod, dx, dy)))
+    with torch.no_grad():                                          # one part by itself
+        enc.blocks[1].attn.proj.weight.mul_(-2.0)
+        other.blocks[1].attn.proj.weight.mul_(-2.0)
+        y16 = rnd(*x.shape, dtype=BF16, seed=4)
+        assert torch.equal(enc.blocks[1].attn(y16, pos, mod), other.blocks[1].attn(y16, pos, mod))
