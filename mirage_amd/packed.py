@@ -52,11 +52,18 @@ def _learns(*tensors) -> bool:
     return torch.is_grad_enabled() and any(t is not None and t.requires_grad for t in tensors)
 
 
+def _dense(g):
+    """a gradient in one piece that starts on 16 bytes (autograd also hands over slices of larger ones, dense but anywhere)"""
+    if g is None or (g.is_contiguous() and g.data_ptr() % 16 == 0):
+        return g
+    return g.clone(memory_format=torch.contiguous_format)
+
+
 def _dense_heads(g):
     """a gradient as the kernels read it: heads in one piece, rows and heads on 16 bytes (autograd also hands over broadcast and sliced ones)"""
     if g is None or (g.stride(-1) == 1 and not any(s % 8 for s in g.stride()[:-1]) and g.data_ptr() % 16 == 0):
         return g
-    return g.contiguous()
+    return g.clone(memory_format=torch.contiguous_format)
 
 
 _MOD_TENSORS = ("slopes", "pos_q", "pos_k", "doc_q", "doc_k", "prefix")
@@ -137,7 +144,7 @@ class _SeamFn(torch.autograd.Function):
         named = [("post_weight", seam.post and seam.post.weight), ("post_bias", seam.post and seam.post.bias), ("pre_weight", pre and pre.weight),
                  ("pre_bias", pre and pre.bias)] + ([("gate", seam.gate)] if gates is None else [])
         into = {n: grad_buffer(p) for n, p in named if p is not None}
-        dx, dbranch, grads = K.resid_norm_bwd(dx_new.contiguous(), None if pre is None else dy.contiguous(), x_new, branch, stats,
+        dx, dbranch, grads = K.resid_norm_bwd(_dense(dx_new), None if pre is None else _dense(dy), x_new, branch, stats,
                                               gate=gates if gates is not None else seam.gate, alpha=seam.alpha, post=_wb(seam.post), pre=_wb(pre), kind=seam.kind,
                                               eps=seam.eps, grads={n: g for n, g in into.items() if g is not None})
         if gates is not None and seam.gate is not None and seam.gate.grad is not None:
@@ -204,7 +211,7 @@ class _PackedAttentionFn(torch.autograd.Function):
         y16, qkv, pos, freqs, o, lse, o_rest, *tensors = ctx.saved_tensors
         att = ctx.att
         B, N, _ = y16.shape
-        d_o, _ = E.lin_bwd(dbranch.contiguous(), o.view(B, N, -1), att.proj)
+        d_o, _ = E.lin_bwd(_dense(dbranch), o.view(B, N, -1), att.proj)
         q, k, v = att.split(qkv.view(B, N, -1, att.head_dim))
         d_qkv = torch.empty_like(qkv)
         dq, dk, dv = att.split(d_qkv.view(B, N, -1, att.head_dim))
@@ -275,7 +282,7 @@ class _PackedMlpFn(torch.autograd.Function):
     @once_differentiable
     def backward(ctx, dbranch):
         y16, pre, act = ctx.saved_tensors
-        d_pre, _ = E.lin_bwd(dbranch.contiguous(), act, ctx.mlp.fc2, gelu_pre=pre)
+        d_pre, _ = E.lin_bwd(_dense(dbranch), act, ctx.mlp.fc2, gelu_pre=pre)
         dy, _ = E.lin_bwd(d_pre, y16, ctx.mlp.fc1)
         E.join_side_stream()
         return dy, None, None, None

@@ -206,3 +206,24 @@ def test_encoder_sees_weights_that_change_behind_the_optimizers_arena(K, P):
         other.blocks[1].attn.proj.weight.mul_(-2.0)
         y16 = rnd(*x.shape, dtype=BF16, seed=4)
         assert torch.equal(enc.blocks[1].attn(y16, pos, mod), other.blocks[1].attn(y16, pos, mod))
+
+
+def test_gradients_off_alignment(K, P):
+    """what torch.cat hands back behind a piece of odd length is dense but starts off the kernels' 16 bytes: the same gradients as from its copy"""
+    x, pos, mod = rows(P, K)
+    B, N, D = x.shape
+    att, seam, pre = P.PackedAttention(D, 2, sections=(8, 12, 12)).to(dev()), P.Seam(D).to(dev()), P.Norm(D).to(dev())
+    qkv = rnd(B, N, 6, 64, dtype=BF16, seed=5)
+
+    def grads(of):
+        leaves = [t.clone().requires_grad_(True) for t in (qkv[:, :, :2], qkv[:, :, 2:4], qkv[:, :, 4:], x, x.bfloat16())]
+        q, k, v, res, y16 = leaves
+        outs = [P.attention(q, k, v, 0.125, mod), *P.rotary(q, k, pos, att.freqs(dev()), (8, 12, 12)), att(y16, pos, mod), *seam(res, y16, pre)]
+        sum(of(o, i) for i, o in enumerate(outs)).backward()
+        return [t.grad for t in leaves] + [p.grad.clone() for m in (att, seam, pre) for p in m.parameters()]
+
+    weights = [rnd(1 + B * N * D, dtype=F32 if i == 4 else BF16, seed=20 + i) for i in range(6)]
+    behind = lambda o, i: (torch.cat([torch.ones(1, dtype=o.dtype, device=dev()), o.reshape(-1)]) * weights[i]).float().sum()
+    alone = lambda o, i: (o.reshape(-1) * weights[i][1:].clone()).float().sum()
+    got, want = grads(behind), grads(alone)
+    assert len(got) == 5 + 4 + 3 + 2 and all(torch.equal(a, b) for a, b in zip(got, want))
