@@ -170,7 +170,8 @@ class Norm(nn.Module):
 
 class Seam(nn.Module):
     """x' = alpha x + gate * post(branch), y = pre(x') in one kernel (kernels.resid_norm_fwd).  gate: a learnt row of channels (its initial value, or
-    None for no gate); forward(gates=[samples, dim]) puts one row per sample in its place."""
+    None for no gate); forward(gates=[samples, dim]) puts one row per sample in its place.  The gradients of gate and norms sum over all rows, padding
+    among them: in training it has to be finite."""
 
     def __init__(self, dim: int, kind: str = "layer", post: bool = True, gate: Optional[float] = 1.0, alpha: float = 1.0, eps: float = 1e-6):
         super().__init__()
@@ -225,7 +226,8 @@ class _PackedAttentionFn(torch.autograd.Function):
 
 class PackedAttention(nn.Module):
     """Self attention over packed rows: one projection to q (num_heads) and k, v (num_kv_heads each, shared by groups of query heads), rotary positions
-    (sections: pairs per axis; None: no rotation), attention under `mod` (kernels.ScoreMod), output projection.  bf16 in, bf16 out."""
+    (sections: pairs per axis; None: no rotation), attention under `mod` (kernels.ScoreMod), output projection.  bf16 in, bf16 out.  The projections'
+    gradients sum over all rows, padding among them: in training it has to be finite (PackedEncoder sees to that)."""
 
     def __init__(self, dim: int, num_heads: int, num_kv_heads: Optional[int] = None, sections: Optional[Sequence[int]] = None, theta: float = 100.0,
                  pairing: str = "axial", qkv_bias: bool = True):
@@ -312,7 +314,9 @@ class PackedBlock(nn.Module):
 
 class PackedEncoder(nn.Module):
     """A stack of PackedBlocks with a final norm: forward(x fp32 [B, N, dim], pos, mod, gates) -> (x, norm(x) in bf16).  `mod` carries the documents of the
-    packed rows (and whatever else its scores need); padding tokens keep their residual, and what they hold reaches no other token."""
+    packed rows (and whatever else its scores need).  Padding tokens (documents below zero) pass through the row-wise parts like any token, see nothing
+    and are seen by nothing: what they hold reaches no other token.  Weight gradients sum over all rows, so in training the values of
+    padding that are not finite are taken as zero; positions are finite everywhere."""
 
     def __init__(self, dim: int, depth: int, num_heads: int, **block):
         super().__init__()
@@ -325,6 +329,9 @@ class PackedEncoder(nn.Module):
 
     def forward(self, x, pos: Optional[torch.Tensor] = None, mod: Optional[K.ScoreMod] = None, gates=None):
         """gates: per block (attention's, mlp's) rows per sample, or None (the blocks' learnt channel gates)"""
+        if mod is not None and mod.doc_q is not None and torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters())):
+            doc = mod.doc_q if mod.doc_k is mod.doc_q else torch.maximum(mod.doc_q, mod.doc_k)       # (a token that only asks or only answers is none)
+            x = torch.where((doc < 0).unsqueeze(-1), torch.nan_to_num(x, 0.0, 0.0, 0.0), x)
         x, y16 = self._first(x, x, self.blocks[0].norm1)
         for i, blk in enumerate(self.blocks):
             following = self.blocks[i + 1].norm1 if i + 1 < len(self.blocks) else self.norm

@@ -174,7 +174,7 @@ def rows(P, K, B=2, pad=9, seed=1, dim=128):
 def step(enc, x, pos, mod, dx, dy, gates=None):
     h, y = enc(x, pos, mod, gates)
     torch.autograd.backward([h, y], [dx, dy])
-    return [h.detach(), y.detach()] + [p.grad.clone() for p in enc.parameters()]
+    return [h.detach(), y.detach()] + [p.grad.clone() for p in enc.parameters() if p.grad is not None]      # (learnt gates behind `gates`: none)
 
 
 def test_encoder_learns_after_a_first_call_under_inference(K, P):
@@ -227,3 +227,38 @@ def test_gradients_off_alignment(K, P):
     alone = lambda o, i: (o.reshape(-1) * weights[i][1:].clone()).float().sum()
     got, want = grads(behind), grads(alone)
     assert len(got) == 5 + 4 + 3 + 2 and all(torch.equal(a, b) for a, b in zip(got, want))
+
+
+@pytest.mark.parametrize("junk", [float("nan"), float("inf"), -float("inf")])
+@pytest.mark.parametrize("per_sample", [False, True])
+def test_encoder_learns_beside_padding_that_is_not_finite(K, P, junk, per_sample):
+    """weight gradients sum over every row of the batch, and zero times NaN is NaN: such padding learns like padding of zeros"""
+    x, pos, mod = rows(P, K)
+    pad = mod.doc_q < 0
+    gates = [tuple(0.5 * rnd(2, 128, seed=10 * i + j) for j in range(2)) for i in range(2)] if per_sample else None
+    dx, dy = rnd(*x.shape, seed=2), rnd(*x.shape, dtype=BF16, seed=3)
+    dx[pad], dy[pad] = 0, 0                                        # a loss over the samples' tokens
+
+    def learn(fill):
+        t = x.clone()
+        t[pad] = fill
+        t.requires_grad_(True)
+        return step(encoder(P), t, pos, mod, dx, dy, gates) + [t.grad]
+
+    got, want = learn(junk), learn(0.0)
+    assert all(torch.equal(a, b) for a, b in zip(got, want)) and all(bool(torch.isfinite(t).all()) for t in got)
+    finite = learn(3.0)                                            # and finite padding is left alone: its rows differ, nothing that is learnt does
+    assert not torch.equal(finite[0][pad], want[0][pad]) and torch.equal(finite[0][~pad], want[0][~pad])
+    assert all(torch.equal(a, b) for a, b in zip(finite[2:-1], want[2:-1])) and torch.equal(finite[-1][~pad], want[-1][~pad])
+
+
+def test_visible_values_that_are_not_finite_still_show(K, P):
+    """only padding is replaced: a NaN in a sample's own token reaches that sample, and the gradients"""
+    x, pos, mod = rows(P, K)
+    x[0, 5, 7] = float("nan")
+    asks = mod.doc_q.clone()
+    asks[0, 5] = -1                                                # a token that asks nothing, but is seen
+    out = step(encoder(P), x, pos, K.ScoreMod(doc_q=asks, doc_k=mod.doc_k), torch.ones_like(x), torch.ones_like(x, dtype=BF16))
+    assert bool(torch.isnan(out[0][0, :41]).all()) and bool(torch.isfinite(out[0][0, 41:]).all()) and bool(torch.isnan(out[2]).any())
+    out = step(encoder(P), x, pos, mod, torch.ones_like(x), torch.ones_like(x, dtype=BF16))
+    assert bool(torch.isnan(out[0][0, :41]).all()) and bool(torch.isfinite(out[0][0, 41:]).all()) and bool(torch.isnan(out[2]).any())
