@@ -260,6 +260,8 @@ class PackedAttention(nn.Module):
     def forward(self, y16, pos: Optional[torch.Tensor] = None, mod: Optional[K.ScoreMod] = None):
         if y16.dtype != BF16 or y16.dim() != 3 or not y16.is_contiguous():
             raise ValueError(f"mirage_amd.PackedAttention: needs contiguous bf16 [B, N, dim] (a norm's output), got {y16.dtype} {tuple(y16.shape)}")
+        if y16.numel() == 0:
+            raise ValueError(f"mirage_amd.PackedAttention: {tuple(y16.shape)} holds no tokens (the projections' products take at least one)")
         if (pos is None) != (self.sections is None):
             raise ValueError("mirage_amd.PackedAttention: positions go with rotary sections")
         if y16.is_cuda and y16.device.index != torch.cuda.current_device():

@@ -71,3 +71,10 @@ def test_rotary_table_follows_the_module():
     assert torch.equal(att.freqs(cpu), packed.rotary_frequencies((16, 16), 10_000.0))
     att.sections, att.theta = (8, 12, 12), 100.0
     assert att.freqs(cpu) is first
+
+
+def test_attention_module_refuses_a_batch_without_tokens():
+    att = packed.PackedAttention(128, 2)
+    for shape in ((0, 5, 128), (2, 0, 128)):
+        with pytest.raises(ValueError, match="no tokens"):
+            att(torch.zeros(shape, dtype=BF16))
