@@ -235,6 +235,8 @@ int mrg_resid_norm_bwd(const mrg_resid_norm_desc* d, hipStream_t stream);
  * Softmax attention whose scores are modified, csrc/attention_mod.hip (next to mrg_attn_fwd / bwd, which keep the unmodified short rows):
  *   s = scale q.k;  cap > 0: s = cap tanh(s / cap) (both factors 1e-30 to 1e30);  slopes: s -= slopes[h] sum_a |pos_q[b, i, a] - pos_k[b, j, a]|
  *   visible (i, j):  doc_q[b, i] == doc_k[b, j] >= 0 (documents given)  and  j < max(prefix[b], i + Nk - Nq + 1) (causal)
+ * The prefix counts tokens of the packed row, from its start, whatever documents they belong to.  Scores are fp32: forward up to 2^30 in size,
+ * backward p is formed from lse and off by |lse| 2^-23 of its value.
  * A row that sees nothing gives o = 0, lse = -inf and no gradient.  bf16, head_dim 32 or 64; H query heads share Hk key / value heads (H a
  * multiple of Hk: head h reads h / (H / Hk)).  *_bs / *_rs / *_hs: batch, row and head strides in elements.  Rows whose document is negative
  * see nothing and take part in no sum; values behind a mask do not reach the result even when they are not finite; a row

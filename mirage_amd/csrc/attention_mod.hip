@@ -20,15 +20,19 @@
 // row of 8192 in twelve documents, 16 heads: backward 240 -> 200).
 //
 // Sums, maxima, lse and all products accumulate in fp32.  p is rounded to bf16 as an operand of the second product (at most 2^-8 of each weight,
-// averaging over the row; its sum is taken before the rounding).  ds goes into its product as two bf16 parts, and sum(do o) takes o with what its
-// rounding left out: dq and dk are then 0.0017 to 0.0024 from the 64-bit gradient, where 0.0017 is the rounding of the result itself.  In one part
-// they were 0.0024 to 0.0031 away (the terms of a sum that nearly cancel are rounded apart) for 8 to 18 % less time of the backward pass.
+// averaging over what is summed; its sum is taken before the rounding): o and dv are 0.0019 to 0.0026 from the 64-bit result, the most where few
+// terms count, where 0.0017 is the rounding of the result itself.  ds goes into its product as two bf16 parts, and sum(do o) takes o with what its
+// rounding left out: dq and dk are then 0.0017 to 0.0024 from the 64-bit gradient.  In one part they were 0.0024 to 0.0031 away (the terms of a sum
+// that nearly cancel are rounded apart) for 8 to 18 % less time of the backward pass.  Scores are fp32: forward takes them up to 2^30 in size (the
+// exponent's reference point is rounded like them), backward forms p from lse, off by |lse| 2^-23 of its value
+// (2^-9 at scores of 2^14).
 //
 // What bounds it: the arithmetic between the products.  At 16 heads of 4095 tokens behind a prefix a score costs 7 vector operations forward, 10 for
-// dq, 11 for dk and dv; the vector pipe is busy 66 % and the matrix pipe 32 % of the forward pass (98 us, 700 TFLOP/s), 61 / 44 % for dq and
-// 44 / 38 % for dk and dv (370 us together with their joining, 830 TFLOP/s counting the products that are made).  A distance of two axes takes
-// the forward pass to 16 operations, padded rows counted (64 x 12 heads of 257 tokens, 60 us: 57 / 13 %).  One query of many keys is bound by
-// HBM: 16 x 12 heads of 4097 keys in 45.6 us, 4.4 TB/s.
+// dq, 11 for dk and dv; the vector pipe is busy 66 % and the matrix pipe 32 % of the forward pass (100 us, 690 TFLOP/s), 61 / 44 % for dq and
+// 44 / 38 % for dk and dv (375 us together with their joining, 820 TFLOP/s counting the products that are made).  A distance of two axes takes
+// the forward pass to 16 operations, padded rows counted (64 x 12 heads of 257 tokens, 52 us, 61 with lse and o's remainder: 55 / 13 %).  One query
+// of many keys is bound by HBM: 16 x 12 heads of 4097 keys in 43 us, 4.7 TB/s; query heads that share keys read them again, out of L2 (16 over 4
+// heads: 41.5 us for 67 MB of keys and values).
 //
 // Values that are not finite behind a mask: 0 * inf would reach the products, so in partial tiles the rows of the second product's left
 // operand that hold such values are replaced by zeros in LDS and noted; a row that SEES one of them is NaN in full.
@@ -384,9 +388,9 @@ __device__ __forceinline__ void store_o(const ModArgs& a, long at, const float4 
 
 // ================================================ forward ===============================================
 // NW waves of 32 queries.  NW = 1 serves up to 32 queries (a pooled or a single new token): every workgroup is one wave, and the keys are
-// split over many of them.  NW = 4 otherwise: two waves would stage every tile for half as many queries (83 -> 102 us on 16 heads of 8192 packed
-// tokens).  Three waves per SIMD (98 us in three, 99 in two, 105 in four for 16 heads
-// of 4095 tokens behind a prefix); with a distance bias the registers are those of two (64 x 12 heads of 257 tokens 61 us, 63 when held to three).
+// split over many of them.  NW = 4 otherwise: two waves would stage every tile for half as many queries (a fifth slower on 16 heads of 8192 packed
+// tokens).  Three waves per SIMD (16 heads of 4095 tokens behind a prefix: 100 us in three and in two, 107 in four); with a distance bias the
+// registers are those of two (64 x 12 heads of 257 tokens with lse: 61 us, 64 when held to three; 16 heads of 8192 packed tokens 73 and 72).
 template <int HD, int NW, int CAP, bool BIAS>
 __global__ __launch_bounds__(64 * NW, BIAS ? 2 : 3) void attn_mod_fwd_kernel(const ModArgs a) {
     constexpr int KS = HD / 16, DJ = HD / 32, NT = 64 * NW, TB = TT * HD * 2;
@@ -633,8 +637,8 @@ __global__ __launch_bounds__(256) void attn_mod_join_kernel(const ModArgs a) {
 //   OWN_K: lane = key, tiles of queries: S = Q K^T,  dP = dO V^T,  dV^T += dO^T P, dK^T += Q^T dS         (10 hd)
 // Scores and dP are formed twice (4 hd of the 18), which costs less than the atomics or the traffic of dq partials that one kernel would need: a
 // tile of 64 keys would add 64 KiB of fp32 to HBM for every 128 queries.  Four waves of 32 rows; dq runs at three waves per SIMD
-// (375 us the pass above in two), dk / dv and a distance bias at two: in three they spill (370 -> 512 us; 16 heads of 8192 packed tokens with a
-// distance 200 -> 299).
+// (the pass above 375 us, 378 in two; 8 x 12 heads of 1024 in five documents, capped, 110 and 115), dk / dv and a distance bias at two: in three they
+// spill (375 -> 509 us; 16 heads of 8192 packed tokens with a distance 200 -> 295).
 // X, Y: the staged matrices (K, V or Q, dO); own fragments: (Q, dO) or (K, V).  OWN_Q also forms sum(do o), which OWN_K reads.
 template <int HD, bool OWN_Q, int CAP, bool BIAS>
 __global__ __launch_bounds__(256, OWN_Q && !BIAS ? 3 : 2) void attn_mod_bwd_kernel(const ModArgs a) {
@@ -1032,8 +1036,9 @@ void doc_tables(const mrg_attn_mod_desc* d, const Plan& p, ModArgs& a, bool back
 // Do the heads' blocks start side by side?  Where blocks differ in length the short ones then fill the end, and a CU's workgroups are not all of one
 // length: under an order of the keys or of the blocks and with documents (one head after the other left a quarter of the chip idle behind the last
 // head's long blocks; 4 x 12 heads of 1024 tokens in five documents 32 -> 28 us, 32 x 12 of them 113 -> 105), and where the last block holds one
-// wave's rows or fewer, while what a die's heads read stays in its 4 MB of L2 (64 x 12 heads of 129 tokens 29 -> 26 us; 16 x 12 of 1025, 6 MB
-// for a die, 93 -> 96).  Split rows stay together.
+// wave's rows or fewer, while what a die's heads read stays in its 4 MB of L2 (64 x 12 heads of 129 / 144 / 160 tokens: forward 30.3 -> 26.9,
+// 29.7 -> 26.2, 30.0 -> 27.0 us, backward 78 -> 69, 78 -> 71, 79 -> 73; behind it two waves' rows gain less, 161 tokens 31 -> 29 and 84 -> 80, and
+// where a die reads more they lose: 257 / 272 / 288 tokens, 6 MB, 48.7 -> 50.4, 51.2, 51.8; 16 x 12 heads of 1025 93 -> 97).  Split rows stay together.
 bool start_abreast(const ModArgs& a, int rows, int heads, long head_bytes) {
     if (a.causal) return true;
     if (a.splits > 1) return false;

@@ -938,7 +938,8 @@ class ScoreMod:
     cap            s = cap tanh(s / cap), 1e-30 <= cap < 1e30; 0: none
     slopes         fp32 [heads], with pos_q [B, Nq, axes] and pos_k [B, Nk, axes] (fp32, 1 to 3 axes): s -= slopes[h] sum_a |pos_q - pos_k|
     doc_q, doc_k   int32 [B, Nq], [B, Nk]: a query sees the keys of its own document; negative: padding, sees and is seen by nothing
-    causal         query i sees keys j <= i + Nk - Nq (the last query sees all); prefix int32 [B]: and keys j < prefix in any case
+    causal         query i sees keys j <= i + Nk - Nq (the last query sees all); prefix int32 [B]: and keys j < prefix in any case.  One prefix per
+                   batch row, counted from the row's start: with documents only samples that begin inside it have a visible prefix
     slopes, positions and masks are constants: they get no gradient."""
     __slots__ = ("cap", "slopes", "pos_q", "pos_k", "doc_q", "doc_k", "causal", "prefix")
 
@@ -1014,7 +1015,8 @@ def _attn_mod_ws(d, backward: int, dev):
 def attn_mod_fwd(q: torch.Tensor, k: torch.Tensor, v: torch.Tensor, scale: float, mod: Optional[ScoreMod] = None, need_lse: bool = True):
     """softmax(modified scores) v (mrg_attn_mod_fwd): q bf16 [B, Nq, H, hd], k / v bf16 [B, Nk, Hk, hd], H a multiple of Hk, hd 32 or 64, any batch / row /
     head strides that are multiples of 8 elements.  Returns (o bf16 [B, Nq, H, hd], AttnSaved for the backward pass, or None without need_lse); a row that
-    sees nothing gives o = 0 and lse = -inf; what a mask hides may hold anything, and a row that sees a value that is not finite may be NaN in full."""
+    sees nothing gives o = 0 and lse = -inf; what a mask hides may hold anything, and a row that sees a value that is not finite may be NaN in full.
+    Scores are fp32, up to 2^30 in size (the backward pass' weights are off by |lse| 2^-23 of their value)."""
     d, dev = _attn_mod_desc(q, k, v, scale, mod)
     o = torch.empty_like(q, memory_format=_DENSE)
     d.o = o.data_ptr()

@@ -262,3 +262,21 @@ def test_visible_values_that_are_not_finite_still_show(K, P):
     assert bool(torch.isnan(out[0][0, :41]).all()) and bool(torch.isfinite(out[0][0, 41:]).all()) and bool(torch.isnan(out[2]).any())
     out = step(encoder(P), x, pos, mod, torch.ones_like(x), torch.ones_like(x, dtype=BF16))
     assert bool(torch.isnan(out[0][0, :41]).all()) and bool(torch.isfinite(out[0][0, 41:]).all()) and bool(torch.isnan(out[2]).any())
+
+
+def test_scores_up_to_their_limit(K):
+    """scores 2^23 apart up to 99 2^23 (exact in fp32): each row's largest one takes all"""
+    N = 100
+    q, k = (torch.zeros(1, N, 1, 64, dtype=BF16, device=dev()) for _ in range(2))
+    q[..., 0] = 2.0 ** 15
+    q[0, 50:, 0, 0] = -(2.0 ** 15)                                 # these rows want the smallest
+    order = torch.randperm(N, generator=torch.Generator().manual_seed(1)).to(dev())
+    k[0, :, 0, 0] = order.to(BF16)
+    v = rnd(1, N, 1, 64, dtype=BF16, seed=2)
+    for scale, shift in ((256.0, 0.0), (256.0, 1.0)):              # the second: every score of the first rows is far from zero
+        k[0, :, 0, 0] = (order + shift * 28).to(BF16)
+        o, saved = K.attn_mod_fwd(q, k, v, scale)
+        best = torch.where(torch.arange(N, device=dev()) < 50, order.argmax(), order.argmin())
+        want, top = v[:, best].double(), (q[0, :, 0, 0].double() * k[0, best, 0, 0].double() * scale)
+        within(o, want, want.abs() * 2 * HALF16, "o")              # p and the result rounded
+        within(saved.lse[0, 0], top, top.abs() * 4 * HALF32 + 1e-6, "lse")
