@@ -21,11 +21,13 @@
 //
 // Sums, maxima, lse and all products accumulate in fp32.  p is rounded to bf16 as an operand of the second product (at most 2^-8 of each weight,
 // averaging over what is summed; its sum is taken before the rounding): o and dv are 0.0019 to 0.0026 from the 64-bit result, the most where few
-// terms count, where 0.0017 is the rounding of the result itself.  ds goes into its product as two bf16 parts, and sum(do o) takes o with what its
-// rounding left out: dq and dk are then 0.0017 to 0.0024 from the 64-bit gradient.  In one part they were 0.0024 to 0.0031 away (the terms of a sum
-// that nearly cancel are rounded apart) for 8 to 18 % less time of the backward pass.  Scores are fp32: forward takes them up to 2^30 in size (the
-// exponent's reference point is rounded like them), backward forms p from lse, off by |lse| 2^-23 of its value
-// (2^-9 at scores of 2^14).
+// terms count, where 0.0017 is the rounding of the result itself.  (In two parts, like ds, all four results are at 0.0017, for 4 to 15 % more time
+// of a step: 16 over 4 heads of 4095 tokens behind a prefix forward 100 -> 134 us, backward 376 -> 412; 8 x 12 heads of 1024 in five documents 41 ->
+// 44 and 110 -> 114; 16 heads of 8192 with a distance 74 -> 82 and 200 -> 212; one query of 4097 keys 45 -> 47.)  ds goes into its product as two
+// bf16 parts, and sum(do o) takes o with what its rounding left out: dq and dk are then 0.0017 to 0.0024 from the 64-bit gradient.  In one part they
+// were 0.0024 to 0.0031 away (the terms of a sum that nearly cancel are rounded apart) for 8 to 18 % less time of the backward pass.  Scores are
+// fp32: forward takes them up to 2^30 in size (the exponent's reference point is rounded like them), backward forms p from lse, off by |lse| 2^-23
+// of its value (2^-9 at scores of 2^14).
 //
 // What bounds it: the arithmetic between the products.  At 16 heads of 4095 tokens behind a prefix a score costs 7 vector operations forward, 10 for
 // dq, 11 for dk and dv; the vector pipe is busy 66 % and the matrix pipe 32 % of the forward pass (100 us, 690 TFLOP/s), 61 / 44 % for dq and
