@@ -80,6 +80,15 @@ def _mod_whole(plain, tensors) -> Optional[K.ScoreMod]:
     return None if plain is None else K.ScoreMod(plain[0], causal=plain[1], **dict(zip(_MOD_TENSORS, tensors)))
 
 
+def _finite_padding(x, mod: Optional[K.ScoreMod]):
+    """x [B, N, dim] with zeros for padding's values that are not finite (documents that do not fit x are the attention's to refuse)"""
+    docs = () if mod is None or mod.doc_q is None else (mod.doc_q, mod.doc_k)
+    if not docs or any(d.shape != x.shape[:2] or d.device != x.device for d in docs):
+        return x
+    doc = docs[0] if docs[0] is docs[1] else torch.maximum(*docs)      # a token that only asks or only answers is no padding
+    return torch.where((doc < 0).unsqueeze(-1), torch.nan_to_num(x, 0.0, 0.0, 0.0), x)
+
+
 class _RotaryFn(torch.autograd.Function):
     @staticmethod
     def forward(ctx, q, k, pos, freqs, sections, pairing):
@@ -331,9 +340,8 @@ class PackedEncoder(nn.Module):
 
     def forward(self, x, pos: Optional[torch.Tensor] = None, mod: Optional[K.ScoreMod] = None, gates=None):
         """gates: per block (attention's, mlp's) rows per sample, or None (the blocks' learnt channel gates)"""
-        if mod is not None and mod.doc_q is not None and torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters())):
-            doc = mod.doc_q if mod.doc_k is mod.doc_q else torch.maximum(mod.doc_q, mod.doc_k)       # (a token that only asks or only answers is none)
-            x = torch.where((doc < 0).unsqueeze(-1), torch.nan_to_num(x, 0.0, 0.0, 0.0), x)
+        if torch.is_grad_enabled() and (x.requires_grad or any(p.requires_grad for p in self.parameters())):
+            x = _finite_padding(x, mod)
         x, y16 = self._first(x, x, self.blocks[0].norm1)
         for i, blk in enumerate(self.blocks):
             following = self.blocks[i + 1].norm1 if i + 1 < len(self.blocks) else self.norm

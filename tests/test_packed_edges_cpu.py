@@ -78,3 +78,20 @@ def test_attention_module_refuses_a_batch_without_tokens():
     for shape in ((0, 5, 128), (2, 0, 128)):
         with pytest.raises(ValueError, match="no tokens"):
             att(torch.zeros(shape, dtype=BF16))
+
+
+def test_padding_that_is_not_finite():
+    x = torch.randn(2, 5, 8)
+    doc = torch.tensor([[0, 0, 1, -1, -1], [0, -3, 1, 1, -1]], dtype=torch.int32)
+    pad = doc < 0
+    x[0, 3], x[0, 4, 2], x[1, 1, 0], x[0, 0, 1] = float("nan"), float("inf"), -float("inf"), float("nan")
+    x.requires_grad_(True)
+    z = packed._finite_padding(x, K.ScoreMod(doc_q=doc, doc_k=doc))
+    want = torch.where(pad[..., None] & ~torch.isfinite(x), torch.zeros(()), x)
+    assert torch.equal(z.nan_to_num(7.0), want.nan_to_num(7.0)) and bool(torch.isnan(z[0, 0, 1]))
+    z.backward(torch.ones_like(z))
+    assert torch.equal(x.grad, (~pad[..., None] | torch.isfinite(x)).float())
+    asks = torch.where(pad, doc, -1)                              # tokens that ask nothing but are seen
+    assert torch.equal(packed._finite_padding(x, K.ScoreMod(doc_q=asks, doc_k=doc)).nan_to_num(7.0), want.nan_to_num(7.0))
+    for mod in (None, K.ScoreMod(), K.ScoreMod(doc_q=doc[:, :4], doc_k=doc[:, :4]), K.ScoreMod(doc_q=doc, doc_k=doc[:1])):
+        assert packed._finite_padding(x, mod) is x

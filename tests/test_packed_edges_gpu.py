@@ -280,3 +280,12 @@ def test_scores_up_to_their_limit(K):
         want, top = v[:, best].double(), (q[0, :, 0, 0].double() * k[0, best, 0, 0].double() * scale)
         within(o, want, want.abs() * 2 * HALF16, "o")              # p and the result rounded
         within(saved.lse[0, 0], top, top.abs() * 4 * HALF32 + 1e-6, "lse")
+
+
+def test_encoder_in_training_refuses_documents_that_do_not_fit(K, P):
+    x, pos, mod = rows(P, K)
+    for doc in (mod.doc_q[:, :-1].contiguous(), mod.doc_q[:1], mod.doc_q.t().contiguous()):
+        with pytest.raises(ValueError, match="ScoreMod doc_q must have shape"):
+            encoder(P)(x, pos, K.ScoreMod(doc_q=doc, doc_k=doc))
+    with pytest.raises(RuntimeError, match="GPU"):
+        encoder(P)(x, pos, K.ScoreMod(doc_q=mod.doc_q.cpu(), doc_k=mod.doc_k.cpu()))
